@@ -62,7 +62,8 @@ typedef enum hogatt_status {
     HOGATT_ERR_CUDA = -8,               /* a CUDA runtime call failed; see hogatt_last_cuda_error() */
     HOGATT_ERR_BAD_KERNEL_CHOICE = -9,
     HOGATT_ERR_TOO_LARGE = -10,
-    HOGATT_ERR_EXCEEDS_STATIC_SCRATCH = -11  /* hogatt_fused_launch_static: needs more than HOGATT_STATIC_SCRATCH_BYTES */
+    HOGATT_ERR_EXCEEDS_STATIC_SCRATCH = -11, /* hogatt_fused_launch_static: needs more than HOGATT_STATIC_SCRATCH_BYTES */
+    HOGATT_ERR_BAD_UNIT = -12           /* a 4-bit cache's unit is not a power of two between 2^-64 and 2^64 */
 } hogatt_status;
 
 /* Which device code runs.  AUTO picks the tensor-core kernel for f16/bf16 with E == Ev in {64, 128}
@@ -319,6 +320,160 @@ int hogatt_copy_to_blocks_launch(const void* key_states, const void* value_state
                                  const int32_t* block_table, const int32_t* seq_lengths, int32_t B, int32_t Hkv,
                                  int32_t S_new, int32_t E, int32_t Ev, int32_t block_size, int32_t max_blocks,
                                  int32_t dtype, hogatt_stream_t stream);
+
+/* ---- a paged cache in 4 bits --------------------------------------------------------------------------- */
+
+/*
+ * The layout of the paged caches with rows of E/2 + E/16 bytes instead of 2 E:
+ *   codes  uint8 [num_blocks, Hkv, block_size, E/2]    two e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) per byte,
+ *                                                      the even channel in the low half
+ *   scales e4m3  [num_blocks, Hkv, block_size, E/16]   one per 16 consecutive channels
+ *   value[e] = e2m1(code[e]) * scale[e / 16] * unit
+ * `unit` is a power of two between 2^-64 and 2^64 that the caller keeps for the cache's keys and for its values (HOGATT_ERR_BAD_UNIT
+ * otherwise): it moves the range of the scales, 2^-9 to 448, to where the numbers are.  1 suits numbers between 0.1 and 2,688; groups
+ * whose largest magnitude is below 6 * 2^-6 * unit lose precision, below 3 * 2^-9 * unit they are stored as zeros.
+ * Writing: with a = the group's largest magnitude, scale = e4m3(a / (6 unit)), at most 448; code = e2m1(x / (scale unit)), at most 6;
+ * all roundings to the nearest, ties to even, divisions in fp32.  A group that holds an infinity or a NaN gets the scale NaN, and every
+ * row that sees it is NaN: in the channels of that group (values) or in all (keys).
+ * E and Ev are multiples of 16, at most 256.  All pointers are device pointers unless marked; caches and scales start on 16-byte
+ * boundaries.  A page number outside [0, num_blocks), or a position behind the block table, names no page: rows written there are
+ * dropped, keys there are seen by nobody, rows read from there are NaN, and 1024 is ORed into *device_status (which may be NULL).
+ */
+
+/*
+ * Attention over such a cache: hogatt_paged_sdpa_launch with key_cache / value_cache as the codes, and num_blocks given.
+ * `kernel`: AUTO or FMA (CUDA cores).  f32 / f16 / bf16 queries and outputs; E <= 256, Ev in {32, 64, 128, 256}.
+ */
+typedef struct hogatt_paged_q4_problem {
+    hogatt_paged_problem paged;
+    const void* key_scales;
+    const void* value_scales;
+    float key_unit, value_unit;
+} hogatt_paged_q4_problem;
+
+size_t hogatt_paged_q4_workspace_bytes(const hogatt_paged_q4_problem* p);
+int hogatt_paged_q4_sdpa_launch(const hogatt_paged_q4_problem* p, hogatt_stream_t stream);
+
+/*
+ * Append to such a cache: row t of sequence b goes to position seq_lengths[b] + t.
+ *   fixed layout  (cu_seqlens == NULL): element (b, h, t, e) of the source at keys + b*ks[0] + h*ks[1] + t*ks[2] + e, t < S
+ *   packed layout (cu_seqlens != NULL): S tokens in all, token i at keys + h*ks[1] + i*ks[2]; those of sequence b are
+ *                                       cu_seqlens[b] .. cu_seqlens[b + 1] - 1, tokens behind the last sequence stay out
+ * new_rows[b] (or NULL): rows t >= new_rows[b] of sequence b stay out.  Two rows for one position: refused by nobody, either is stored.
+ */
+typedef struct hogatt_q4_append {
+    int32_t B, Hkv, S, E, Ev, block_size, max_blocks, num_blocks, dtype;
+    float   key_unit, value_unit;
+    const void* keys;
+    int64_t     key_strides[3];
+    const void* values;
+    int64_t     value_strides[3];
+    void* key_cache;
+    void* value_cache;
+    void* key_scales;
+    void* value_scales;
+    const int32_t* block_table;      /* [B, max_blocks] */
+    const int32_t* seq_lengths;      /* [B] */
+    const int32_t* cu_seqlens;       /* [B + 1] or NULL */
+    const int32_t* new_rows;         /* [B] or NULL */
+    int32_t* device_status;
+} hogatt_q4_append;
+
+int hogatt_copy_to_blocks_q4_launch(const hogatt_q4_append* p, hogatt_stream_t stream);
+
+/*
+ * The way back: rows first_rows[b] .. first_rows[b] + S - 1 of every sequence as numbers, keys [B, Hkv, S, E] and values [B, Hkv, S, Ev],
+ * rounded to `dtype` (exact in every type while the unit keeps them in its range).
+ */
+typedef struct hogatt_q4_read {
+    int32_t B, Hkv, S, E, Ev, block_size, max_blocks, num_blocks, dtype;
+    float   key_unit, value_unit;
+    void* keys;
+    void* values;
+    const void* key_cache;
+    const void* value_cache;
+    const void* key_scales;
+    const void* value_scales;
+    const int32_t* block_table;      /* [B, max_blocks] */
+    const int32_t* first_rows;       /* [B] */
+    int32_t* device_status;
+} hogatt_q4_read;
+
+int hogatt_copy_from_blocks_q4_launch(const hogatt_q4_read* p, hogatt_stream_t stream);
+
+/* ---- the pages of a paged cache ------------------------------------------------------------------------- */
+
+/*
+ * Who holds which page, on the device.  refs[p] counts the block-table entries that name page p; a caller that keeps a page without a
+ * table entry (a prefix for later) adds one.  A page with refs[p] == 0 is free.  A row of a block table names the pages of its
+ * sequence in order, -1 behind the last.  Everything here works for caches of any type: the `caches` are all tensors whose first axis is the
+ * page (keys, values and scales of every layer), `block_bytes` what one page of each takes.  Host arrays.
+ */
+typedef struct hogatt_block_tensors {
+    int32_t count;
+    void* const*   data;             /* host array of device pointers */
+    const int64_t* block_bytes;      /* host array */
+} hogatt_block_tensors;
+
+#define HOGATT_MAX_BLOCK_ROWS 65536
+
+/*
+ * One step of a batch: fork, reorder, free, and room for the tokens that come next.
+ *   1. Row w takes over row source[w] of the old table (source == NULL: row w stays where it is; negative: row w is empty): its length and
+ *      the pages that the length fills.  A row of the old table that nobody takes over is freed, one that several take over is
+ *      forked: they share its pages.  Pages that a row held beyond its length go back.
+ *   2. Rows get the pages for new_tokens[w] (NULL: none) tokens behind their length, lowest free page first, in row order.  A row whose last
+ *      page is partly filled and shared gets a page of its own with the old one's contents, in all caches, unless it is the last that
+ *      still holds it.
+ *   room[w] = new_tokens[w] if the row has its pages, else 0 (what hogatt_q4_append takes as new_rows).  A row that does not fit the table gets
+ *      none (2048 in *device_status; so does a source row that does not exist).  Rows are served in order until one finds too few free
+ *      pages (512): it and all rows behind it get none, and their tables stay as step 1 leaves them.
+ * Writes refs_out, table_out [rows_out, max_blocks], lengths_out [rows_out] = the rows' lengths without the new tokens, room [rows_out].  Outputs
+ * may be the inputs' buffers (refs always; table and lengths without a source).  Enqueues one kernel, one more per 128 caches when
+ * there are new tokens.
+ */
+typedef struct hogatt_step_blocks {
+    int32_t num_blocks, block_size, max_blocks, rows_in, rows_out;
+    const int32_t* refs_in;          /* [num_blocks] */
+    const int32_t* table_in;         /* [rows_in, max_blocks] */
+    const int32_t* lengths_in;       /* [rows_in] */
+    const int32_t* source;           /* [rows_out] or NULL */
+    const int32_t* new_tokens;       /* [rows_out] or NULL */
+    int32_t* refs_out;
+    int32_t* table_out;
+    int32_t* lengths_out;
+    int32_t* room;
+    hogatt_block_tensors caches;
+    void*   workspace;               /* >= hogatt_step_blocks_workspace_bytes(rows_out), 256-byte aligned */
+    size_t  workspace_bytes;
+    int32_t* device_status;
+} hogatt_step_blocks;
+
+size_t hogatt_step_blocks_workspace_bytes(int32_t rows_out);
+int hogatt_step_blocks_launch(const hogatt_step_blocks* p, hogatt_stream_t stream);
+
+/*
+ * Moves the n pages that are held to places 0 .. n - 1: the k-th held page behind them to the k-th free place among them, its contents in all
+ * caches with it.  moved[p] = the new number of page p (its own if it stays), -1 for a free one; refs and table follow.  A table entry
+ * that names a free page or none there is becomes -1 (the latter and entries outside the cache: 1024 in *device_status; -1 stays -1).
+ * Outputs may be the inputs' buffers.
+ */
+typedef struct hogatt_compact_blocks {
+    int32_t num_blocks;
+    int64_t table_entries;           /* of the whole block table, 0: none */
+    const int32_t* refs_in;          /* [num_blocks] */
+    const int32_t* table_in;
+    int32_t* refs_out;
+    int32_t* table_out;
+    int32_t* moved;                  /* [num_blocks] */
+    hogatt_block_tensors caches;
+    void*   workspace;               /* >= hogatt_compact_blocks_workspace_bytes(num_blocks), 256-byte aligned */
+    size_t  workspace_bytes;
+    int32_t* device_status;
+} hogatt_compact_blocks;
+
+size_t hogatt_compact_blocks_workspace_bytes(int32_t num_blocks);
+int hogatt_compact_blocks_launch(const hogatt_compact_blocks* p, hogatt_stream_t stream);
 
 /* ---- the steps either side of the attention op in a decode step ------------------------------------- */
 

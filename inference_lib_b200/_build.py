@@ -62,7 +62,7 @@ def build_cabi(force: bool = False, verbose: bool = False, ptxas_info: bool = Fa
     srcs = cabi_sources()
     if force or _stale(CABI_SO, srcs):
         units = [s for s in srcs if s.endswith(".cu")]
-        cmd = [nvcc_path()] + NVCC_FLAGS + (["-Xptxas", "-v"] if ptxas_info else []) + ["-shared", "-o", CABI_SO] + units
+        cmd = [nvcc_path()] + NVCC_FLAGS + ["--threads", str(len(units))] + (["-Xptxas", "-v"] if ptxas_info else []) + ["-shared", "-o", CABI_SO] + units
         _run(cmd, "libhogatt_b200.so", verbose or ptxas_info)
     return CABI_SO
 

@@ -20,7 +20,10 @@ MAX_FRAGMENTS = 128
 EXPORTS = ["hogatt_abi_version", "hogatt_status_string", "hogatt_last_cuda_error", "hogatt_workspace_bytes",
            "hogatt_sdpa_launch", "hogatt_fused_launch", "hogatt_fused_launch_static", "hogatt_fused_launch_gather", "hogatt_rope_launch",
            "hogatt_paged_workspace_bytes", "hogatt_paged_sdpa_launch", "hogatt_copy_to_blocks_launch", "hogatt_plan_describe",
-           "hogatt_plan_ranges", "hogatt_dense_plan", "hogatt_launch_shape", "hogatt_step_plan_launch", "hogatt_append_launch"]
+           "hogatt_plan_ranges", "hogatt_dense_plan", "hogatt_launch_shape", "hogatt_step_plan_launch", "hogatt_append_launch",
+           "hogatt_paged_q4_workspace_bytes", "hogatt_paged_q4_sdpa_launch", "hogatt_copy_to_blocks_q4_launch", "hogatt_copy_from_blocks_q4_launch",
+           "hogatt_step_blocks_workspace_bytes", "hogatt_step_blocks_launch", "hogatt_compact_blocks_workspace_bytes",
+           "hogatt_compact_blocks_launch"]
 
 
 class Problem(C.Structure):
@@ -47,6 +50,41 @@ class PagedProblem(C.Structure):
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("kernel", C.c_int32), ("num_blocks", C.c_int32),
         ("device_status", C.c_void_p),
     ]
+
+
+class PagedQ4Problem(C.Structure):
+    _fields_ = [("paged", PagedProblem), ("key_scales", C.c_void_p), ("value_scales", C.c_void_p), ("key_unit", C.c_float), ("value_unit", C.c_float)]
+
+
+class Q4Append(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("B", "Hkv", "S", "E", "Ev", "block_size", "max_blocks", "num_blocks", "dtype")] + [
+        ("key_unit", C.c_float), ("value_unit", C.c_float),
+        ("keys", C.c_void_p), ("key_strides", C.c_int64 * 3), ("values", C.c_void_p), ("value_strides", C.c_int64 * 3),
+    ] + [(n, C.c_void_p) for n in ("key_cache", "value_cache", "key_scales", "value_scales", "block_table", "seq_lengths", "cu_seqlens",
+                                   "new_rows", "device_status")]
+
+
+class Q4Read(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("B", "Hkv", "S", "E", "Ev", "block_size", "max_blocks", "num_blocks", "dtype")] + [
+        ("key_unit", C.c_float), ("value_unit", C.c_float),
+    ] + [(n, C.c_void_p) for n in ("keys", "values", "key_cache", "value_cache", "key_scales", "value_scales", "block_table", "first_rows",
+                                   "device_status")]
+
+
+class BlockTensors(C.Structure):
+    _fields_ = [("count", C.c_int32), ("data", C.POINTER(C.c_void_p)), ("block_bytes", C.POINTER(C.c_int64))]
+
+
+class StepBlocks(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("num_blocks", "block_size", "max_blocks", "rows_in", "rows_out")] + [
+        (n, C.c_void_p) for n in ("refs_in", "table_in", "lengths_in", "source", "new_tokens", "refs_out", "table_out", "lengths_out", "room")
+    ] + [("caches", BlockTensors), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("device_status", C.c_void_p)]
+
+
+class CompactBlocks(C.Structure):
+    _fields_ = [("num_blocks", C.c_int32), ("table_entries", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("refs_in", "table_in", "refs_out", "table_out", "moved")
+    ] + [("caches", BlockTensors), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("device_status", C.c_void_p)]
 
 
 MAX_PEERS = 8
@@ -100,6 +138,18 @@ def load() -> C.CDLL:
         lib.hogatt_dense_plan.restype = C.c_int
         lib.hogatt_dense_plan.argtypes = [C.POINTER(C.c_int32), C.POINTER(C.c_uint8)] + [C.c_int32] * 3 + [C.POINTER(C.c_int64),
                                                                                                       C.POINTER(C.c_int32)]
+        for name, struct in (("hogatt_paged_q4_sdpa_launch", PagedQ4Problem), ("hogatt_copy_to_blocks_q4_launch", Q4Append),
+                             ("hogatt_copy_from_blocks_q4_launch", Q4Read), ("hogatt_step_blocks_launch", StepBlocks),
+                             ("hogatt_compact_blocks_launch", CompactBlocks)):
+            fn = getattr(lib, name)
+            fn.restype = C.c_int
+            fn.argtypes = [C.POINTER(struct), C.c_void_p]
+        lib.hogatt_paged_q4_workspace_bytes.restype = C.c_size_t
+        lib.hogatt_paged_q4_workspace_bytes.argtypes = [C.POINTER(PagedQ4Problem)]
+        for name in ("hogatt_step_blocks_workspace_bytes", "hogatt_compact_blocks_workspace_bytes"):
+            fn = getattr(lib, name)
+            fn.restype = C.c_size_t
+            fn.argtypes = [C.c_int32]
         _lib = lib
     return _lib
 

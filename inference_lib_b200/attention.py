@@ -9,7 +9,7 @@ only), and importing this module fails loudly when the compiled library cannot b
 from __future__ import annotations
 
 import os
-from typing import List, Optional
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -35,6 +35,12 @@ _FUSED_PLANNED = torch.ops.libhogatt.hogwild_fused_planned.default
 _PAGED_SDPA = torch.ops.libhogatt.hogwild_paged_sdpa.default
 _VARLEN_PAGED_SDPA = torch.ops.libhogatt.hogwild_varlen_paged_sdpa.default
 _COPY_TO_BLOCKS = torch.ops.libhogatt.copy_to_blocks.default
+_PAGED_SDPA_Q4 = torch.ops.libhogatt.hogwild_paged_sdpa_q4.default
+_VARLEN_PAGED_SDPA_Q4 = torch.ops.libhogatt.hogwild_varlen_paged_sdpa_q4.default
+_COPY_TO_BLOCKS_Q4 = torch.ops.libhogatt.copy_to_blocks_q4.default
+_COPY_FROM_BLOCKS_Q4 = torch.ops.libhogatt.copy_from_blocks_q4.default
+_STEP_BLOCKS = torch.ops.libhogatt.step_blocks.default
+_COMPACT_BLOCKS = torch.ops.libhogatt.compact_blocks.default
 fragment_append = torch.ops.libhogatt.fragment_append.default              # FragmentCache.update's two steps
 fragment_step_plan = torch.ops.libhogatt.fragment_step_plan.default
 
@@ -128,6 +134,95 @@ def copy_to_blocks(key_states: torch.Tensor, value_states: torch.Tensor, key_cac
     (``src/binding.cu:370-371``)."""
     _COPY_TO_BLOCKS(key_states.contiguous(), value_states.contiguous(), key_cache, value_cache,
                     block_table, seq_lengths)
+
+
+# ---- a paged cache in 4 bits (no counterpart in the reference) -----------------------------------------------------
+# Codes ``uint8 [NumBlocks,Hkv,bs,E/2]`` (two e2m1 values a byte, the even channel in the low half), scales ``float8_e4m3fn
+# [NumBlocks,Hkv,bs,E/16]``, one per 16 channels: value = e2m1(code) * scale * unit.  ``key_unit`` / ``value_unit`` are powers of two that
+# belong to a cache (1 suits magnitudes from 0.1 to 2,688).  ``status`` (optional, int32) gets the C ABI's status bits ORed in.
+
+def hogwild_paged_sdpa_q4(queries: torch.Tensor, locations: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                          key_scales: torch.Tensor, value_scales: torch.Tensor, block_table: torch.Tensor, scale: float,
+                          fragment_lengths: torch.Tensor, out: Optional[torch.Tensor] = None, *, key_unit: float = 1.0,
+                          value_unit: float = 1.0, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`hogwild_paged_sdpa` over a 4-bit cache: ``queries [F,W,Hq,S,E]`` (rotated) and ``out [W,Hq,S,Ev]`` in fp32, fp16 or bf16."""
+    if out is None:
+        out = torch.empty((queries.size(1), queries.size(2), queries.size(3), value_cache.size(3) * 2), dtype=queries.dtype, device=queries.device)
+    _PAGED_SDPA_Q4(out, scale, locations, queries.contiguous(), fragment_lengths, key_cache, value_cache, key_scales, value_scales,
+                   block_table, key_unit, value_unit, status)
+    return out
+
+
+def hogwild_varlen_paged_sdpa_q4(queries: torch.Tensor, locations: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                                 key_scales: torch.Tensor, value_scales: torch.Tensor, block_table: torch.Tensor, scale: float,
+                                 fragment_lengths: torch.Tensor, cu_seqlens_q: torch.Tensor, out: Optional[torch.Tensor] = None, *,
+                                 key_unit: float = 1.0, value_unit: float = 1.0, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`hogwild_varlen_paged_sdpa` over a 4-bit cache: ``queries [F,total_q,Hq,E]``, ``locations [F,total_q]``,
+    ``fragment_lengths [F,W]``, ``cu_seqlens_q [W+1]``.  Rows of ``out`` behind the last sequence are left as they are."""
+    if out is None:
+        out = torch.empty((queries.size(1), queries.size(2), value_cache.size(3) * 2), dtype=queries.dtype, device=queries.device)
+    _VARLEN_PAGED_SDPA_Q4(out, scale, locations, queries.contiguous(), fragment_lengths, key_cache, value_cache, key_scales, value_scales,
+                          block_table, cu_seqlens_q, key_unit, value_unit, status)
+    return out
+
+
+def copy_to_blocks_q4(key_states: torch.Tensor, value_states: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                      key_scales: torch.Tensor, value_scales: torch.Tensor, block_table: torch.Tensor, seq_lengths: torch.Tensor, *,
+                      cu_seqlens: Optional[torch.Tensor] = None, new_rows: Optional[torch.Tensor] = None, key_unit: float = 1.0,
+                      value_unit: float = 1.0, status: Optional[torch.Tensor] = None) -> None:
+    """:func:`copy_to_blocks` into a 4-bit cache: row ``t`` of sequence ``b`` is stored at position ``seq_lengths[b] + t``.  The states
+    are ``[B,Hkv,S,E]`` with any strides (the transposed view of a projection's output is taken as it is) or, with ``cu_seqlens [B+1]``,
+    packed ``[T,Hkv,E]``.  ``new_rows [B]``: rows from there on stay out (what :func:`step_blocks` returns as ``room``).  Rows whose page
+    the table does not name are dropped."""
+    _COPY_TO_BLOCKS_Q4(key_states, value_states, key_cache, value_cache, key_scales, value_scales, block_table, seq_lengths, cu_seqlens,
+                       new_rows, key_unit, value_unit, status)
+
+
+def copy_from_blocks_q4(key_cache: torch.Tensor, value_cache: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor,
+                        block_table: torch.Tensor, first_rows: torch.Tensor, rows: int, *, dtype: torch.dtype = torch.bfloat16,
+                        key_unit: float = 1.0, value_unit: float = 1.0,
+                        status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The numbers that a 4-bit cache holds: rows ``first_rows[b]`` ... ``first_rows[b] + rows - 1`` of every sequence of ``block_table``,
+    as keys ``[B,Hkv,rows,E]`` and values ``[B,Hkv,rows,Ev]``.  Rows without a page are NaN."""
+    shape = (block_table.size(0), key_cache.size(1), int(rows))
+    keys = torch.empty(shape + (key_cache.size(3) * 2,), dtype=dtype, device=key_cache.device)
+    values = torch.empty(shape + (value_cache.size(3) * 2,), dtype=dtype, device=key_cache.device)
+    _COPY_FROM_BLOCKS_Q4(keys, values, key_cache, value_cache, key_scales, value_scales, block_table, first_rows, key_unit, value_unit, status)
+    return keys, values
+
+
+# ---- the pages of a paged cache of any type (no counterpart in the reference) ------------------------------------------
+# ``block_refs[p]`` counts the block-table entries that name page ``p`` (plus what a caller adds to keep a page); 0: free.
+
+def step_blocks(block_refs: torch.Tensor, block_table: torch.Tensor, seq_lengths: torch.Tensor, caches: Sequence[torch.Tensor],
+                block_size: int, *, source: Optional[torch.Tensor] = None, new_tokens: Optional[torch.Tensor] = None,
+                out: Optional[Sequence[torch.Tensor]] = None,
+                status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """One step of a batch's pages: row ``w`` of the new table is row ``source[w]`` of the old one (``None``: every row stays; negative: an
+    empty row; several rows may take over the same one and then share its pages; rows that nobody takes over are freed), and every
+    row gets the pages for ``new_tokens[w]`` tokens behind its length, lowest free page first.  A last page that is partly filled and
+    shared is copied, in all ``caches`` (every tensor ``[NumBlocks,...]`` of every layer: keys, values, scales), unless its row is the last
+    holder.  Returns ``(block_refs, block_table, seq_lengths, room)`` in new tensors or in ``out``: lengths without the new tokens, and
+    ``room[w]`` = ``new_tokens[w]`` where the row has its pages, otherwise 0 (rows are served in order until the pool is empty).  ``out`` may
+    hold the inputs themselves where there is no ``source``; ``block_refs`` always.  Nothing is read back from the device."""
+    if out is None:
+        rows = seq_lengths.size(0) if source is None else source.size(0)
+        out = (torch.empty_like(block_refs), torch.empty((rows, block_table.size(-1)), dtype=torch.int32, device=block_table.device),
+               torch.empty(rows, dtype=torch.int32, device=block_table.device), torch.empty(rows, dtype=torch.int32, device=block_table.device))
+    refs, table, lengths, room = out
+    _STEP_BLOCKS(block_refs, block_table, seq_lengths, source, new_tokens, block_size, caches, refs, table, lengths, room, status)
+    return refs, table, lengths, room
+
+
+def compact_blocks(block_refs: torch.Tensor, block_table: torch.Tensor, caches: Sequence[torch.Tensor], *,
+                   out: Optional[Sequence[torch.Tensor]] = None,
+                   status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Moves the held pages to the front of ``caches`` (in place) and returns ``(block_refs, block_table, moved)`` in new tensors or in
+    ``out`` (which may hold the inputs): ``moved[p]`` is page ``p``'s new number, -1 for a free one.  The pages that are held end up as
+    ``0 .. n-1``; one that was there already stays."""
+    refs, table, moved = out if out is not None else (torch.empty_like(block_refs), torch.empty_like(block_table), torch.empty_like(block_refs))
+    _COMPACT_BLOCKS(block_refs, block_table, caches, refs, table, moved, status)
+    return refs, table, moved
 
 
 def rotate_half(x: torch.Tensor) -> torch.Tensor:

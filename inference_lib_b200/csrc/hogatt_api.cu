@@ -7,6 +7,7 @@
 #include <cstdlib>
 #include <cstring>
 
+#include "hogatt_host.h"
 #include "hogatt_device.cuh"
 #include "hogatt_f32.cuh"
 #include "hogatt_fma.cuh"
@@ -21,27 +22,16 @@
 #include <vector>
 
 namespace hogatt {
-namespace {
 
 thread_local int tl_last_cuda_error = 0;
 
-#define HOGATT_CUDA_OK(expr)                         \
-    do {                                             \
-        cudaError_t err__ = (expr);                  \
-        if (err__ != cudaSuccess) {                  \
-            tl_last_cuda_error = (int)err__;         \
-            (void)cudaGetLastError();                \
-            return HOGATT_ERR_CUDA;                  \
-        }                                            \
-    } while (0)
-
-constexpr int kMaxDevices = 64;
-
+namespace {
 struct DeviceInfo {
     std::atomic<int> sms{0};
     std::atomic<int> smem_optin{0};
 };
 DeviceInfo g_devices[kMaxDevices];
+}  // namespace
 
 int current_device_info(int* dev, int* sms, int* smem_optin) {
     HOGATT_CUDA_OK(cudaGetDevice(dev));
@@ -67,20 +57,6 @@ int current_device_info(int* dev, int* sms, int* smem_optin) {
     return HOGATT_OK;
 }
 
-// cudaFuncSetAttribute(MaxDynamicSharedMemorySize) once per (kernel instantiation, device).
-template <class Kernel>
-int ensure_smem_limit(Kernel kernel, int dev, size_t bytes, std::atomic<size_t>* granted /*[kMaxDevices]*/) {
-    if (bytes <= 48 * 1024) return HOGATT_OK;
-    if (granted[dev].load(std::memory_order_acquire) >= bytes) return HOGATT_OK;
-    HOGATT_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    granted[dev].store(bytes, std::memory_order_release);
-    return HOGATT_OK;
-}
-
-// Launch with the programmatic-stream-serialization attribute: the kernel may be scheduled while its
-// stream predecessor is still running (each of our kernels calls griddepcontrol.wait before it touches
-// global memory that earlier work may write -- everything except the K/V rows of fragments the caller
-// declared stable).  On unless HOGATT_PDL=0 is set in the environment when the library is first used.
 bool pdl_enabled() {
     static const bool on = [] {
         const char* v = getenv("HOGATT_PDL");
@@ -88,6 +64,8 @@ bool pdl_enabled() {
     }();
     return on;
 }
+
+namespace {
 
 // HOGATT_DENSE=0 in the environment keeps AUTO away from the tcgen05 kernel (A/B measurements).
 bool dense_disabled() {
@@ -107,25 +85,6 @@ bool host_plan_disabled() {
     }();
     return off;
 }
-
-template <class... KArgs, class... Args>
-cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
-}
-
-size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
-
-size_t dtype_size(int dtype) { return dtype == HOGATT_F32 ? 4 : 2; }
 
 // What will run for this problem.
 struct Resolved {
@@ -665,8 +624,6 @@ int fragment_map(const void* ptr, int rows, int Hkv, int dtype, CUtensorMap* out
     cache.emplace(key, *out);
     return HOGATT_OK;
 }
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 // `beside_predecessor`: the stream's preceding kernel is one of ours that writes nothing this one reads and lets it start
 // early; the rotation kernels end only after it (programmatic launch, waited for at the end).
@@ -1249,6 +1206,7 @@ const char* hogatt_status_string(int status) {
         case HOGATT_ERR_BAD_KERNEL_CHOICE: return "the requested kernel cannot run this dtype / head size";
         case HOGATT_ERR_TOO_LARGE: return "problem too large for 32-bit row indexing";
         case HOGATT_ERR_EXCEEDS_STATIC_SCRATCH: return "problem needs more scratch than the fixed HOGATT_STATIC_SCRATCH_BYTES array of hogatt_fused_launch_static; use hogatt_fused_launch with a caller workspace";
+        case HOGATT_ERR_BAD_UNIT: return "a 4-bit cache's unit is not a power of two between 2^-64 and 2^64";
     }
     return "unknown status";
 }

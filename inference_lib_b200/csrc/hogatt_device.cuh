@@ -186,17 +186,17 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 constexpr uint64_t kWaitLimitNs = 1000ull * 1000ull * 1000ull;
 // The limit the kernels read (only on the slow path of a wait): one second unless the host was started with
 // HOGATT_WAIT_LIMIT_MS in the environment, which the library copies here once per device (tests of the give-up path).
-__device__ unsigned long long g_wait_limit_ns = kWaitLimitNs;
+static __device__ unsigned long long g_wait_limit_ns = kWaitLimitNs;   // (one per translation unit)
 
 // The polling loop lives out of line: these kernels run for microseconds and their instruction fetch
 // shows in the call time, so every wait site is just a try_wait and a call.
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int bit);
+static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int bit);
 __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                                   int* status, int bit) {
     if (mbar_try_wait(bar, parity)) return true;
     return mbar_wait_slow(bar, parity, abort_flag, status, bit);
 }
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int bit) {
+static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int bit) {
     const uint64_t t0 = global_timer_ns();
     uint32_t spins = 0;
     while (!mbar_try_wait(bar, parity)) {
@@ -215,7 +215,7 @@ __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volat
 // The same limit without a call and in a few instructions, for kernels that cannot have calls or must stay small: it counts
 // failing polls, each of which the hardware holds for 3.96 us (B200).
 constexpr unsigned int kPollsPerMs = 250;
-__device__ unsigned int g_wait_polls = 1000u * kPollsPerMs;
+static __device__ unsigned int g_wait_polls = 1000u * kPollsPerMs;
 __device__ __forceinline__ bool wait_polls(uint32_t bar, uint32_t parity) {
     unsigned int polls = 0;
 #pragma unroll 1
@@ -233,7 +233,7 @@ __device__ __forceinline__ void settle() {
 // A CTA must not leave while copies may still be landing in its shared memory.  Unlike the waits above this one neither
 // goes by the abort flag -- after a wait that ran out the copies in flight still need their microseconds -- nor by the
 // configured limit.
-__device__ __noinline__ void drain_stage(uint32_t bar, uint32_t parity, int* status) {
+static __device__ __noinline__ void drain_stage(uint32_t bar, uint32_t parity, int* status) {
     if (mbar_try_wait(bar, parity)) return;              // (before the timer: a read of it takes a microsecond)
     const uint64_t t0 = global_timer_ns();
     while (!mbar_try_wait(bar, parity))

@@ -8,6 +8,8 @@
 // keeps 16 query rows of one kv head (all workers and GQA heads share each K/V tile) instead of
 // one (worker, token) per CTA.
 #pragma once
+#include <limits.h>
+
 #include "hogatt_device.cuh"
 
 namespace hogatt {
@@ -60,8 +62,9 @@ struct FmaCore {
         for (int r = 0; r < RPT; ++r) acc[r] = 0.f;
     }
     // Keys tok0 .. tok0+ntok-1 are staged (V rows past ntok zeroed) and the CTA has synchronised.
-    // Key `k` is visible to row r iff k < lim_s[r].  Ends before the trailing __syncthreads().
-    __device__ __forceinline__ void compute(int tok0, int ntok, float l2scale) {
+    // Key `k` is visible to row r iff k < lim_s[r] (and, where `odd` is given, odd[k - tok0] has no bit 16: there is such a key).  Ends
+    // before the trailing __syncthreads().
+    __device__ __forceinline__ void compute(int tok0, int ntok, float l2scale, const int* odd = nullptr) {
         {
             float s0 = 0.f, s1 = 0.f;
             if (lane < ntok) {
@@ -74,7 +77,7 @@ struct FmaCore {
                     s1 = fmaf(qb[e], kv, s1);
                 }
             }
-            const int key = tok0 + lane;
+            const int key = odd && odd[lane] >> 16 ? INT_MAX : tok0 + lane;
             s0 = (lane < ntok && key < lim_s[warp]) ? s0 * l2scale : -INFINITY;
             s1 = (lane < ntok && key < lim_s[warp + 8]) ? s1 * l2scale : -INFINITY;
             float x0 = s0, x1 = s1;

@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(WW * 32, (WW == 4 && KP == 16) ? 5 : 1) merge_
 struct PeerFlags {
     int* f[HOGATT_MAX_PEERS];
 };
-__global__ void __launch_bounds__(32) gather_signal_kernel(const __grid_constant__ PeerFlags flags, int world, int rank,
+static __global__ void __launch_bounds__(32) gather_signal_kernel(const __grid_constant__ PeerFlags flags, int world, int rank,
                                                            int* status, int debug_id) {
     const int lane = threadIdx.x;
     int* mine = flags.f[rank];

@@ -1,0 +1,341 @@
+// C ABI of the 4-bit paged cache and of page bookkeeping (declared in include/hogatt.h): argument validation, kernel choice, workspace
+// carving and launches, like hogatt_api.cu.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "hogatt_host.h"
+#include "hogatt_blocks.cuh"
+#include "hogatt_q4.cuh"
+
+namespace hogatt {
+namespace {
+
+// A power of two far enough from the ends of fp32 that a scale times it, and six times it, are normal numbers.
+bool unit_ok(float u) {
+    int e;
+    return u > 0.f && std::isfinite(u) && std::frexp(u, &e) == 0.5f && e >= -63 && e <= 65;
+}
+
+int cache_shape(int Hkv, int E, int Ev, int block_size, int max_blocks, int num_blocks, int dtype) {
+    if (Hkv <= 0 || E <= 0 || Ev <= 0 || block_size <= 0 || max_blocks <= 0 || num_blocks <= 0) return HOGATT_ERR_BAD_SHAPE;
+    if (dtype != HOGATT_F32 && dtype != HOGATT_F16 && dtype != HOGATT_BF16) return HOGATT_ERR_UNSUPPORTED_DTYPE;
+    if (E % kGroup != 0 || Ev % kGroup != 0 || E > 256 || Ev > 256) return HOGATT_ERR_UNSUPPORTED_HEAD_DIM;
+    return HOGATT_OK;
+}
+
+struct Q4Plan {
+    int tokens_per_group, head_blocks, groups_bound, units, splits;
+    size_t o, m, l, total;
+};
+
+int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
+    if (x == nullptr) return HOGATT_ERR_NULL_POINTER;
+    const hogatt_paged_problem* p = &x->paged;
+    const bool packed = p->cu_seqlens_q != nullptr;
+    if (p->F <= 0 || p->W <= 0 || p->Hq <= 0 || p->Hkv <= 0 || p->Hq % p->Hkv != 0 || (packed ? p->total_q_tokens < 0 : p->S <= 0))
+        return HOGATT_ERR_BAD_SHAPE;
+    if (const int rc = cache_shape(p->Hkv, p->E, p->Ev, p->block_size, p->max_blocks_per_seq, p->num_blocks, p->dtype)) return rc;
+    if (p->Ev != 32 && p->Ev != 64 && p->Ev != 128 && p->Ev != 256) return HOGATT_ERR_UNSUPPORTED_HEAD_DIM;
+    if (p->F > 4096) return HOGATT_ERR_TOO_MANY_FRAGMENTS;
+    if (p->kernel != HOGATT_KERNEL_AUTO && p->kernel != HOGATT_KERNEL_FMA) return HOGATT_ERR_BAD_KERNEL_CHOICE;
+    if (!packed && (int64_t)p->F * p->W * p->S >= ((int64_t)1 << 31)) return HOGATT_ERR_TOO_LARGE;
+    if (packed && (int64_t)p->F * std::max(p->total_q_tokens, p->W) >= ((int64_t)1 << 31)) return HOGATT_ERR_TOO_LARGE;
+    const int G = p->Hq / p->Hkv;
+    pl->tokens_per_group = G >= 16 ? 1 : 16 / G;
+    pl->head_blocks = (G + 15) / 16;
+    const int64_t groups = packed ? ((int64_t)p->total_q_tokens + pl->tokens_per_group - 1) / pl->tokens_per_group + p->W
+                                  : (int64_t)p->W * ((p->S + pl->tokens_per_group - 1) / pl->tokens_per_group);
+    const int64_t units = groups * pl->head_blocks * p->Hkv;
+    if (units > (1 << 24)) return HOGATT_ERR_TOO_LARGE;
+    pl->groups_bound = (int)groups;
+    pl->units = (int)std::max<int64_t>(units, 1);
+    pl->splits = std::max(1, std::min(24, (3 * sms + pl->units - 1) / pl->units));      // (24: the merge step's one round trip)
+    const size_t slots = (size_t)pl->units * pl->splits * kFmaRows;
+    pl->o = 0;
+    pl->m = pl->o + align_up(slots * p->Ev * sizeof(float), 256);
+    pl->l = pl->m + align_up(slots * sizeof(float), 256);
+    pl->total = pl->l + align_up(slots * sizeof(float), 256);
+    return HOGATT_OK;
+}
+
+template <class T>
+int launch_q4_merge(const Q4Args& x, const Q4Plan& pl, cudaStream_t stream) {
+    HOGATT_CUDA_OK(launch_kernel(q4_merge_kernel<T>, dim3(pl.units, kFmaRows / kMergeWarps), dim3(kMergeWarps * 32), 0, stream, x.p));
+    return HOGATT_OK;
+}
+
+template <class T, int EV>
+int launch_q4_fma(const Q4Args& x, const Q4Plan& pl, int dev, int smem_optin, cudaStream_t stream) {
+    static std::atomic<size_t> granted[kMaxDevices];
+    const size_t smem = q4_smem_bytes(x.p.E, EV, x.p.F);
+    if (smem > (size_t)smem_optin) return HOGATT_ERR_TOO_MANY_FRAGMENTS;
+    const int rc = ensure_smem_limit(q4_attention_kernel<T, EV>, dev, smem, granted);
+    if (rc != HOGATT_OK) return rc;
+    HOGATT_CUDA_OK(launch_kernel(q4_attention_kernel<T, EV>, dim3(pl.units, pl.splits), dim3(kFmaThreads), smem, stream, x));
+    return launch_q4_merge<T>(x, pl, stream);
+}
+
+template <class T>
+int launch_q4(const Q4Args& x, const Q4Plan& pl, int dev, int smem_optin, cudaStream_t stream) {
+    switch (x.p.Ev) {
+        case 32: return launch_q4_fma<T, 32>(x, pl, dev, smem_optin, stream);
+        case 64: return launch_q4_fma<T, 64>(x, pl, dev, smem_optin, stream);
+        case 128: return launch_q4_fma<T, 128>(x, pl, dev, smem_optin, stream);
+        default: return launch_q4_fma<T, 256>(x, pl, dev, smem_optin, stream);
+    }
+}
+
+// Bookkeeping runs as one cluster; the copies follow on the whole GPU.
+int launch_copies(const hogatt_block_tensors* t, const int* count, const int* pairs, int64_t most, int sms, cudaStream_t stream) {
+    for (int first = 0; first < t->count; first += kMaxPageTensors) {
+        CopyPagesArgs c;
+        memset(&c, 0, sizeof(c));
+        c.n = std::min(kMaxPageTensors, t->count - first);
+        c.count = count;
+        c.pairs = pairs;
+        int64_t pieces = 0;
+        for (int i = 0; i < c.n; ++i) {
+            const int64_t bytes = t->block_bytes[first + i];
+            c.t[i] = {static_cast<char*>(t->data[first + i]), bytes, (int)pieces, aligned16(t->data[first + i]) && bytes % 16 == 0};
+            pieces += (bytes + kPagePiece - 1) / kPagePiece;
+            if (pieces >= ((int64_t)1 << 31)) return HOGATT_ERR_TOO_LARGE;
+        }
+        c.pieces = (int)pieces;
+        const int64_t ctas = (most * pieces + 7) / 8;
+        HOGATT_CUDA_OK(launch_kernel(copy_pages_kernel, dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(ctas, (int64_t)sms * 6))), dim3(256), 0, stream, c));
+    }
+    return HOGATT_OK;
+}
+
+template <class Args>
+cudaError_t launch_cluster(void (*kernel)(Args), cudaStream_t stream, const Args& args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kBlocksCluster);
+    cfg.blockDim = dim3(kBlocksThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kBlocksCluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args);
+}
+
+int check_tensors(const hogatt_block_tensors* t) {
+    if (t->count < 0) return HOGATT_ERR_BAD_SHAPE;
+    if (t->count > 0 && (!t->data || !t->block_bytes)) return HOGATT_ERR_NULL_POINTER;
+    for (int i = 0; i < t->count; ++i) {
+        if (!t->data[i]) return HOGATT_ERR_NULL_POINTER;
+        if (t->block_bytes[i] <= 0) return HOGATT_ERR_BAD_SHAPE;
+    }
+    return HOGATT_OK;
+}
+
+}  // namespace
+}  // namespace hogatt
+
+using namespace hogatt;
+
+extern "C" {
+
+size_t hogatt_paged_q4_workspace_bytes(const hogatt_paged_q4_problem* p) {
+    int dev, sms, smem_optin;
+    if (current_device_info(&dev, &sms, &smem_optin) != HOGATT_OK) return 0;
+    Q4Plan pl;
+    return plan_q4(p, sms, &pl) == HOGATT_OK ? pl.total : 0;
+}
+
+int hogatt_paged_q4_sdpa_launch(const hogatt_paged_q4_problem* x, hogatt_stream_t stream_) {
+    cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+    Q4Plan pl;
+    int rc = plan_q4(x, 1, &pl);                          // (arguments before anything about the device)
+    if (rc != HOGATT_OK) return rc;
+    const hogatt_paged_problem* p = &x->paged;
+    if (!unit_ok(x->key_unit) || !unit_ok(x->value_unit)) return HOGATT_ERR_BAD_UNIT;
+    if (!p->out || !p->queries || !p->locations || !p->fragment_lengths || !p->key_cache || !p->value_cache || !x->key_scales ||
+        !x->value_scales || !p->block_table || !p->workspace)
+        return HOGATT_ERR_NULL_POINTER;
+    if (!aligned16(p->out) || !aligned16(p->queries) || !aligned16(p->key_cache) || !aligned16(p->value_cache) || !aligned16(x->key_scales) ||
+        !aligned16(x->value_scales) || ((uintptr_t)p->workspace & 255u))
+        return HOGATT_ERR_MISALIGNED;
+    const bool packed = p->cu_seqlens_q != nullptr;
+    if (packed && p->total_q_tokens == 0) return HOGATT_OK;
+    int dev, sms, smem_optin;
+    rc = current_device_info(&dev, &sms, &smem_optin);
+    if (rc == HOGATT_OK) rc = plan_q4(x, sms, &pl);
+    if (rc != HOGATT_OK) return rc;
+    if (p->workspace_bytes < pl.total) return HOGATT_ERR_WORKSPACE_TOO_SMALL;
+
+    Q4Args args;
+    memset(&args, 0, sizeof(args));
+    PagedArgs& a = args.p;
+    a.F = p->F; a.W = p->W; a.Hq = p->Hq; a.Hkv = p->Hkv; a.G = p->Hq / p->Hkv; a.E = p->E; a.Ev = p->Ev;
+    a.S = p->S; a.total_q = packed ? p->total_q_tokens : p->W * p->S;
+    a.block_size = p->block_size; a.max_blocks = p->max_blocks_per_seq;
+    a.tokens_per_group = pl.tokens_per_group; a.head_blocks = pl.head_blocks; a.groups_bound = pl.groups_bound;
+    a.splits = pl.splits;
+    a.l2scale = (float)((double)p->scale * 1.4426950408889634 * x->key_unit);
+    if (packed) {     // q [F,total_q,Hq,E], out [total_q,Hq,Ev], loc [F,total_q], len [F,W]; s is the packed token index
+        a.q_f = (long long)a.total_q * p->Hq * p->E; a.q_w = 0; a.q_s = (long long)p->Hq * p->E; a.q_h = p->E;
+        a.o_w = 0; a.o_s = (long long)p->Hq * p->Ev; a.o_h = p->Ev;
+        a.loc_f = a.total_q; a.loc_w = 0; a.len_f = p->W; a.len_w = 1;
+    } else {          // q [F,W,Hq,S,E], out [W,Hq,S,Ev], loc [F,W,S], len [F]
+        a.q_f = (long long)p->W * p->Hq * p->S * p->E; a.q_w = (long long)p->Hq * p->S * p->E; a.q_s = p->E;
+        a.q_h = (long long)p->S * p->E;
+        a.o_w = (long long)p->Hq * p->S * p->Ev; a.o_s = p->Ev; a.o_h = (long long)p->S * p->Ev;
+        a.loc_f = p->W * p->S; a.loc_w = p->S; a.len_f = 1; a.len_w = 0;
+    }
+    a.out = p->out; a.q = p->queries; a.loc = p->locations; a.flen = p->fragment_lengths;
+    a.kcache = p->key_cache; a.vcache = p->value_cache; a.block_table = p->block_table; a.cu_seqlens = p->cu_seqlens_q;
+    unsigned char* ws = static_cast<unsigned char*>(p->workspace);
+    a.ws_o = reinterpret_cast<float*>(ws + pl.o);
+    a.ws_m = reinterpret_cast<float*>(ws + pl.m);
+    a.ws_l = reinterpret_cast<float*>(ws + pl.l);
+    a.status = p->device_status;
+    args.kscale = static_cast<const unsigned char*>(x->key_scales);
+    args.vscale = static_cast<const unsigned char*>(x->value_scales);
+    args.num_blocks = p->num_blocks;
+    args.vunit = x->value_unit;
+    switch (p->dtype) {
+        case HOGATT_F32: return launch_q4<float>(args, pl, dev, smem_optin, stream);
+        case HOGATT_F16: return launch_q4<__half>(args, pl, dev, smem_optin, stream);
+        default: return launch_q4<__nv_bfloat16>(args, pl, dev, smem_optin, stream);
+    }
+}
+
+int hogatt_copy_to_blocks_q4_launch(const hogatt_q4_append* p, hogatt_stream_t stream_) {
+    cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+    if (p == nullptr) return HOGATT_ERR_NULL_POINTER;
+    const bool packed = p->cu_seqlens != nullptr;
+    if (p->B <= 0 || p->S < 0) return HOGATT_ERR_BAD_SHAPE;
+    if (const int rc = cache_shape(p->Hkv, p->E, p->Ev, p->block_size, p->max_blocks, p->num_blocks, p->dtype)) return rc;
+    if (!unit_ok(p->key_unit) || !unit_ok(p->value_unit)) return HOGATT_ERR_BAD_UNIT;
+    if (!p->keys || !p->values || !p->key_cache || !p->value_cache || !p->key_scales || !p->value_scales || !p->block_table || !p->seq_lengths)
+        return HOGATT_ERR_NULL_POINTER;
+    if (!aligned16(p->key_cache) || !aligned16(p->value_cache) || !aligned16(p->key_scales) || !aligned16(p->value_scales)) return HOGATT_ERR_MISALIGNED;
+    if (p->S == 0) return HOGATT_OK;
+    Q4AppendArgs a;
+    memset(&a, 0, sizeof(a));
+    a.B = p->B; a.Hkv = p->Hkv; a.S = p->S; a.E = p->E; a.Ev = p->Ev;
+    a.block_size = p->block_size; a.max_blocks = p->max_blocks; a.num_blocks = p->num_blocks;
+    a.packed_tokens = packed ? p->S : 0;
+    const int vec = 16 / (int)dtype_size(p->dtype);
+    bool vectorised = aligned16(p->keys) && aligned16(p->values);
+    for (int i = 0; i < 3; ++i) {
+        a.ks[i] = p->key_strides[i];
+        a.vs[i] = p->value_strides[i];
+        vectorised = vectorised && a.ks[i] % vec == 0 && a.vs[i] % vec == 0;
+    }
+    a.key_unit = p->key_unit; a.value_unit = p->value_unit;
+    a.k = p->keys; a.v = p->values;
+    a.codes[0] = static_cast<unsigned char*>(p->key_cache); a.codes[1] = static_cast<unsigned char*>(p->value_cache);
+    a.scales[0] = static_cast<unsigned char*>(p->key_scales); a.scales[1] = static_cast<unsigned char*>(p->value_scales);
+    a.table = p->block_table; a.lengths = p->seq_lengths; a.cu = p->cu_seqlens; a.new_rows = p->new_rows; a.status = p->device_status;
+    int dev, sms, smem_optin;
+    if (const int rc = current_device_info(&dev, &sms, &smem_optin)) return rc;
+    const int64_t total = (packed ? (int64_t)p->S : (int64_t)p->B * p->S) * p->Hkv * ((p->E + p->Ev) / kGroup);
+    const dim3 grid((unsigned)std::min<int64_t>((total + 255) / 256, (int64_t)sms * 8));
+    cudaError_t err;
+    switch (p->dtype) {
+        case HOGATT_F32: err = launch_kernel(q4_append_kernel<float>, grid, dim3(256), 0, stream, a, (int)vectorised); break;
+        case HOGATT_F16: err = launch_kernel(q4_append_kernel<__half>, grid, dim3(256), 0, stream, a, (int)vectorised); break;
+        default: err = launch_kernel(q4_append_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, a, (int)vectorised); break;
+    }
+    HOGATT_CUDA_OK(err);
+    return HOGATT_OK;
+}
+
+int hogatt_copy_from_blocks_q4_launch(const hogatt_q4_read* p, hogatt_stream_t stream_) {
+    cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+    if (p == nullptr) return HOGATT_ERR_NULL_POINTER;
+    if (p->B <= 0 || p->S < 0) return HOGATT_ERR_BAD_SHAPE;
+    if (const int rc = cache_shape(p->Hkv, p->E, p->Ev, p->block_size, p->max_blocks, p->num_blocks, p->dtype)) return rc;
+    if (!unit_ok(p->key_unit) || !unit_ok(p->value_unit)) return HOGATT_ERR_BAD_UNIT;
+    if (p->S == 0) return HOGATT_OK;
+    if (!p->keys || !p->values || !p->key_cache || !p->value_cache || !p->key_scales || !p->value_scales || !p->block_table || !p->first_rows)
+        return HOGATT_ERR_NULL_POINTER;
+    if (!aligned16(p->keys) || !aligned16(p->values) || !aligned16(p->key_cache) || !aligned16(p->value_cache) || !aligned16(p->key_scales) ||
+        !aligned16(p->value_scales))
+        return HOGATT_ERR_MISALIGNED;
+    Q4ReadArgs a;
+    memset(&a, 0, sizeof(a));
+    a.B = p->B; a.Hkv = p->Hkv; a.S = p->S; a.E = p->E; a.Ev = p->Ev;
+    a.block_size = p->block_size; a.max_blocks = p->max_blocks; a.num_blocks = p->num_blocks;
+    a.key_unit = p->key_unit; a.value_unit = p->value_unit;
+    a.k = p->keys; a.v = p->values;
+    a.codes[0] = static_cast<const unsigned char*>(p->key_cache); a.codes[1] = static_cast<const unsigned char*>(p->value_cache);
+    a.scales[0] = static_cast<const unsigned char*>(p->key_scales); a.scales[1] = static_cast<const unsigned char*>(p->value_scales);
+    a.table = p->block_table; a.first = p->first_rows; a.status = p->device_status;
+    int dev, sms, smem_optin;
+    if (const int rc = current_device_info(&dev, &sms, &smem_optin)) return rc;
+    const int64_t total = (int64_t)p->B * p->S * p->Hkv * ((p->E + p->Ev) / kGroup);
+    const dim3 grid((unsigned)std::min<int64_t>((total + 255) / 256, (int64_t)sms * 8));
+    cudaError_t err;
+    switch (p->dtype) {
+        case HOGATT_F32: err = launch_kernel(q4_read_kernel<float>, grid, dim3(256), 0, stream, a); break;
+        case HOGATT_F16: err = launch_kernel(q4_read_kernel<__half>, grid, dim3(256), 0, stream, a); break;
+        default: err = launch_kernel(q4_read_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, a); break;
+    }
+    HOGATT_CUDA_OK(err);
+    return HOGATT_OK;
+}
+
+size_t hogatt_step_blocks_workspace_bytes(int32_t rows_out) {
+    return rows_out > 0 && rows_out <= HOGATT_MAX_BLOCK_ROWS ? align_up((size_t)step_blocks_ints(rows_out) * sizeof(int), 256) : 0;
+}
+
+int hogatt_step_blocks_launch(const hogatt_step_blocks* p, hogatt_stream_t stream_) {
+    cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+    if (p == nullptr) return HOGATT_ERR_NULL_POINTER;
+    if (p->num_blocks <= 0 || p->block_size <= 0 || p->max_blocks <= 0 || p->rows_in <= 0 || p->rows_out <= 0 || (!p->source && p->rows_out != p->rows_in))
+        return HOGATT_ERR_BAD_SHAPE;
+    if (p->rows_in > HOGATT_MAX_BLOCK_ROWS || p->rows_out > HOGATT_MAX_BLOCK_ROWS) return HOGATT_ERR_TOO_LARGE;
+    if (!p->refs_in || !p->table_in || !p->lengths_in || !p->refs_out || !p->table_out || !p->lengths_out || !p->room || !p->workspace)
+        return HOGATT_ERR_NULL_POINTER;
+    // rows that change places cannot be taken over in place
+    if (p->source && (p->table_out == p->table_in || p->lengths_out == p->lengths_in)) return HOGATT_ERR_BAD_SHAPE;
+    if (const int rc = check_tensors(&p->caches)) return rc;
+    if ((uintptr_t)p->workspace & 255u) return HOGATT_ERR_MISALIGNED;
+    if (p->workspace_bytes < hogatt_step_blocks_workspace_bytes(p->rows_out)) return HOGATT_ERR_WORKSPACE_TOO_SMALL;
+    int dev, sms, smem_optin;
+    if (const int rc = current_device_info(&dev, &sms, &smem_optin)) return rc;
+    StepBlocksArgs a;
+    a.num_blocks = p->num_blocks; a.block_size = p->block_size; a.max_blocks = p->max_blocks; a.rows_in = p->rows_in; a.rows_out = p->rows_out;
+    a.refs_in = p->refs_in; a.table_in = p->table_in; a.lengths_in = p->lengths_in; a.source = p->source; a.new_tokens = p->new_tokens;
+    a.refs_out = p->refs_out; a.table_out = p->table_out; a.lengths_out = p->lengths_out; a.room = p->room;
+    a.ws = static_cast<int*>(p->workspace);
+    a.status = p->device_status;
+    HOGATT_CUDA_OK(launch_cluster(step_blocks_kernel, stream, a));
+    if (p->new_tokens == nullptr) return HOGATT_OK;                 // (nobody writes: nothing is copied)
+    return launch_copies(&p->caches, a.ws, a.ws + step_blocks_pairs(p->rows_out), p->rows_out, sms, stream);
+}
+
+size_t hogatt_compact_blocks_workspace_bytes(int32_t num_blocks) {
+    return num_blocks > 0 ? align_up((size_t)compact_blocks_ints(num_blocks) * sizeof(int), 256) : 0;
+}
+
+int hogatt_compact_blocks_launch(const hogatt_compact_blocks* p, hogatt_stream_t stream_) {
+    cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+    if (p == nullptr) return HOGATT_ERR_NULL_POINTER;
+    if (p->num_blocks <= 0 || p->table_entries < 0) return HOGATT_ERR_BAD_SHAPE;
+    if (!p->refs_in || !p->refs_out || !p->moved || !p->workspace || (p->table_entries > 0 && (!p->table_in || !p->table_out)))
+        return HOGATT_ERR_NULL_POINTER;
+    if (const int rc = check_tensors(&p->caches)) return rc;
+    if ((uintptr_t)p->workspace & 255u) return HOGATT_ERR_MISALIGNED;
+    if (p->workspace_bytes < hogatt_compact_blocks_workspace_bytes(p->num_blocks)) return HOGATT_ERR_WORKSPACE_TOO_SMALL;
+    int dev, sms, smem_optin;
+    if (const int rc = current_device_info(&dev, &sms, &smem_optin)) return rc;
+    CompactBlocksArgs a;
+    a.num_blocks = p->num_blocks; a.entries = p->table_entries;
+    a.refs_in = p->refs_in; a.table_in = p->table_in; a.refs_out = p->refs_out; a.table_out = p->table_out; a.moved = p->moved;
+    a.ws = static_cast<int*>(p->workspace);
+    a.status = p->device_status;
+    HOGATT_CUDA_OK(launch_cluster(compact_blocks_kernel, stream, a));
+    return launch_copies(&p->caches, a.ws, a.ws + kCompactHead, p->num_blocks / 2 + 1, sms, stream);
+}
+
+}  // extern "C"

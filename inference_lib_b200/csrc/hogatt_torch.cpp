@@ -455,6 +455,302 @@ void fragment_step_plan(const at::Tensor& order, const at::Tensor& fragment_leng
     check_status(hogatt_step_plan_launch(&p, reinterpret_cast<hogatt_stream_t>(stream)), "fragment_step_plan");
 }
 
+// --- a paged cache in 4 bits, and the pages of a cache -------------------------------------------------------------
+
+// The four tensors of a 4-bit cache: codes uint8 [NumBlocks,Hkv,bs,E/2] and scales float8_e4m3fn [NumBlocks,Hkv,bs,E/16].
+struct Q4Cache {
+    int num_blocks, Hkv, block_size, E, Ev;
+};
+Q4Cache check_q4_cache(const char* what, const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& key_scales,
+                       const at::Tensor& value_scales, const at::Tensor& block_table, c10::Device device) {
+    for (const at::Tensor* t : {&key_cache, &value_cache, &key_scales, &value_scales, &block_table})
+        TORCH_CHECK(t->device() == device && t->is_contiguous(), what, ": caches, scales and block_table must be contiguous and on one device");
+    for (const at::Tensor* t : {&key_cache, &value_cache})
+        TORCH_CHECK(t->dim() == 4 && t->scalar_type() == at::kByte, what, ": 4-bit caches are uint8 [NumBlocks,Hkv,bs,E/2]");
+    for (const at::Tensor* t : {&key_scales, &value_scales})
+        TORCH_CHECK(t->dim() == 4 && t->scalar_type() == at::kFloat8_e4m3fn, what, ": scales are float8_e4m3fn [NumBlocks,Hkv,bs,E/16]");
+    for (int i = 0; i < 3; ++i)
+        TORCH_CHECK(value_cache.size(i) == key_cache.size(i) && key_scales.size(i) == key_cache.size(i) && value_scales.size(i) == key_cache.size(i),
+                    what, ": caches and scales must agree in [NumBlocks,Hkv,bs]");
+    TORCH_CHECK(key_cache.size(3) == 8 * key_scales.size(3) && value_cache.size(3) == 8 * value_scales.size(3),
+                what, ": a row of E/2 code bytes has E/16 scales");
+    TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt, what, ": block_table must be int32 [W,max_blocks]");
+    TORCH_CHECK(key_cache.size(0) <= INT32_MAX && key_cache.size(2) <= INT32_MAX && block_table.size(1) <= INT32_MAX, what, ": too large");
+    return {(int)key_cache.size(0), (int)key_cache.size(1), (int)key_cache.size(2), (int)key_cache.size(3) * 2, (int)value_cache.size(3) * 2};
+}
+int32_t* status_word(const char* what, const std::optional<at::Tensor>& status, c10::Device device) {
+    if (!status.has_value()) return nullptr;
+    TORCH_CHECK(status->device() == device && status->numel() > 0 && status->scalar_type() == at::kInt, what, ": status must be int32 on the same device");
+    return status->data_ptr<int>();
+}
+const int32_t* int_vector(const char* what, const char* name, const at::Tensor& t, int64_t n, c10::Device device) {
+    TORCH_CHECK(t.device() == device && t.dim() == 1 && t.size(0) == n && t.is_contiguous() && t.scalar_type() == at::kInt,
+                what, ": ", name, " must be contiguous int32 [", n, "]");
+    return t.const_data_ptr<int>();
+}
+const int32_t* int_vector(const char* what, const char* name, const std::optional<at::Tensor>& t, int64_t n, c10::Device device) {
+    return t.has_value() ? int_vector(what, name, *t, n, device) : nullptr;
+}
+
+void run_paged_q4(const char* what, at::Tensor& out, double scale, const at::Tensor& locations, const at::Tensor& queries,
+                  const at::Tensor& fragment_lengths, const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& key_scales,
+                  const at::Tensor& value_scales, const at::Tensor& block_table, const at::Tensor* cu_seqlens_q, double key_unit,
+                  double value_unit, const std::optional<at::Tensor>& status) {
+    TORCH_CHECK(out.is_cuda(), "libhogatt: tensors must live on a CUDA device");
+    const c10::cuda::CUDAGuard guard(out.device());
+    const bool packed = cu_seqlens_q != nullptr;
+    for (const at::Tensor* t : {(const at::Tensor*)&out, &locations, &queries, &fragment_lengths})
+        TORCH_CHECK(t->is_contiguous() && t->device() == out.device(), what, ": tensors must be contiguous and on one device");
+    TORCH_CHECK(locations.scalar_type() == at::kInt && fragment_lengths.scalar_type() == at::kInt, what, ": locations and fragment_lengths must be int32");
+    TORCH_CHECK(queries.scalar_type() == out.scalar_type(), what, ": queries must have the dtype of output");
+    const Q4Cache c = check_q4_cache(what, key_cache, value_cache, key_scales, value_scales, block_table, out.device());
+    hogatt_paged_q4_problem x = {};
+    hogatt_paged_problem& p = x.paged;
+    p.Hkv = c.Hkv; p.E = c.E; p.Ev = c.Ev; p.block_size = c.block_size; p.num_blocks = c.num_blocks;
+    p.max_blocks_per_seq = (int32_t)block_table.size(1);
+    if (packed) {
+        TORCH_CHECK(out.dim() == 3 && queries.dim() == 4 && locations.dim() == 2 && fragment_lengths.dim() == 2,
+                    what, ": out [total_q,Hq,Ev], queries [F,total_q,Hq,E], locations [F,total_q], fragment_lengths [F,W]");
+        TORCH_CHECK(cu_seqlens_q->dim() == 1 && cu_seqlens_q->size(0) > 0, what, ": cu_seqlens_q must be int32 [W+1]");
+        p.W = (int32_t)cu_seqlens_q->size(0) - 1;
+        p.cu_seqlens_q = int_vector(what, "cu_seqlens_q", *cu_seqlens_q, p.W + 1, out.device());
+        p.F = (int32_t)queries.size(0);
+        p.total_q_tokens = (int32_t)out.size(0);
+        p.Hq = (int32_t)out.size(1);
+        TORCH_CHECK_EQ(queries.size(1), out.size(0));
+        TORCH_CHECK_EQ(queries.size(2), out.size(1));
+        TORCH_CHECK_EQ(locations.size(0), p.F);
+        TORCH_CHECK_EQ(locations.size(1), out.size(0));
+        TORCH_CHECK_EQ(fragment_lengths.size(0), p.F);
+        TORCH_CHECK_EQ(fragment_lengths.size(1), p.W);
+    } else {
+        TORCH_CHECK(out.dim() == 4 && queries.dim() == 5 && locations.dim() == 3 && fragment_lengths.dim() == 1,
+                    what, ": out [W,Hq,S,Ev], queries [F,W,Hq,S,E], locations [F,W,S], fragment_lengths [F]");
+        p.F = (int32_t)queries.size(0);
+        p.W = (int32_t)out.size(0);
+        p.Hq = (int32_t)out.size(1);
+        p.S = (int32_t)out.size(2);
+        for (int i = 0; i < 3; ++i) TORCH_CHECK_EQ(queries.size(i + 1), out.size(i));
+        TORCH_CHECK_EQ(locations.size(0), p.F);
+        TORCH_CHECK_EQ(locations.size(1), p.W);
+        TORCH_CHECK_EQ(locations.size(2), p.S);
+        TORCH_CHECK_EQ(fragment_lengths.size(0), p.F);
+    }
+    TORCH_CHECK(queries.size(-1) == c.E && out.size(-1) == c.Ev, what, ": head sizes of queries / out and caches differ");
+    TORCH_CHECK_EQ(block_table.size(0), p.W);
+    p.dtype = dtype_code(out);
+    p.scale = (float)scale;
+    p.out = out.data_ptr();
+    p.queries = queries.const_data_ptr();
+    p.locations = locations.const_data_ptr<int>();
+    p.fragment_lengths = fragment_lengths.const_data_ptr<int>();
+    p.key_cache = key_cache.const_data_ptr();
+    p.value_cache = value_cache.const_data_ptr();
+    p.block_table = block_table.const_data_ptr<int>();
+    p.device_status = status_word(what, status, out.device());
+    x.key_scales = key_scales.const_data_ptr();
+    x.value_scales = value_scales.const_data_ptr();
+    x.key_unit = (float)key_unit;
+    x.value_unit = (float)value_unit;
+    if (packed && p.total_q_tokens == 0) return;
+    const size_t need = hogatt_paged_q4_workspace_bytes(&x);
+    TORCH_CHECK(need > 0, what, ": unsupported problem (head sizes ", p.E, "/", p.Ev, ", Hq ", p.Hq, ", Hkv ", p.Hkv, ", ", c.num_blocks, " blocks of ",
+                c.block_size, ")");
+    at::Tensor workspace = at::empty({(int64_t)need}, out.options().dtype(at::kByte));
+    p.workspace = workspace.data_ptr();
+    p.workspace_bytes = need;
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream();
+    check_status(hogatt_paged_q4_sdpa_launch(&x, reinterpret_cast<hogatt_stream_t>(stream)), what);
+}
+
+void hogwild_paged_attention_q4(at::Tensor& out, double scale, const at::Tensor& locations, const at::Tensor& queries,
+                                const at::Tensor& fragment_lengths, const at::Tensor& key_cache, const at::Tensor& value_cache,
+                                const at::Tensor& key_scales, const at::Tensor& value_scales, const at::Tensor& block_table, double key_unit,
+                                double value_unit, const std::optional<at::Tensor>& status) {
+    run_paged_q4("hogwild_paged_sdpa_q4", out, scale, locations, queries, fragment_lengths, key_cache, value_cache, key_scales, value_scales,
+                 block_table, nullptr, key_unit, value_unit, status);
+}
+
+void hogwild_varlen_paged_attention_q4(at::Tensor& out, double scale, const at::Tensor& locations, const at::Tensor& queries,
+                                       const at::Tensor& fragment_lengths, const at::Tensor& key_cache, const at::Tensor& value_cache,
+                                       const at::Tensor& key_scales, const at::Tensor& value_scales, const at::Tensor& block_table,
+                                       const at::Tensor& cu_seqlens_q, double key_unit, double value_unit, const std::optional<at::Tensor>& status) {
+    run_paged_q4("hogwild_varlen_paged_sdpa_q4", out, scale, locations, queries, fragment_lengths, key_cache, value_cache, key_scales, value_scales,
+                 block_table, &cu_seqlens_q, key_unit, value_unit, status);
+}
+
+void copy_to_blocks_q4(const at::Tensor& key_states, const at::Tensor& value_states, at::Tensor& key_cache, at::Tensor& value_cache,
+                       at::Tensor& key_scales, at::Tensor& value_scales, const at::Tensor& block_table, const at::Tensor& seq_lengths,
+                       const std::optional<at::Tensor>& cu_seqlens, const std::optional<at::Tensor>& new_rows, double key_unit, double value_unit,
+                       const std::optional<at::Tensor>& status) {
+    const char* what = "copy_to_blocks_q4";
+    TORCH_CHECK(key_states.is_cuda(), "libhogatt: tensors must live on a CUDA device");
+    const c10::cuda::CUDAGuard guard(key_states.device());
+    const c10::Device device = key_states.device();
+    const bool packed = cu_seqlens.has_value();
+    const int dim = packed ? 3 : 4;                       // [T,Hkv,E] or [B,Hkv,S,E]
+    TORCH_CHECK(key_states.dim() == dim && value_states.dim() == dim, what, ": states are [B,Hkv,S,E], with cu_seqlens [T,Hkv,E]");
+    TORCH_CHECK(value_states.device() == device && value_states.scalar_type() == key_states.scalar_type(), what, ": keys and values must agree in dtype and device");
+    for (int i = 0; i + 1 < dim; ++i) TORCH_CHECK_EQ(value_states.size(i), key_states.size(i));
+    const Q4Cache c = check_q4_cache(what, key_cache, value_cache, key_scales, value_scales, block_table, device);
+    TORCH_CHECK(key_states.size(dim - 1) == c.E && value_states.size(dim - 1) == c.Ev, what, ": head sizes of states and caches differ");
+    TORCH_CHECK_EQ(key_states.size(1), c.Hkv);
+    const int64_t B = block_table.size(0), S = packed ? key_states.size(0) : key_states.size(2);
+    TORCH_CHECK(packed || key_states.size(0) == B, what, ": block_table must have a row per sequence");
+    TORCH_CHECK(S <= INT32_MAX, what, ": too many tokens");
+    hogatt_q4_append p = {};
+    p.B = (int32_t)B; p.Hkv = c.Hkv; p.S = (int32_t)S; p.E = c.E; p.Ev = c.Ev;
+    p.block_size = c.block_size; p.num_blocks = c.num_blocks; p.max_blocks = (int32_t)block_table.size(1);
+    p.dtype = dtype_code(key_states);
+    p.key_unit = (float)key_unit;
+    p.value_unit = (float)value_unit;
+    p.seq_lengths = int_vector(what, "seq_lengths", seq_lengths, B, device);
+    p.cu_seqlens = int_vector(what, "cu_seqlens", cu_seqlens, B + 1, device);
+    p.new_rows = int_vector(what, "new_rows", new_rows, B, device);
+    p.device_status = status_word(what, status, device);
+    if (B == 0 || S == 0) return;
+    // (the last axis has to be dense; other strides are taken as they are)
+    const at::Tensor keys = key_states.stride(dim - 1) == 1 ? key_states : key_states.contiguous();
+    const at::Tensor values = value_states.stride(dim - 1) == 1 ? value_states : value_states.contiguous();
+    p.keys = keys.const_data_ptr();
+    p.values = values.const_data_ptr();
+    for (int i = 0; i < 3; ++i) {
+        p.key_strides[i] = packed ? (i == 0 ? 0 : keys.stride(i == 1 ? 1 : 0)) : keys.stride(i);
+        p.value_strides[i] = packed ? (i == 0 ? 0 : values.stride(i == 1 ? 1 : 0)) : values.stride(i);
+    }
+    p.key_cache = key_cache.data_ptr();
+    p.value_cache = value_cache.data_ptr();
+    p.key_scales = key_scales.data_ptr();
+    p.value_scales = value_scales.data_ptr();
+    p.block_table = block_table.const_data_ptr<int>();
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream();
+    check_status(hogatt_copy_to_blocks_q4_launch(&p, reinterpret_cast<hogatt_stream_t>(stream)), what);
+}
+
+void copy_from_blocks_q4(at::Tensor& keys, at::Tensor& values, const at::Tensor& key_cache, const at::Tensor& value_cache,
+                         const at::Tensor& key_scales, const at::Tensor& value_scales, const at::Tensor& block_table, const at::Tensor& first_rows,
+                         double key_unit, double value_unit, const std::optional<at::Tensor>& status) {
+    const char* what = "copy_from_blocks_q4";
+    TORCH_CHECK(keys.is_cuda(), "libhogatt: tensors must live on a CUDA device");
+    const c10::cuda::CUDAGuard guard(keys.device());
+    const c10::Device device = keys.device();
+    TORCH_CHECK(keys.dim() == 4 && values.dim() == 4 && keys.is_contiguous() && values.is_contiguous() && values.device() == device &&
+                    values.scalar_type() == keys.scalar_type(), what, ": keys and values must be contiguous [B,Hkv,S,E] of one dtype on one device");
+    for (int i = 0; i < 3; ++i) TORCH_CHECK_EQ(values.size(i), keys.size(i));
+    const Q4Cache c = check_q4_cache(what, key_cache, value_cache, key_scales, value_scales, block_table, device);
+    TORCH_CHECK(keys.size(3) == c.E && values.size(3) == c.Ev, what, ": head sizes of rows and caches differ");
+    TORCH_CHECK_EQ(keys.size(1), c.Hkv);
+    TORCH_CHECK_EQ(block_table.size(0), keys.size(0));
+    TORCH_CHECK(keys.size(2) <= INT32_MAX, what, ": too many rows");
+    hogatt_q4_read p = {};
+    p.B = (int32_t)keys.size(0); p.Hkv = c.Hkv; p.S = (int32_t)keys.size(2); p.E = c.E; p.Ev = c.Ev;
+    p.block_size = c.block_size; p.num_blocks = c.num_blocks; p.max_blocks = (int32_t)block_table.size(1);
+    p.dtype = dtype_code(keys);
+    p.key_unit = (float)key_unit;
+    p.value_unit = (float)value_unit;
+    p.keys = keys.data_ptr();
+    p.values = values.data_ptr();
+    p.key_cache = key_cache.const_data_ptr();
+    p.value_cache = value_cache.const_data_ptr();
+    p.key_scales = key_scales.const_data_ptr();
+    p.value_scales = value_scales.const_data_ptr();
+    p.block_table = block_table.const_data_ptr<int>();
+    p.first_rows = int_vector(what, "first_rows", first_rows, p.B, device);
+    p.device_status = status_word(what, status, device);
+    if (p.B == 0 || p.S == 0) return;
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream();
+    check_status(hogatt_copy_from_blocks_q4_launch(&p, reinterpret_cast<hogatt_stream_t>(stream)), what);
+}
+
+struct BlockTensors {
+    c10::SmallVector<void*, 64> data;
+    c10::SmallVector<int64_t, 64> bytes;
+    hogatt_block_tensors view() const { return {(int32_t)data.size(), data.data(), bytes.data()}; }
+};
+BlockTensors block_tensors(const char* what, at::TensorList caches, int64_t num_blocks, c10::Device device) {
+    BlockTensors b;
+    for (const at::Tensor& t : caches) {
+        TORCH_CHECK(t.device() == device && t.is_contiguous() && t.dim() > 0 && t.size(0) == num_blocks,
+                    what, ": caches must be contiguous [", num_blocks, ",...] tensors on the counts' device, not ", t.sizes());
+        TORCH_CHECK(t.numel() > 0, what, ": an empty cache");
+        b.data.push_back(t.data_ptr());
+        b.bytes.push_back(t.numel() / num_blocks * (int64_t)t.element_size());
+    }
+    return b;
+}
+int* int_output(const char* what, const char* name, at::Tensor& t, at::IntArrayRef sizes, c10::Device device) {
+    TORCH_CHECK(t.device() == device && t.sizes() == sizes && t.is_contiguous() && t.scalar_type() == at::kInt,
+                what, ": ", name, " must be contiguous int32 ", sizes);
+    return t.data_ptr<int>();
+}
+
+void step_blocks(const at::Tensor& block_refs, const at::Tensor& block_table, const at::Tensor& seq_lengths, const std::optional<at::Tensor>& source,
+                 const std::optional<at::Tensor>& new_tokens, int64_t block_size, at::TensorList caches, at::Tensor& refs_out, at::Tensor& table_out,
+                 at::Tensor& lengths_out, at::Tensor& room, const std::optional<at::Tensor>& status) {
+    const char* what = "step_blocks";
+    TORCH_CHECK(block_refs.is_cuda(), "libhogatt: tensors must live on a CUDA device");
+    const c10::cuda::CUDAGuard guard(block_refs.device());
+    const c10::Device device = block_refs.device();
+    TORCH_CHECK(block_table.device() == device && block_table.dim() == 2 && block_table.is_contiguous() && block_table.scalar_type() == at::kInt,
+                what, ": block_table must be contiguous int32 [W,max_blocks]");
+    TORCH_CHECK(block_refs.dim() == 1 && block_refs.size(0) <= INT32_MAX && block_table.size(1) <= INT32_MAX && block_size > 0 && block_size <= INT32_MAX &&
+                    block_table.size(0) <= HOGATT_MAX_BLOCK_ROWS && (!source.has_value() || (source->dim() == 1 && source->size(0) <= HOGATT_MAX_BLOCK_ROWS)),
+                what, ": block_refs [NumBlocks], at most ", HOGATT_MAX_BLOCK_ROWS, " rows, a positive block size");
+    const int64_t rows_in = block_table.size(0), rows_out = source.has_value() ? source->size(0) : rows_in;
+    hogatt_step_blocks p = {};
+    p.num_blocks = (int32_t)block_refs.size(0); p.block_size = (int32_t)block_size; p.max_blocks = (int32_t)block_table.size(1);
+    p.rows_in = (int32_t)rows_in; p.rows_out = (int32_t)rows_out;
+    p.refs_in = int_vector(what, "block_refs", block_refs, block_refs.size(0), device);
+    p.table_in = block_table.const_data_ptr<int>();
+    p.lengths_in = int_vector(what, "seq_lengths", seq_lengths, rows_in, device);
+    p.source = int_vector(what, "source", source, rows_out, device);
+    p.new_tokens = int_vector(what, "new_tokens", new_tokens, rows_out, device);
+    p.refs_out = int_output(what, "refs_out", refs_out, {block_refs.size(0)}, device);
+    p.table_out = int_output(what, "table_out", table_out, {rows_out, block_table.size(1)}, device);
+    p.lengths_out = int_output(what, "lengths_out", lengths_out, {rows_out}, device);
+    p.room = int_output(what, "room", room, {rows_out}, device);
+    const BlockTensors tensors = block_tensors(what, caches, block_refs.size(0), device);
+    p.caches = tensors.view();
+    p.device_status = status_word(what, status, device);
+    const size_t need = hogatt_step_blocks_workspace_bytes((int32_t)rows_out);
+    TORCH_CHECK(need > 0, what, ": no rows");
+    at::Tensor workspace = at::empty({(int64_t)need}, block_refs.options().dtype(at::kByte));
+    p.workspace = workspace.data_ptr();
+    p.workspace_bytes = need;
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream();
+    check_status(hogatt_step_blocks_launch(&p, reinterpret_cast<hogatt_stream_t>(stream)), what);
+}
+
+void compact_blocks(const at::Tensor& block_refs, const at::Tensor& block_table, at::TensorList caches, at::Tensor& refs_out, at::Tensor& table_out,
+                    at::Tensor& moved, const std::optional<at::Tensor>& status) {
+    const char* what = "compact_blocks";
+    TORCH_CHECK(block_refs.is_cuda(), "libhogatt: tensors must live on a CUDA device");
+    const c10::cuda::CUDAGuard guard(block_refs.device());
+    const c10::Device device = block_refs.device();
+    TORCH_CHECK(block_refs.dim() == 1 && block_refs.size(0) <= INT32_MAX, what, ": block_refs must be int32 [NumBlocks]");
+    TORCH_CHECK(block_table.device() == device && block_table.is_contiguous() && block_table.scalar_type() == at::kInt,
+                what, ": block_table must be contiguous int32");
+    hogatt_compact_blocks p = {};
+    p.num_blocks = (int32_t)block_refs.size(0);
+    p.table_entries = block_table.numel();
+    p.refs_in = int_vector(what, "block_refs", block_refs, block_refs.size(0), device);
+    p.table_in = block_table.const_data_ptr<int>();
+    p.refs_out = int_output(what, "refs_out", refs_out, {block_refs.size(0)}, device);
+    p.table_out = int_output(what, "table_out", table_out, block_table.sizes(), device);
+    p.moved = int_output(what, "moved", moved, {block_refs.size(0)}, device);
+    TORCH_CHECK(p.moved != p.refs_in && p.moved != p.refs_out, what, ": moved must be a buffer of its own");
+    const BlockTensors tensors = block_tensors(what, caches, block_refs.size(0), device);
+    p.caches = tensors.view();
+    p.device_status = status_word(what, status, device);
+    const size_t need = hogatt_compact_blocks_workspace_bytes(p.num_blocks);
+    TORCH_CHECK(need > 0, what, ": no blocks");
+    at::Tensor workspace = at::empty({(int64_t)need}, block_refs.options().dtype(at::kByte));
+    p.workspace = workspace.data_ptr();
+    p.workspace_bytes = need;
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream();
+    check_status(hogatt_compact_blocks_launch(&p, reinterpret_cast<hogatt_stream_t>(stream)), what);
+}
+
 }  // namespace
 
 extern "C" {
@@ -490,6 +786,24 @@ TORCH_LIBRARY(libhogatt, m) {
           "Tensor(d!) status) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
     m.def("fragment_step_plan(Tensor order, Tensor fragment_lengths, Tensor inv_freq, Tensor(a!) locations, Tensor(b!) cosines, "
           "Tensor(c!) sines, float attention_scaling, int round_tables_to) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
+    // a paged cache in 4 bits
+    m.def("hogwild_paged_sdpa_q4(Tensor(a!) output, float scale, Tensor locations, Tensor queries, Tensor fragment_lengths, Tensor key_cache, "
+          "Tensor value_cache, Tensor key_scales, Tensor value_scales, Tensor block_table, float key_unit, float value_unit, "
+          "Tensor(b!)? status) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("hogwild_varlen_paged_sdpa_q4(Tensor(a!) output, float scale, Tensor locations, Tensor queries, Tensor fragment_lengths, "
+          "Tensor key_cache, Tensor value_cache, Tensor key_scales, Tensor value_scales, Tensor block_table, Tensor cu_seqlens_q, "
+          "float key_unit, float value_unit, Tensor(b!)? status) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("copy_to_blocks_q4(Tensor key_states, Tensor value_states, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor(c!) key_scales, "
+          "Tensor(d!) value_scales, Tensor block_table, Tensor seq_lengths, Tensor? cu_seqlens, Tensor? new_rows, float key_unit, "
+          "float value_unit, Tensor(e!)? status) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("copy_from_blocks_q4(Tensor(a!) keys, Tensor(b!) values, Tensor key_cache, Tensor value_cache, Tensor key_scales, Tensor value_scales, "
+          "Tensor block_table, Tensor first_rows, float key_unit, float value_unit, Tensor(c!)? status) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
+    // ... and the pages of a paged cache of any type
+    m.def("step_blocks(Tensor block_refs, Tensor block_table, Tensor seq_lengths, Tensor? source, Tensor? new_tokens, int block_size, "
+          "Tensor(a!)[] caches, Tensor(b!) refs_out, Tensor(c!) table_out, Tensor(d!) lengths_out, Tensor(e!) room, Tensor(f!)? status) -> ()",
+          tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("compact_blocks(Tensor block_refs, Tensor block_table, Tensor(a!)[] caches, Tensor(b!) refs_out, Tensor(c!) table_out, "
+          "Tensor(d!) moved, Tensor(e!)? status) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
 }
 
 TORCH_LIBRARY_IMPL(libhogatt, CUDA, m) {
@@ -502,4 +816,10 @@ TORCH_LIBRARY_IMPL(libhogatt, CUDA, m) {
     m.impl("hogwild_fused_planned", hogwild_fused_planned);
     m.impl("fragment_append", fragment_append);
     m.impl("fragment_step_plan", fragment_step_plan);
+    m.impl("hogwild_paged_sdpa_q4", hogwild_paged_attention_q4);
+    m.impl("hogwild_varlen_paged_sdpa_q4", hogwild_varlen_paged_attention_q4);
+    m.impl("copy_to_blocks_q4", copy_to_blocks_q4);
+    m.impl("copy_from_blocks_q4", copy_from_blocks_q4);
+    m.impl("step_blocks", step_blocks);
+    m.impl("compact_blocks", compact_blocks);
 }
