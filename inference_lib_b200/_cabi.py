@@ -390,6 +390,38 @@ def bind_paged(*, out, queries, locations, fragment_lengths, key_cache, value_ca
     return p, [ws, out, queries, locations, fragment_lengths, key_cache, value_cache, block_table, cu_seqlens_q, status]
 
 
+def bind_paged_q4(*, key_scales, value_scales, key_unit=1.0, value_unit=1.0, out, queries, key_cache, value_cache, block_table, locations,
+                  fragment_lengths, scale, cu_seqlens_q=None, kernel=KERNEL_AUTO, status=None):
+    """:func:`bind_paged` for a 4-bit cache (codes as the caches).  Returns ``(problem, keepalive)``, ``(None, None)`` where the library refuses."""
+    import torch
+    x = PagedQ4Problem()
+    p = x.paged
+    if cu_seqlens_q is not None:
+        p.F, p.total_q_tokens, p.Hq, p.E = queries.shape
+        p.W = cu_seqlens_q.numel() - 1
+    else:
+        p.F, p.W, p.Hq, p.S, p.E = queries.shape
+    p.num_blocks, p.Hkv, p.block_size, p.Ev = key_cache.shape[0], key_cache.shape[1], key_cache.shape[2], value_cache.shape[3] * 2
+    p.max_blocks_per_seq = block_table.shape[1]
+    p.dtype, p.scale, p.kernel = dtype_code(out.dtype), float(scale), int(kernel)
+    p.out, p.queries, p.locations, p.fragment_lengths = (t.data_ptr() for t in (out, queries, locations, fragment_lengths))
+    p.key_cache, p.value_cache, p.block_table = key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr()
+    x.key_scales, x.value_scales, x.key_unit, x.value_unit = key_scales.data_ptr(), value_scales.data_ptr(), key_unit, value_unit
+    p.cu_seqlens_q = cu_seqlens_q.data_ptr() if cu_seqlens_q is not None else None
+    p.device_status = status.data_ptr() if status is not None else None
+    need = int(load().hogatt_paged_q4_workspace_bytes(C.byref(x)))
+    if need == 0:
+        return None, None
+    ws = torch.empty(need + 256, dtype=torch.uint8, device=out.device)
+    p.workspace, p.workspace_bytes = ws.data_ptr() + (-ws.data_ptr()) % 256, need
+    return x, [ws, out, queries, locations, fragment_lengths, key_cache, value_cache, key_scales, value_scales, block_table, cu_seqlens_q, status]
+
+
+def launch_paged_q4(problem: PagedQ4Problem, stream: int = 0) -> int:
+    """``hogatt_paged_q4_sdpa_launch``: enqueue one call; returns the library's status code."""
+    return int(load().hogatt_paged_q4_sdpa_launch(C.byref(problem), C.c_void_p(stream)))
+
+
 def launch_paged(problem: PagedProblem, stream: int = 0) -> int:
     """``hogatt_paged_sdpa_launch``: enqueue one call; returns the library's status code."""
     return int(load().hogatt_paged_sdpa_launch(C.byref(problem), C.c_void_p(stream)))

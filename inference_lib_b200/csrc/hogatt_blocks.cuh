@@ -15,32 +15,6 @@ namespace hogatt {
 
 constexpr int kBlocksCluster = 8, kBlocksThreads = 1024;
 
-// exclusive prefix of `x` over the CTA's threads; the total comes back in *total.  Called by all threads.
-__device__ __forceinline__ int block_exclusive(int x, int* total) {
-    __shared__ int warp_sum[32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int inc = x;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += y;
-    }
-    __syncthreads();                                      // (the array may still be in use from the last call)
-    if (lane == 31) warp_sum[warp] = inc;
-    __syncthreads();
-    if (warp == 0) {
-        int s = warp_sum[lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, s, o);
-            if (lane >= o) s += y;
-        }
-        warp_sum[lane] = s;
-    }
-    __syncthreads();
-    *total = warp_sum[31];
-    return inc - x + (warp ? warp_sum[warp - 1] : 0);
-}
 // this CTA's share [begin, end) of `n` things
 __device__ __forceinline__ void cluster_share(int n, int* begin, int* end) {
     const int rank = cluster_ctarank(), ctas = cluster_nctarank();

@@ -7,6 +7,7 @@
 #include "hogatt_host.h"
 #include "hogatt_blocks.cuh"
 #include "hogatt_q4.cuh"
+#include "hogatt_q4_mma.cuh"
 
 namespace hogatt {
 namespace {
@@ -25,9 +26,16 @@ int cache_shape(int Hkv, int E, int Ev, int block_size, int max_blocks, int num_
 }
 
 struct Q4Plan {
+    int kernel;                     // HOGATT_KERNEL_FMA or HOGATT_KERNEL_MMA
     int tokens_per_group, head_blocks, groups_bound, units, splits;
-    size_t o, m, l, total;
+    int rows;                       // (MMA) query rows of a unit at most
+    int ctas;                       // (MMA) shares of the list of tiles; 0: a CTA per unit
+    size_t o, m, l, plan, total;
 };
+
+// Units beyond this many per resident CTA get a CTA each: the list's shares then hold several units, whose ends (the eight warps' fold, the next
+// unit's first copies) do not overlap inside a CTA, and the merge step is saved.
+constexpr int kQ4UnitsPerCta = 4;
 
 int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
     if (x == nullptr) return HOGATT_ERR_NULL_POINTER;
@@ -38,25 +46,63 @@ int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
     if (const int rc = cache_shape(p->Hkv, p->E, p->Ev, p->block_size, p->max_blocks_per_seq, p->num_blocks, p->dtype)) return rc;
     if (p->Ev != 32 && p->Ev != 64 && p->Ev != 128 && p->Ev != 256) return HOGATT_ERR_UNSUPPORTED_HEAD_DIM;
     if (p->F > 4096) return HOGATT_ERR_TOO_MANY_FRAGMENTS;
-    if (p->kernel != HOGATT_KERNEL_AUTO && p->kernel != HOGATT_KERNEL_FMA) return HOGATT_ERR_BAD_KERNEL_CHOICE;
+    const bool mma = p->dtype != HOGATT_F32 && p->E == p->Ev && (p->E == 64 || p->E == 128);
+    if (p->kernel != HOGATT_KERNEL_AUTO && p->kernel != HOGATT_KERNEL_FMA && !(p->kernel == HOGATT_KERNEL_MMA && mma)) return HOGATT_ERR_BAD_KERNEL_CHOICE;
+    pl->kernel = mma && p->kernel != HOGATT_KERNEL_FMA ? HOGATT_KERNEL_MMA : HOGATT_KERNEL_FMA;
     if (!packed && (int64_t)p->F * p->W * p->S >= ((int64_t)1 << 31)) return HOGATT_ERR_TOO_LARGE;
     if (packed && (int64_t)p->F * std::max(p->total_q_tokens, p->W) >= ((int64_t)1 << 31)) return HOGATT_ERR_TOO_LARGE;
-    const int G = p->Hq / p->Hkv;
-    pl->tokens_per_group = G >= 16 ? 1 : 16 / G;
+    const int G = p->Hq / p->Hkv, most = G >= 16 ? 1 : 16 / G;
+    // (tokens that a sequence is likely to have: a group of more would be empty rows; one of fewer is another reader of the same keys)
+    const int64_t tokens = packed ? ((int64_t)p->total_q_tokens + p->W - 1) / p->W : p->S;
+    pl->tokens_per_group = pl->kernel == HOGATT_KERNEL_MMA ? (int)std::max<int64_t>(1, std::min<int64_t>(most, tokens)) : most;
     pl->head_blocks = (G + 15) / 16;
+    pl->rows = std::min(G, 16) * pl->tokens_per_group;
     const int64_t groups = packed ? ((int64_t)p->total_q_tokens + pl->tokens_per_group - 1) / pl->tokens_per_group + p->W
                                   : (int64_t)p->W * ((p->S + pl->tokens_per_group - 1) / pl->tokens_per_group);
     const int64_t units = groups * pl->head_blocks * p->Hkv;
     if (units > (1 << 24)) return HOGATT_ERR_TOO_LARGE;
     pl->groups_bound = (int)groups;
     pl->units = (int)std::max<int64_t>(units, 1);
-    pl->splits = std::max(1, std::min(24, (3 * sms + pl->units - 1) / pl->units));      // (24: the merge step's one round trip)
-    const size_t slots = (size_t)pl->units * pl->splits * kFmaRows;
+    size_t slots;
+    if (pl->kernel == HOGATT_KERNEL_MMA) {
+        pl->splits = 0;
+        pl->ctas = pl->units > kQ4UnitsPerCta * kQ4Ctas * sms ? 0 : kQ4Ctas * sms;
+        slots = pl->ctas ? ((size_t)pl->units + pl->ctas) * kFmaRows : 0;
+    } else {
+        pl->ctas = 0;
+        pl->splits = std::max(1, std::min(24, (3 * sms + pl->units - 1) / pl->units));      // (24: the merge step's one round trip)
+        slots = (size_t)pl->units * pl->splits * kFmaRows;
+    }
     pl->o = 0;
     pl->m = pl->o + align_up(slots * p->Ev * sizeof(float), 256);
     pl->l = pl->m + align_up(slots * sizeof(float), 256);
-    pl->total = pl->l + align_up(slots * sizeof(float), 256);
+    pl->plan = pl->l + align_up(slots * sizeof(float), 256);
+    pl->total = pl->plan + align_up(((size_t)pl->groups_bound + 1) * sizeof(int), 256);
     return HOGATT_OK;
+}
+
+FastDiv fast_div_by(uint32_t d) {
+    uint32_t shift = 0;
+    while (shift < 32 && ((uint64_t)1 << shift) < d) ++shift;
+    return {(uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1), shift, d};
+}
+
+template <class T, int HD, int NT, bool ALIGNED>
+int launch_q4_mma(const Q4MmaArgs& x, const Q4Plan& pl, int dev, int smem_optin, cudaStream_t stream) {
+    static std::atomic<size_t> granted[kMaxDevices];
+    const size_t smem = q4_mma_smem_bytes<HD>(NT, x.p.W, pl.groups_bound, x.ctas > 0);
+    if (smem > (size_t)smem_optin) return HOGATT_ERR_TOO_LARGE;
+    const int rc = ensure_smem_limit(q4_mma_kernel<T, HD, NT, ALIGNED>, dev, smem, granted);
+    if (rc != HOGATT_OK) return rc;
+    HOGATT_CUDA_OK(launch_kernel(q4_mma_kernel<T, HD, NT, ALIGNED>, dim3(x.ctas ? x.ctas : pl.units), dim3(kQ4Threads), smem, stream, x));
+    if (x.ctas) HOGATT_CUDA_OK(launch_kernel(q4_mma_merge_kernel<T, HD>, dim3(pl.units, pl.rows), dim3(128), 0, stream, x));
+    return HOGATT_OK;
+}
+template <class T, int HD>
+int launch_q4_mma_rows(const Q4MmaArgs& x, const Q4Plan& pl, int dev, int smem_optin, cudaStream_t stream) {
+    const bool aligned = x.p.block_size % 16 == 0;
+    if (pl.rows <= 8) return aligned ? launch_q4_mma<T, HD, 1, true>(x, pl, dev, smem_optin, stream) : launch_q4_mma<T, HD, 1, false>(x, pl, dev, smem_optin, stream);
+    return aligned ? launch_q4_mma<T, HD, 2, true>(x, pl, dev, smem_optin, stream) : launch_q4_mma<T, HD, 2, false>(x, pl, dev, smem_optin, stream);
 }
 
 template <class T>
@@ -78,6 +124,17 @@ int launch_q4_fma(const Q4Args& x, const Q4Plan& pl, int dev, int smem_optin, cu
 
 template <class T>
 int launch_q4(const Q4Args& x, const Q4Plan& pl, int dev, int smem_optin, cudaStream_t stream) {
+    if constexpr (!std::is_same<T, float>::value) {
+        if (pl.kernel == HOGATT_KERNEL_MMA) {
+            Q4MmaArgs y;
+            y.p = x.p;
+            y.kscale = x.kscale; y.vscale = x.vscale; y.num_blocks = x.num_blocks; y.vunit = x.vunit;
+            y.block = fast_div_by((uint32_t)x.p.block_size);
+            y.ctas = pl.ctas;
+            y.plan = x.plan;
+            return x.p.E == 128 ? launch_q4_mma_rows<T, 128>(y, pl, dev, smem_optin, stream) : launch_q4_mma_rows<T, 64>(y, pl, dev, smem_optin, stream);
+        }
+    }
     switch (x.p.Ev) {
         case 32: return launch_q4_fma<T, 32>(x, pl, dev, smem_optin, stream);
         case 64: return launch_q4_fma<T, 64>(x, pl, dev, smem_optin, stream);
@@ -200,6 +257,7 @@ int hogatt_paged_q4_sdpa_launch(const hogatt_paged_q4_problem* x, hogatt_stream_
     args.vscale = static_cast<const unsigned char*>(x->value_scales);
     args.num_blocks = p->num_blocks;
     args.vunit = x->value_unit;
+    args.plan = reinterpret_cast<int*>(ws + pl.plan);
     switch (p->dtype) {
         case HOGATT_F32: return launch_q4<float>(args, pl, dev, smem_optin, stream);
         case HOGATT_F16: return launch_q4<__half>(args, pl, dev, smem_optin, stream);

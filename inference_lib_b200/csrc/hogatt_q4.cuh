@@ -64,6 +64,32 @@ __device__ __forceinline__ long long paged_row_at(const int* table, int pos, int
     return ((long long)page * Hkv + h) * block_size + (pos - at * block_size);
 }
 
+// exclusive prefix of `x` over the CTA's threads; the total comes back in *total.  Called by all threads.
+__device__ __forceinline__ int block_exclusive(int x, int* total) {
+    __shared__ int warp_sum[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+    }
+    __syncthreads();                                      // (the array may still be in use from the last call)
+    if (lane == 31) warp_sum[warp] = inc;
+    __syncthreads();
+    if (warp == 0) {
+        int s = lane < (int)(blockDim.x >> 5) ? warp_sum[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += y;
+        }
+        warp_sum[lane] = s;
+    }
+    __syncthreads();
+    *total = warp_sum[31];
+    return inc - x + (warp ? warp_sum[warp - 1] : 0);
+}
 struct Q4AppendArgs {
     int B, Hkv, S, E, Ev, block_size, max_blocks, num_blocks;
     int packed_tokens;            // packed layout: rows of the source; fixed layout: 0
@@ -215,6 +241,7 @@ struct Q4Args {
     const unsigned char* vscale;
     int num_blocks;
     float vunit;                  // (the keys' unit is in p.l2scale)
+    int* plan;                    // (the tensor-core kernel's)
 };
 
 // Any type, any head size: the units, splits and partials of paged_attention_kernel and its arithmetic, rows unpacked to fp32 as they are

@@ -1,0 +1,667 @@
+// Attention over 4-bit pages on the tensor cores, few query rows per kv head (decode, short chunks): f16 / bf16, E == Ev == 64 or 128.
+//
+// Bound by HBM: 9/8 byte per (key, channel) of K and V together, 144 bytes per key and kv head at head size 128, against 512 in
+// 16 bits -- so what a key costs on the SM counts: at the full copy rate an SM has to finish one every six cycles.
+//
+// Both products are taken transposed, keys or value channels as the M of mma.sync m16n8k16 and up to eight query rows as its N:
+//     S^T [16 keys x 8 rows] = K [16 x E] Q^T,      O^T [E x 8 rows] += V^T [E x 16 keys] P^T
+// With rows as the M (16) and four heads per kv head three quarters of the products would be padding.  The 4-bit operand is the A
+// operand of both; its fragments are unpacked from shared memory straight into registers, two values per conversion:
+//   * K: the order of a product's channels is free as long as Q has the same, so a thread's A fragments of all steps are 32 (16)
+//     consecutive channels of two keys: one 16-byte (8-byte) load each, and two scales (one).
+//   * V^T: a thread's rows of all tiles are the 16 (8) consecutive channels of one scale group, for four keys; pairs of keys at one
+//     channel are put together from two words with masks and a shift.
+// Values times scales are exact in fp16 (six significant bits), so the only rounding is that of P.  bf16 queries are brought to fp16 by a
+// power of two per row, which loses nothing a float accumulator would keep: magnitudes down to 2^-39 of the row's largest are held.
+// P goes from the accumulators of the first product to the B operand of the second by movmatrix.
+//
+// Every warp works alone: 16 keys of each 128-key tile, fetched by its own cp.async copies into its own ring, its own running maximum and
+// sum; the eight warps meet only where a unit ends.  Rows are looked up in the block table one tile ahead of their copies.  O is
+// rescaled only when some score exceeds the row's reference by 2^7 (P then stays below 128 in fp16).
+//
+// Split: units (<= 16 query rows that share keys, kv head) are cut into 128-key tiles, all units' tiles are one list, every CTA takes an
+// equal contiguous share (two CTAs per SM).  A share's part of a unit is a partial; q4_mma_merge_kernel adds them up.  With many more units than
+// CTAs each unit gets a CTA of its own, and no merge step.
+#pragma once
+#include "hogatt_q4.cuh"
+
+namespace hogatt {
+
+constexpr int kQ4Warps = 8, kQ4Threads = kQ4Warps * 32, kQ4Tile = kQ4Warps * 16, kQ4Ctas = 2;
+
+// n / d for 0 <= n < 2^31
+struct FastDiv {
+    uint32_t mul, shift, d;
+};
+__device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv& f) { return (__umulhi(n, f.mul) + n) >> f.shift; }
+
+struct Q4MmaArgs {
+    PagedArgs p;                  // kcache / vcache: the codes; splits: unused; groups_bound: entries of the prefix
+    const unsigned char* kscale;
+    const unsigned char* vscale;
+    int num_blocks;
+    float vunit;
+    FastDiv block;                // block size
+    int ctas;                     // the list's shares; 0: a CTA per unit
+    int* plan;                    // [groups_bound + 1]: tiles of a kv head's units in front of every group of query tokens
+};
+
+template <int HD>
+struct Q4MmaCfg {
+    static constexpr int ROW = HD / 2, SROW = HD / kGroup;         // bytes of a row's codes and scales
+    static constexpr int STAGE = 16 * 2 * (ROW + SROW) + 16;       // K, V, K scales, V scales of 16 keys; which have no page
+    static constexpr int OFF_V = 16 * ROW, OFF_KS = 32 * ROW, OFF_VS = OFF_KS + 16 * SROW, OFF_BAD = OFF_VS + 16 * SROW;
+    static constexpr int NSTAGE = HD == 128 ? 5 : 8;
+    static constexpr int RING = kQ4Warps * NSTAGE * STAGE;
+    static constexpr int PITCH = HD + 4;                           // floats between rows of the fold
+    static constexpr int fold_bytes(int rows) { return kQ4Warps * rows * (PITCH + 2) * 4; }
+    static constexpr int work_bytes(int nt) { return RING > fold_bytes(8 * nt) ? RING : fold_bytes(8 * nt); }
+};
+template <int HD>
+__host__ __device__ inline size_t q4_mma_smem_bytes(int nt, int W, int groups, bool list) {
+    return Q4MmaCfg<HD>::work_bytes(nt) + (list ? ((size_t)W + 1 + groups + 1) * sizeof(int) : 0);
+}
+
+// the 8x8 matrix of 16-bit elements that the warp holds (row lane / 4, columns 2 (lane % 4) and + 1), transposed
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// `n` of 16 (8, 4) bytes copied, the others zeros
+template <int BYTES>
+__device__ __forceinline__ void cp_async_zfill(uint32_t dst, const void* src, bool real) {
+    const int n = real ? BYTES : 0;
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+
+// Visible keys of (group of query tokens, fragment): the most that any of its rows sees.
+__device__ __forceinline__ int group_visible(const PagedArgs& a, int f, int w, int s_base, int s_begin, int s_end) {
+    int top = -1;
+    for (int s = s_begin; s < s_end; ++s) top = max(top, a.loc[(size_t)f * a.loc_f + (size_t)w * a.loc_w + s_base + s]);
+    return max(0, min(top, a.flen[f * a.len_f + w * a.len_w] - 1) + 1);
+}
+__device__ __forceinline__ int tokens_of(const PagedArgs& a, int w, int* start) {
+    *start = a.cu_seqlens ? a.cu_seqlens[w] : 0;
+    return a.cu_seqlens ? max(0, min(a.cu_seqlens[w + 1], a.total_q) - *start) : a.S;
+}
+
+// Sequence, tokens and heads of unit x, by a whole warp (32 sequences at a time).
+__device__ __forceinline__ bool locate_unit(const PagedArgs& a, int x, PagedUnit* u) {
+    const int lane = threadIdx.x & 31;
+    u->hkv = x % a.Hkv;
+    const int y = x / a.Hkv;
+    u->g0 = (y % a.head_blocks) * 16;
+    int grp = y / a.head_blocks;
+    for (int w0 = 0; w0 < a.W; w0 += 32) {
+        const int w = w0 + lane;
+        int start = 0;
+        const int n = w < a.W ? tokens_of(a, w, &start) : 0;
+        const int ng = (n + a.tokens_per_group - 1) / a.tokens_per_group;
+        int inc = ng;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int z = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += z;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, grp < inc);
+        if (here) {
+            const int src = __ffs(here) - 1;
+            grp -= __shfl_sync(0xffffffffu, inc - ng, src);
+            u->w = w0 + src;
+            u->s_base = __shfl_sync(0xffffffffu, start, src);
+            u->s_begin = grp * a.tokens_per_group;
+            u->s_end = min(__shfl_sync(0xffffffffu, n, src), u->s_begin + a.tokens_per_group);
+            return true;
+        }
+        grp -= __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return false;
+}
+
+template <class T, int HD, int NT, bool ALIGNED>
+__global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __grid_constant__ Q4MmaArgs x) {
+    using C = Q4MmaCfg<HD>;
+    constexpr int KS = HD / 16;              // steps of S^T = tiles of O^T
+    constexpr int CPT = HD / 4, DPT = HD / 8;        // channels of a key, of a value that a thread holds
+    const PagedArgs& a = x.p;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    unsigned char* const ring = smem_raw + warp * C::NSTAGE * C::STAGE;
+    const uint32_t ring_u32 = smem_u32(ring);
+    int* const first_group = reinterpret_cast<int*>(smem_raw + C::work_bytes(NT));      // [W + 1]
+    int* const pre = first_group + a.W + 1;                                              // [groups + 1]
+    const unsigned char* const kc = static_cast<const unsigned char*>(a.kcache);
+    const unsigned char* const vc = static_cast<const unsigned char*>(a.vcache);
+    const int per_group = a.Hkv * a.head_blocks;          // units of a group of query tokens
+
+    pdl_wait();
+    pdl_trigger();
+
+    // ---- the list: tiles of every group, and this CTA's share ----
+    int64_t item = 0, item_end = 0;
+    int groups = 0;
+    if (x.ctas) {
+        int before = 0;
+        for (int w0 = 0; w0 < a.W; w0 += kQ4Threads) {
+            int start, n = 0, total;
+            if (w0 + tid < a.W) n = (tokens_of(a, w0 + tid, &start) + a.tokens_per_group - 1) / a.tokens_per_group;
+            const int at = before + block_exclusive(n, &total);
+            if (w0 + tid < a.W) first_group[w0 + tid] = at;
+            before += total;
+        }
+        groups = min(before, a.groups_bound);
+        if (tid == 0) first_group[a.W] = before;
+        __syncthreads();
+        before = 0;
+        for (int e0 = 0; e0 < groups; e0 += kQ4Threads) {
+            const int e = e0 + tid;
+            int n = 0, total;
+            if (e < groups) {
+                int lo = 0, hi = a.W;                     // the sequence: the last one that starts at or in front of e
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (first_group[mid] <= e) lo = mid;
+                    else hi = mid;
+                }
+                int start;
+                const int tokens = tokens_of(a, lo, &start), s0 = (e - first_group[lo]) * a.tokens_per_group;
+                for (int f = 0; f < a.F; ++f) n += ceil_div(group_visible(a, f, lo, start, s0, min(tokens, s0 + a.tokens_per_group)), kQ4Tile);
+            }
+            const int at = before + block_exclusive(n, &total);
+            if (e < groups) pre[e] = at;
+            before += total;
+        }
+        if (tid == 0) pre[groups] = before;
+        __syncthreads();
+        if (blockIdx.x == 0)
+            for (int e = tid; e <= a.groups_bound; e += kQ4Threads) x.plan[e] = pre[min(e, groups)];
+        const int64_t N = (int64_t)before * per_group;
+        const int shares = effective_ctas(N, x.ctas);     // none of them empty
+        if ((int)blockIdx.x >= shares) return;
+        item = cta_first_tile(blockIdx.x, N, shares);
+        item_end = cta_first_tile(blockIdx.x + 1, N, shares);
+    }
+
+    int grp = 0;
+    bool again = true;
+    while (again) {
+        // ---- the next unit of the share: its tiles [j0, j1) ----
+        PagedUnit u;
+        int unit = blockIdx.x, j0 = 0, j1 = INT_MAX;
+        if (x.ctas) {
+            int lo = grp, hi = groups;                    // the group: the last one that starts at or in front of `item`, with tiles
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if ((int64_t)pre[mid] * per_group <= item) lo = mid;
+                else hi = mid;
+            }
+            grp = lo;
+            const int n = pre[grp + 1] - pre[grp];
+            const int64_t off = item - (int64_t)pre[grp] * per_group;
+            const int of_group = (int)floor_div(off, n);
+            unit = grp * per_group + of_group;
+            j0 = (int)(off - (int64_t)of_group * n);
+            j1 = (int)min((int64_t)n, j0 + (item_end - item));
+            item += j1 - j0;
+            again = item < item_end;
+            int wl = 0, wh = a.W;
+            while (wh - wl > 1) {
+                const int mid = (wl + wh) >> 1;
+                if (first_group[mid] <= grp) wl = mid;
+                else wh = mid;
+            }
+            int start;
+            const int tokens = tokens_of(a, wl, &start);
+            u.w = wl;
+            u.s_base = start;
+            u.s_begin = (grp - first_group[wl]) * a.tokens_per_group;
+            u.s_end = min(tokens, u.s_begin + a.tokens_per_group);
+            u.hkv = of_group % a.Hkv;
+            u.g0 = of_group / a.Hkv * 16;
+        } else {
+            again = false;
+            if (!locate_unit(a, unit, &u)) return;        // (uniform: the grid is an upper bound)
+        }
+        const int* const table = a.block_table + (size_t)u.w * a.max_blocks;
+
+        float o[NT][KS][4];
+        float m[NT][2], l[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) o[n][k][0] = o[n][k][1] = o[n][k][2] = o[n][k][3] = 0.f;
+        }
+
+        int tiles_before = 0;
+        bool whole = true;                                // this CTA has all of the unit's tiles
+        for (int f = 0; f < a.F; ++f) {
+            // ---- this fragment's tiles of the share ----
+            const int vis = group_visible(a, f, u.w, u.s_base, u.s_begin, u.s_end);
+            const int tiles = ceil_div(vis, kQ4Tile);
+            const int b0 = max(j0, tiles_before) - tiles_before, b1 = min(j1, tiles_before + tiles) - tiles_before;
+            whole = whole && (tiles == 0 || (b0 == 0 && b1 == tiles));
+            tiles_before += tiles;
+            if (b0 >= b1) continue;
+
+            // ---- its query rows as B fragments: thread (g, t) has channels CPT t ... of row g of each eight ----
+            uint32_t q[NT][KS][2];
+            float factor[NT][2];                          // what a product of columns 2 t, 2 t + 1 is multiplied with: log2 e * scale / row's power
+            int lim[NT][2], lowest = INT_MAX;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                int s_abs, hq;
+                const bool real = paged_row(a, u, n * 8 + g, &s_abs, &hq);
+                uint4 raw[CPT / 8];
+#pragma unroll
+                for (int k = 0; k < CPT / 8; ++k) raw[k] = make_uint4(0u, 0u, 0u, 0u);
+                if (real) {
+                    const T* src = static_cast<const T*>(a.q) + f * a.q_f + u.w * a.q_w + s_abs * a.q_s + hq * a.q_h + t * CPT;
+#pragma unroll
+                    for (int k = 0; k < CPT / 8; ++k) {
+                        const int4 v = load_16(src + k * 8);
+                        raw[k] = make_uint4(v.x, v.y, v.z, v.w);
+                    }
+                }
+                float mine = a.l2scale;
+                const uint32_t* r = reinterpret_cast<const uint32_t*>(raw);
+                if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        q[n][k][0] = r[2 * k];
+                        q[n][k][1] = r[2 * k + 1];
+                    }
+                } else {
+                    uint32_t top = 0;                     // the largest magnitude's bits: bf16 in the upper half
+#pragma unroll
+                    for (int k = 0; k < CPT / 2; ++k) top = max(top, max(r[k] & 0x7fff0000u, (r[k] & 0x7fffu) << 16));
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    // times 2^e so that the largest lies in [2^14, 2^15); an infinity or a NaN makes the row NaN
+                    const int e = min(120, 14 - ((int)(top >> 23) - 127));
+                    const float up = top >= 0x7f800000u ? NAN : __int_as_float((e + 127) << 23);
+                    mine *= top >= 0x7f800000u ? NAN : __int_as_float((127 - e) << 23);
+#pragma unroll
+                    for (int k = 0; k < CPT / 2; ++k) {
+                        const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&r[k]);
+                        q[n][k / 2][k & 1] = pack2<__half>(__low2float(v) * up, __high2float(v) * up);
+                    }
+                }
+                int mylim = INT_MAX;                      // (a row that is not there is never masked, nor stored)
+                if (real) {
+                    const int loc = a.loc[(size_t)f * a.loc_f + (size_t)u.w * a.loc_w + s_abs];
+                    mylim = max(0, min(loc, a.flen[f * a.len_f + u.w * a.len_w] - 1) + 1);
+                }
+                lowest = min(lowest, mylim);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {             // row 2 t + c is lane 8 t + 4 c's
+                    lim[n][c] = __shfl_sync(0xffffffffu, mylim, 8 * t + 4 * c);
+                    factor[n][c] = __shfl_sync(0xffffffffu, mine, 8 * t + 4 * c);
+                }
+            }
+#pragma unroll
+            for (int k = 4; k < 32; k <<= 1) lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, k));
+
+            // ---- copies of 16 keys: rows of 4 (2) 16-byte chunks, dealt over the lanes; scales of K by lanes 0-15, of V by 16-31 ----
+            constexpr int CPR = C::ROW / 16, PASSES = 16 * CPR / 32, RPP = 32 / CPR;
+            int page[PASSES + 1];                         // of this lane's rows, and of its scales' row; -1: none
+            auto look_up = [&](int j) {
+                const int k0 = j * kQ4Tile + warp * 16;
+                auto page_of = [&](int key) {
+                    const int at = (int)fast_div((uint32_t)key, x.block);
+                    if (key >= vis) return -1;
+                    const int p = at < a.max_blocks ? table[at] : -1;
+                    return p >= 0 && p < x.num_blocks ? p : -2;        // -2: a key without a page
+                };
+                if constexpr (ALIGNED) {                  // 16 keys from a multiple of 16 lie in one block
+                    page[0] = page_of(k0);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < PASSES; ++i) page[i] = page_of(k0 + i * RPP + lane / CPR);
+                    page[PASSES] = page_of(k0 + (lane & 15));
+                }
+            };
+            auto fetch = [&](int j, int stage) {
+                const int k0 = j * kQ4Tile + warp * 16;
+                const uint32_t base = ring_u32 + stage * C::STAGE;
+                auto row_of = [&](int key, int p) {       // (an address inside the cache whatever the page)
+                    const int off = key - (int)(fast_div((uint32_t)key, x.block) * x.block.d);
+                    return ((int64_t)max(p, 0) * a.Hkv + u.hkv) * a.block_size + off;
+                };
+#pragma unroll
+                for (int i = 0; i < PASSES; ++i) {
+                    const int r = i * RPP + lane / CPR, c = lane % CPR, p = ALIGNED ? page[0] : page[i];
+                    const bool real = p >= 0 && k0 + r < vis;
+                    const int64_t at = row_of(k0 + r, p) * C::ROW + c * 16;
+                    const uint32_t dst = base + r * C::ROW + (HD == 128 ? (c ^ (r & 2)) * 16 : c * 16);
+                    cp_async_zfill<16>(dst, kc + at, real);
+                    cp_async_zfill<16>(dst + C::OFF_V, vc + at, real);
+                }
+                const int r = lane & 15, p = ALIGNED ? page[0] : page[PASSES];
+                const int64_t at = row_of(k0 + r, p) * C::SROW;
+                cp_async_zfill<C::SROW>(base + (lane < 16 ? C::OFF_KS : C::OFF_VS) + r * C::SROW, (lane < 16 ? x.kscale : x.vscale) + at, p >= 0 && k0 + r < vis);
+                cp_async_commit();
+                const uint32_t bad = __ballot_sync(0xffffffffu, p == -2 && k0 + r < vis) & 0xffffu;
+                if (lane == 0) *reinterpret_cast<uint32_t*>(ring + stage * C::STAGE + C::OFF_BAD) = bad;
+                if (bad && lane == 0 && a.status) atomicOr(a.status, STATUS_BAD_BLOCK);
+            };
+
+            // ---- the walk ----
+            look_up(b0);
+#pragma unroll 1
+            for (int k = 0; k < C::NSTAGE - 1; ++k) {
+                if (b0 + k < b1) {
+                    fetch(b0 + k, k);
+                    if (b0 + k + 1 < b1) look_up(b0 + k + 1);
+                } else {
+                    cp_async_commit();
+                }
+            }
+            int stage = 0;
+#pragma unroll 1
+            for (int j = b0; j < b1; ++j) {
+                cp_async_wait<C::NSTAGE - 2>();
+                __syncwarp();                             // every lane's copies have landed, and every lane has left the last stage
+                {
+                    const int ahead = j + C::NSTAGE - 1;
+                    if (ahead < b1) {
+                        fetch(ahead, stage == 0 ? C::NSTAGE - 1 : stage - 1);
+                        if (ahead + 1 < b1) look_up(ahead + 1);
+                    } else {
+                        cp_async_commit();
+                    }
+                }
+                const unsigned char* const s = ring + stage * C::STAGE;
+                if (++stage == C::NSTAGE) stage = 0;
+                const int k0 = j * kQ4Tile + warp * 16;
+                if (k0 >= vis) continue;
+                // row i of the product is key i with the last bit flipped in every second four: the loads of V below then hit all banks
+                const int ka = g ^ ((g >> 2) & 1), kb = ka + 8;
+
+                float c[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+                {
+                    uint32_t wa[CPT / 8], wb[CPT / 8], sa, sb;
+                    if constexpr (HD == 128) {
+                        *reinterpret_cast<uint4*>(wa) = *reinterpret_cast<const uint4*>(s + ka * 64 + ((t ^ (ka & 2)) * 16));
+                        *reinterpret_cast<uint4*>(wb) = *reinterpret_cast<const uint4*>(s + kb * 64 + ((t ^ (kb & 2)) * 16));
+                        sa = from_e4m3x2(*reinterpret_cast<const uint16_t*>(s + C::OFF_KS + ka * 8 + t * 2));
+                        sb = from_e4m3x2(*reinterpret_cast<const uint16_t*>(s + C::OFF_KS + kb * 8 + t * 2));
+                    } else {
+                        *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(s + ka * 32 + t * 8);
+                        *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(s + kb * 32 + t * 8);
+                        sa = from_e4m3x2(s[C::OFF_KS + ka * 4 + t]);
+                        sb = from_e4m3x2(s[C::OFF_KS + kb * 4 + t]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        const uint32_t ya = __byte_perm(sa, sa, k < KS / 2 || HD == 64 ? 0x1010 : 0x3232);
+                        const uint32_t yb = __byte_perm(sb, sb, k < KS / 2 || HD == 64 ? 0x1010 : 0x3232);
+                        const uint32_t va = wa[k / 2] >> (k & 1) * 16, vb = wb[k / 2] >> (k & 1) * 16;
+                        const uint32_t frag[4] = {mul_half2(from_e2m1x2(va), ya), mul_half2(from_e2m1x2(vb), yb),
+                                                  mul_half2(from_e2m1x2(va >> 8), ya), mul_half2(from_e2m1x2(vb >> 8), yb)};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_16816<__half>(c[n], frag, q[n][k][0], q[n][k][1]);
+                    }
+                }
+                const uint32_t bad = *reinterpret_cast<const uint32_t*>(s + C::OFF_BAD);
+                const bool edge = k0 + 16 > lowest || bad != 0;
+                bool grow = false;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) c[n][i] *= factor[n][i & 1];
+                    if (edge) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int key = i < 2 ? ka : kb;
+                            if (k0 + key >= lim[n][i & 1] || (bad >> key & 1)) c[n][i] = -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) grow = grow || fmaxf(c[n][i], c[n][i + 2]) > m[n][i] + 7.f;
+                }
+                if (__any_sync(0xffffffffu, grow)) {      // (rare behind the first tiles) every row's reference becomes its maximum so far
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float top = fmaxf(m[n][i], fmaxf(c[n][i], c[n][i + 2]));
+#pragma unroll
+                            for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+                            const float down = top == -INFINITY ? 1.f : exp2_fast(m[n][i] - top);
+                            m[n][i] = top;
+                            l[n][i] *= down;
+#pragma unroll
+                            for (int k = 0; k < KS; ++k) {
+                                o[n][k][i] *= down;
+                                o[n][k][i + 2] *= down;
+                            }
+                        }
+                }
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) c[n][i] = exp2_fast(c[n][i] - (m[n][i & 1] == -INFINITY ? 0.f : m[n][i & 1]));
+                    l[n][0] += c[n][0] + c[n][2];
+                    l[n][1] += c[n][1] + c[n][3];
+                    pb[n][0] = movmatrix(pack2<__half>(c[n][0], c[n][1]));
+                    pb[n][1] = movmatrix(pack2<__half>(c[n][2], c[n][3]));
+                }
+                // ---- O^T += V^T P^T: columns of the product are keys 2 t, 2 t + 1 and eight further, in the order of the rows above ----
+                {
+                    const int flip = (t >> 1) & 1, v0 = 2 * t + flip, v1 = 2 * t + 1 - flip;
+                    uint32_t w[4][DPT / 8], sc[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = (i & 1 ? v1 : v0) + (i >> 1) * 8;
+                        if constexpr (HD == 128) {
+                            *reinterpret_cast<uint2*>(w[i]) = *reinterpret_cast<const uint2*>(s + C::OFF_V + key * 64 + (((g >> 1) ^ (key & 2)) * 16) + (g & 1) * 8);
+                            sc[i] = s[C::OFF_VS + key * 8 + g];
+                        } else {
+                            w[i][0] = *reinterpret_cast<const uint32_t*>(s + C::OFF_V + key * 32 + g * 4);
+                            sc[i] = s[C::OFF_VS + key * 4 + (g >> 1)];
+                        }
+                    }
+                    if (edge) {
+                        // a value that is not a number reaches the rows that see its key, and no others (0 * NaN would)
+                        uint32_t odd = 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (is_nan_e4m3(sc[i])) {
+                                odd |= 1u << ((i & 1 ? v1 : v0) + (i >> 1) * 8);
+                                sc[i] = 0u;
+                            }
+                        if (__any_sync(0xffffffffu, odd != 0)) {
+                            odd |= __shfl_xor_sync(0xffffffffu, odd, 1);
+                            odd |= __shfl_xor_sync(0xffffffffu, odd, 2);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    const int seen = max(0, min(16, lim[n][i] - k0));
+                                    if (odd & ((1u << seen) - 1u) & ~bad) {
+#pragma unroll
+                                        for (int k = 0; k < KS; ++k) o[n][k][i] = o[n][k][i + 2] = NAN;
+                                    }
+                                }
+                        }
+                    }
+                    const uint32_t ya = from_e4m3x2(sc[0] | sc[1] << 8), yb = from_e4m3x2(sc[2] | sc[3] << 8);
+#pragma unroll
+                    for (int h = 0; h < DPT / 8; ++h) {
+                        // byte k: channel 2 k of both keys, and channel 2 k + 1
+                        const uint32_t a0 = (w[0][h] & 0x0f0f0f0fu) | ((w[1][h] << 4) & 0xf0f0f0f0u), a1 = ((w[0][h] >> 4) & 0x0f0f0f0fu) | (w[1][h] & 0xf0f0f0f0u);
+                        const uint32_t b0_ = (w[2][h] & 0x0f0f0f0fu) | ((w[3][h] << 4) & 0xf0f0f0f0u), b1_ = ((w[2][h] >> 4) & 0x0f0f0f0fu) | (w[3][h] & 0xf0f0f0f0u);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t frag[4] = {mul_half2(from_e2m1x2(a0 >> 8 * k), ya), mul_half2(from_e2m1x2(a1 >> 8 * k), ya),
+                                                      mul_half2(from_e2m1x2(b0_ >> 8 * k), yb), mul_half2(from_e2m1x2(b1_ >> 8 * k), yb)};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma_16816<__half>(o[n][h * 4 + k], frag, pb[n][0], pb[n][1]);
+                        }
+                    }
+                }
+            }
+            cp_async_wait<0>();
+            __syncwarp();
+        }
+
+        // ---- the eight warps' results become one ----
+        __syncthreads();                                  // (the fold lies on the rings)
+        float* const fold = reinterpret_cast<float*>(smem_raw);
+        float* const fold_m = fold + kQ4Warps * 8 * NT * C::PITCH;
+        float* const fold_l = fold_m + kQ4Warps * 8 * NT;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float sum = l[n][i];
+#pragma unroll
+                for (int k = 4; k < 32; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+                const int row = warp * 8 * NT + n * 8 + 2 * t + i;
+                float* dst = fold + row * C::PITCH + g * DPT;
+#pragma unroll
+                for (int k = 0; k < KS; k += 2)
+                    *reinterpret_cast<float4*>(dst + 2 * k) = make_float4(o[n][k][i], o[n][k][i + 2], o[n][k + 1][i], o[n][k + 1][i + 2]);
+                if (g == 0) {
+                    fold_m[row] = m[n][i];
+                    fold_l[row] = sum;
+                }
+            }
+        __syncthreads();
+        for (int i = tid; i < 8 * NT * (HD / 4); i += kQ4Threads) {
+            const int r = i / (HD / 4), col = (i - r * (HD / 4)) * 4;
+            int s_abs, hq;
+            if (!paged_row(a, u, r, &s_abs, &hq)) continue;
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kQ4Warps; ++w) M = fmaxf(M, fold_m[w * 8 * NT + r]);
+            const float mu = M == -INFINITY ? 0.f : M;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float L = 0.f;
+#pragma unroll
+            for (int w = 0; w < kQ4Warps; ++w) {
+                const float wgt = exp2_fast(fold_m[w * 8 * NT + r] - mu);
+                const float4 v = *reinterpret_cast<const float4*>(fold + (w * 8 * NT + r) * C::PITCH + col);
+                acc.x = fmaf(v.x, wgt, acc.x);
+                acc.y = fmaf(v.y, wgt, acc.y);
+                acc.z = fmaf(v.z, wgt, acc.z);
+                acc.w = fmaf(v.w, wgt, acc.w);
+                L = fmaf(fold_l[w * 8 * NT + r], wgt, L);
+            }
+            if (whole) {
+                const float inv = L == 0.f ? 0.f : x.vunit / L;
+                store4<T>(static_cast<T*>(a.out) + u.w * a.o_w + s_abs * a.o_s + hq * a.o_h + col, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            } else {
+                const size_t slot = (size_t)blockIdx.x + unit;            // (both only grow along the list)
+                *reinterpret_cast<float4*>(a.ws_o + (slot * kFmaRows + r) * HD + col) = acc;
+                if (col == 0) {
+                    a.ws_m[slot * kFmaRows + r] = M;
+                    a.ws_l[slot * kFmaRows + r] = L;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Adds up the partials of one output row (one CTA): warp w takes every fourth, a lane four (two) columns.  Units that one CTA had to
+// itself are stored already; rows that see nothing, of which the list has no tile, are zeros.
+template <class T, int HD>
+__global__ void __launch_bounds__(128) q4_mma_merge_kernel(const __grid_constant__ Q4MmaArgs x) {
+    constexpr int VEC = HD / 32;
+    const PagedArgs& a = x.p;
+    __shared__ float sm_m[4], sm_l[4], sm_o[4][HD];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, unit = blockIdx.x, row = blockIdx.y;
+    const int per_group = a.Hkv * a.head_blocks, grp = unit / per_group;
+    pdl_wait();
+    pdl_trigger();
+    PagedUnit u;
+    const int before = __ldcg(x.plan + grp), n = __ldcg(x.plan + grp + 1) - before;
+    const int64_t N = (int64_t)__ldcg(x.plan + a.groups_bound) * per_group;
+    int first = 0, count = 0;
+    if (n > 0) {
+        const int64_t start = (int64_t)before * per_group + (int64_t)(unit - grp * per_group) * n;
+        const int shares = effective_ctas(N, x.ctas);
+        first = cta_of_tile(start, N, shares);
+        count = cta_of_tile(start + n - 1, N, shares) - first + 1;
+        if (count == 1) return;
+    }
+    if (!locate_unit(a, unit, &u)) return;
+    int s_abs, hq;
+    if (!paged_row(a, u, row, &s_abs, &hq)) return;
+    T* const out = static_cast<T*>(a.out) + u.w * a.o_w + s_abs * a.o_s + hq * a.o_h;
+    float M = -INFINITY, L = 0.f, acc[VEC] = {};
+    for (int p0 = warp; p0 < count; p0 += 32) {           // eight partials of a warp in flight
+        float mp[8], lp[8], v[8][VEC];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const size_t at = ((size_t)(first + p0 + 4 * k) + unit) * kFmaRows + row;
+            const bool have = p0 + 4 * k < count;
+            mp[k] = have ? __ldcg(a.ws_m + at) : -INFINITY;
+            lp[k] = have ? __ldcg(a.ws_l + at) : 0.f;
+            if constexpr (VEC == 4) {
+                const float4 y = have ? __ldcg(reinterpret_cast<const float4*>(a.ws_o + at * HD + lane * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[k][0] = y.x; v[k][1] = y.y; v[k][2] = y.z; v[k][3] = y.w;
+            } else {
+                const float2 y = have ? __ldcg(reinterpret_cast<const float2*>(a.ws_o + at * HD + lane * 2)) : make_float2(0.f, 0.f);
+                v[k][0] = y.x; v[k][1] = y.y;
+            }
+        }
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, mp[k]);
+        const float mu = top == -INFINITY ? 0.f : top, down = exp2_fast(M - mu);
+        M = top;
+        L *= down;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] *= down;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float wgt = exp2_fast(mp[k] - mu);
+            L = fmaf(lp[k], wgt, L);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[i] = fmaf(v[k][i], wgt, acc[i]);
+        }
+    }
+    if (lane == 0) {
+        sm_m[warp] = M;
+        sm_l[warp] = L;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sm_o[warp][lane * VEC + i] = acc[i];
+    __syncthreads();
+    if (warp != 0) return;
+    float top = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
+    const float mu = top == -INFINITY ? 0.f : top;
+    L = 0.f;
+    float r[VEC] = {};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float wgt = exp2_fast(sm_m[w] - mu);
+        L = fmaf(sm_l[w], wgt, L);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) r[i] = fmaf(sm_o[w][lane * VEC + i], wgt, r[i]);
+    }
+    const float inv = L == 0.f ? 0.f : x.vunit / L;
+    if constexpr (VEC == 4) store4<T>(out + lane * 4, r[0] * inv, r[1] * inv, r[2] * inv, r[3] * inv);
+    else *reinterpret_cast<uint32_t*>(out + lane * 2) = pack2<T>(r[0] * inv, r[1] * inv);
+}
+
+}  // namespace hogatt

@@ -182,7 +182,28 @@ def paged(A, q, loc, lens, cache, table, scale, units=(1.0, 1.0), cu=None, out=N
         exact = q4_util.attention(q, loc, lens, kc, vc, ks, vs, table, scale, *units, cu)
         got = A.hogwild_varlen_paged_sdpa_q4(*args, cu.to(DEV), out, **more)
     torch.cuda.synchronize()
+    if kernel is not None:                                   # the same by a kernel of the caller's choice, workspace full of NaN and canaries behind it
+        from inference_lib_b200 import _cabi
+        again = torch.full_like(got, float("nan")) if cu is not None else torch.full((q.shape[1], q.shape[2], q.shape[3], vc.shape[3] * 2), float("nan"),
+                                                                                       dtype=q.dtype, device=DEV)
+        x, keep = _cabi.bind_paged_q4(out=again, queries=args[0], locations=args[1], key_cache=args[2], value_cache=args[3], key_scales=args[4],
+                                      value_scales=args[5], block_table=args[6], scale=scale, fragment_lengths=args[8], key_unit=units[0],
+                                      value_unit=units[1], cu_seqlens_q=None if cu is None else cu.to(DEV), kernel=kernel)
+        keep[0].fill_(0xFF)
+        end = x.paged.workspace - keep[0].data_ptr() + x.paged.workspace_bytes
+        assert _cabi.launch_paged_q4(x, torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert bool((keep[0][end:] == 0xFF).all())
+        got = again if cu is not None else again.transpose(1, 2).reshape(got.shape)
     return got, exact
+
+
+KERNELS = [None, 1, 2]                                       # the operator; by name on the CUDA cores; mma.sync
+
+
+def skip_unless_eligible(kernel, dtype, E, Ev):
+    if kernel == 2 and (dtype == torch.float32 or E != Ev or E not in (64, 128)):
+        pytest.skip("not for this type and head size")
 
 
 SHAPES = [
@@ -204,8 +225,10 @@ SHAPES = [
 
 
 @pytest.mark.parametrize("case", SHAPES, ids=[str(i) for i in range(len(SHAPES))])
-def test_paged_attention(A, case):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_paged_attention(A, case, kernel):
     dtype, W, S, Hkv, G, E, Ev, bs, F, keys, units = case
+    skip_unless_eligible(kernel, dtype, E, Ev)
     gen, rng = torch.Generator().manual_seed(keys), np.random.default_rng(keys)
     width = -(-keys // bs) + 1
     blocks = W * width + 2
@@ -215,7 +238,7 @@ def test_paged_attention(A, case):
     lens = torch.tensor([keys] + [int(x) for x in rng.integers(0, keys + 1, F - 1)], dtype=torch.int32)
     loc = torch.from_numpy(rng.integers(-1, keys + 9, (F, W, S)).astype(np.int32))
     loc[0, 0] = keys - 1
-    got, exact = paged(A, q, loc, lens, (kc, vc, ks, vs), table, E ** -0.5 / units[0], units)
+    got, exact = paged(A, q, loc, lens, (kc, vc, ks, vs), table, E ** -0.5 / units[0], units, kernel=kernel)
     q4_util.check(got, exact)
 
 
@@ -232,8 +255,10 @@ PACKED = [
 
 @pytest.mark.parametrize("case", PACKED, ids=[str(i) for i in range(len(PACKED))])
 @pytest.mark.parametrize("causal", [True, False])
-def test_packed_attention(A, case, causal):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_packed_attention(A, case, causal, kernel):
     dtype, counts, Hkv, G, E, bs, F, keys, units = case
+    skip_unless_eligible(kernel, dtype, E, E)
     gen, rng = torch.Generator().manual_seed(keys), np.random.default_rng(keys)
     W, T, width = len(counts), sum(counts), -(-keys // bs) + 1
     blocks = W * width + 1
@@ -251,8 +276,8 @@ def test_packed_attention(A, case, causal):
     loc = torch.cat([loc, torch.full((F, 2), 5, dtype=torch.int32)], 1)
     out = torch.full((T + 2, Hkv * G, E), 7.0, dtype=dtype, device=DEV)
     st = status()
-    got, exact = paged(A, q, loc, lens, (kc, vc, ks, vs), table, E ** -0.5 / units[0], units, cu, out, st)
-    assert bool((got[T:] == 7.0).all()) and int(st) == 0
+    got, exact = paged(A, q, loc, lens, (kc, vc, ks, vs), table, E ** -0.5 / units[0], units, cu, out, st, kernel)
+    assert bool((out[T:] == 7.0).all()) and int(st) == 0
     q4_util.check(got[:T], (exact[0][:T], exact[1][:T], *exact[2:]))
 
 
@@ -264,8 +289,10 @@ def odd_scales(rng, cache, table, bs, spots):
 
 @pytest.mark.parametrize("dtype,E,counts,bs", [(torch.bfloat16, 128, [1, 1, 3], 16), (torch.float16, 64, [2, 1, 1], 24), (torch.float32, 64, [1, 2, 1], 16),
                                                (torch.bfloat16, 128, [130, 1, 20], 16)])
-def test_numbers_that_are_not(A, dtype, E, counts, bs):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_numbers_that_are_not(A, dtype, E, counts, bs, kernel):
     """A NaN key is the whole row's, a NaN value its channels', and only of rows that see it; behind the lengths there may be anything."""
+    skip_unless_eligible(kernel, dtype, E, E)
     gen, rng = torch.Generator().manual_seed(5), np.random.default_rng(5)
     Hkv, G, keys, W, T = 2, 4, 150, len(counts), sum(counts)
     width = -(-keys // bs)
@@ -280,23 +307,26 @@ def test_numbers_that_are_not(A, dtype, E, counts, bs):
     q[0, T - 1, 2, 5] = float("nan")
     q[0, 0, 6, 5] = float("inf")                                           # inf * 0 or inf - inf: NaN as well
     cu = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32)
-    got, exact = paged(A, q, loc, lens, cache, table, E ** -0.5, cu=cu)
+    got, exact = paged(A, q, loc, lens, cache, table, E ** -0.5, cu=cu, kernel=kernel)
     exact[0][T - 1, 2] = np.nan
     exact[0][0, 6] = np.nan
     q4_util.check(got, exact)
 
 
 @pytest.mark.parametrize("dtype,E,G", [(torch.bfloat16, 128, 4), (torch.float16, 64, 12), (torch.float32, 128, 2)])
-def test_keys_without_a_page_are_not_seen(A, dtype, E, G):
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("bs", [16, 8])
+def test_keys_without_a_page_are_not_seen(A, dtype, E, G, kernel, bs):
+    skip_unless_eligible(kernel, dtype, E, E)
     gen, rng = torch.Generator().manual_seed(6), np.random.default_rng(6)
-    W, Hkv, bs, keys = 3, 2, 16, 100
-    (kc, ks), (vc, vs) = (q4_util.random_cache(gen, 24, Hkv, bs, E) for _ in range(2))
-    table = table_of(rng, W, 6, 24)
-    table[0, 2], table[1, 0], table[2] = -1, 24, -7                        # a hole, a page outside, no page at all
+    W, Hkv, keys, width = 3, 2, 100, 96 // bs
+    (kc, ks), (vc, vs) = (q4_util.random_cache(gen, 4 * width, Hkv, bs, E) for _ in range(2))
+    table = table_of(rng, W, width, 4 * width)
+    table[0, 2], table[1, 0], table[2] = -1, 4 * width, -7                        # a hole, a page outside, no page at all
     q = torch.randn(1, W, Hkv * G, 2, E, generator=gen).to(dtype)
     loc = torch.tensor([[[98, 99], [20, 95], [50, 99]]], dtype=torch.int32)      # (keys 96 ... lie behind the table)
     st = status()
-    got, exact = paged(A, q, loc, torch.tensor([keys], dtype=torch.int32), (kc, vc, ks, vs), table, E ** -0.5, st=st)
+    got, exact = paged(A, q, loc, torch.tensor([keys], dtype=torch.int32), (kc, vc, ks, vs), table, E ** -0.5, st=st, kernel=kernel)
     q4_util.check(got, exact)
     assert int(st) == 1024 and bool((got.reshape(W, 2, -1)[2] == 0).all())
 
