@@ -23,6 +23,8 @@
 // equal contiguous share (two CTAs per SM).  A share's part of a unit is a partial; q4_mma_merge_kernel adds them up.  With many more units than
 // CTAs each unit gets a CTA of its own, and no merge step.
 #pragma once
+#include <float.h>
+
 #include "hogatt_q4.cuh"
 
 namespace hogatt {
@@ -55,7 +57,10 @@ struct Q4MmaCfg {
     static constexpr int RING = kQ4Warps * NSTAGE * STAGE;
     static constexpr int PITCH = HD + 4;                           // floats between rows of the fold
     static constexpr int fold_bytes(int rows) { return kQ4Warps * rows * (PITCH + 2) * 4; }
-    static constexpr int work_bytes(int nt) { return RING > fold_bytes(8 * nt) ? RING : fold_bytes(8 * nt); }
+    static constexpr int ring_bytes(int nt) { return RING > fold_bytes(8 * nt) ? RING : fold_bytes(8 * nt); }
+    // sixteen query rows do not fit in registers beside O: their fragments, the same for every warp, lie in shared memory
+    static constexpr int q_bytes(int nt) { return nt == 2 ? nt * (HD / 32) * 512 : 0; }
+    static constexpr int work_bytes(int nt) { return ring_bytes(nt) + q_bytes(nt); }
 };
 template <int HD>
 __host__ __device__ inline size_t q4_mma_smem_bytes(int nt, int W, int groups, bool list) {
@@ -77,6 +82,37 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// shared memory by its 32-bit address, `OFF` bytes further (generic pointers cost the loop an address per load)
+template <int OFF>
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4+%5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at), "n"(OFF));
+    return v;
+}
+template <int OFF>
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2+%3];" : "=r"(v.x), "=r"(v.y) : "r"(at), "n"(OFF));
+    return v;
+}
+template <int OFF>
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1+%2];" : "=r"(v) : "r"(at), "n"(OFF));
+    return v;
+}
+template <int OFF>
+__device__ __forceinline__ uint32_t lds16(uint32_t at) {
+    uint16_t v;
+    asm volatile("ld.shared.b16 %0, [%1+%2];" : "=h"(v) : "r"(at), "n"(OFF));
+    return v;
+}
+template <int OFF>
+__device__ __forceinline__ uint32_t lds8(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1+%2];" : "=r"(v) : "r"(at), "n"(OFF));
+    return v;
 }
 // `n` of 16 (8, 4) bytes copied, the others zeros
 template <int BYTES>
@@ -240,7 +276,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
         float m[NT][2], l[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            m[n][0] = m[n][1] = -INFINITY;
+            m[n][0] = m[n][1] = -FLT_MAX;                 // (nothing seen yet; finite, so that differences with it are)
             l[n][0] = l[n][1] = 0.f;
 #pragma unroll
             for (int k = 0; k < KS; ++k) o[n][k][0] = o[n][k][1] = o[n][k][2] = o[n][k][3] = 0.f;
@@ -258,7 +294,9 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
             if (b0 >= b1) continue;
 
             // ---- its query rows as B fragments: thread (g, t) has channels CPT t ... of row g of each eight ----
-            uint32_t q[NT][KS][2];
+            uint32_t q[NT == 1 ? KS : 1][2];
+            uint4* const q_smem = reinterpret_cast<uint4*>(smem_raw + C::ring_bytes(NT)) + lane;
+            if (NT == 2 && f > 0) __syncthreads();        // (every warp has left the last fragment)
             float factor[NT][2];                          // what a product of columns 2 t, 2 t + 1 is multiplied with: log2 e * scale / row's power
             int lim[NT][2], lowest = INT_MAX;
 #pragma unroll
@@ -276,15 +314,9 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
                         raw[k] = make_uint4(v.x, v.y, v.z, v.w);
                     }
                 }
-                float mine = a.l2scale;
-                const uint32_t* r = reinterpret_cast<const uint32_t*>(raw);
-                if constexpr (std::is_same<T, __half>::value) {
-#pragma unroll
-                    for (int k = 0; k < KS; ++k) {
-                        q[n][k][0] = r[2 * k];
-                        q[n][k][1] = r[2 * k + 1];
-                    }
-                } else {
+                float mine = fabsf(a.l2scale);
+                uint32_t* r = reinterpret_cast<uint32_t*>(raw);
+                if constexpr (!std::is_same<T, __half>::value) {
                     uint32_t top = 0;                     // the largest magnitude's bits: bf16 in the upper half
 #pragma unroll
                     for (int k = 0; k < CPT / 2; ++k) top = max(top, max(r[k] & 0x7fff0000u, (r[k] & 0x7fffu) << 16));
@@ -297,8 +329,23 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
 #pragma unroll
                     for (int k = 0; k < CPT / 2; ++k) {
                         const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&r[k]);
-                        q[n][k / 2][k & 1] = pack2<__half>(__low2float(v) * up, __high2float(v) * up);
+                        r[k] = pack2<__half>(__low2float(v) * up, __high2float(v) * up);
                     }
+                }
+                mine = fmaxf(mine, FLT_MIN);              // (a masked score is -inf and has to stay it; scores this small are none)
+                if (a.l2scale < 0.f) {                    // (the row's maximum is taken before the factor)
+#pragma unroll
+                    for (int k = 0; k < CPT / 2; ++k) r[k] ^= 0x80008000u;
+                }
+                if constexpr (NT == 1) {
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        q[k][0] = r[2 * k];
+                        q[k][1] = r[2 * k + 1];
+                    }
+                } else if (warp == 0) {
+#pragma unroll
+                    for (int k = 0; k < KS / 2; ++k) q_smem[(n * (KS / 2) + k) * 32] = raw[k];
                 }
                 int mylim = INT_MAX;                      // (a row that is not there is never masked, nor stored)
                 if (real) {
@@ -314,136 +361,193 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
             }
 #pragma unroll
             for (int k = 4; k < 32; k <<= 1) lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, k));
+            if (NT == 2) __syncthreads();
 
             // ---- copies of 16 keys: rows of 4 (2) 16-byte chunks, dealt over the lanes; scales of K by lanes 0-15, of V by 16-31 ----
             constexpr int CPR = C::ROW / 16, PASSES = 16 * CPR / 32, RPP = 32 / CPR;
-            int page[PASSES + 1];                         // of this lane's rows, and of its scales' row; -1: none
+            const int row0 = lane / CPR, srow = lane & 15;                 // this lane's first row, and its scales' row
+            const uint32_t dst0 = ring_u32 + row0 * C::ROW + (HD == 128 ? ((lane % CPR) ^ (row0 & 2)) * 16 : (lane % CPR) * 16);
+            const uint32_t sdst0 = ring_u32 + (lane < 16 ? C::OFF_KS : C::OFF_VS) + srow * C::SROW;
+            const unsigned char* const scales = lane < 16 ? x.kscale : x.vscale;
+            // Where key `key`'s row of codes begins in either cache, in bytes (its scales: an eighth of that); -1: behind the keys, -2: a
+            // key without a page.
+            auto row_of = [&](int key) -> int64_t {
+                if (key >= vis) return -1;
+                const int at = (int)fast_div((uint32_t)key, x.block);
+                const int p = at < a.max_blocks ? table[at] : -1;
+                if (p < 0 || p >= x.num_blocks) return -2;
+                return (((int64_t)p * a.Hkv + u.hkv) * a.block_size + (key - at * (int)x.block.d)) * C::ROW;
+            };
+            // ALIGNED: the 16 keys of a tile lie in one block, and the lanes look up 32 tiles at a time, the next 32 ahead of their use;
+            // otherwise every lane looks its rows of the next tile up
+            constexpr int LOOKUPS = ALIGNED ? 2 : PASSES + 1;
+            int64_t from[LOOKUPS];
+            int looked = b0;                              // ALIGNED: from[0] has tiles `looked` ..., from[1] the 32 behind them
             auto look_up = [&](int j) {
                 const int k0 = j * kQ4Tile + warp * 16;
-                auto page_of = [&](int key) {
-                    const int at = (int)fast_div((uint32_t)key, x.block);
-                    if (key >= vis) return -1;
-                    const int p = at < a.max_blocks ? table[at] : -1;
-                    return p >= 0 && p < x.num_blocks ? p : -2;        // -2: a key without a page
-                };
-                if constexpr (ALIGNED) {                  // 16 keys from a multiple of 16 lie in one block
-                    page[0] = page_of(k0);
+                if constexpr (ALIGNED) {
+                    if (j - looked == 32) {
+                        looked = j;
+                        from[0] = from[1];
+                        from[1] = row_of(k0 + (32 + lane) * kQ4Tile);
+                    }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < PASSES; ++i) page[i] = page_of(k0 + i * RPP + lane / CPR);
-                    page[PASSES] = page_of(k0 + (lane & 15));
+                    for (int i = 0; i < PASSES; ++i) from[i] = row_of(k0 + i * RPP + row0);
+                    from[PASSES] = row_of(k0 + srow);
                 }
             };
-            auto fetch = [&](int j, int stage) {
-                const int k0 = j * kQ4Tile + warp * 16;
-                const uint32_t base = ring_u32 + stage * C::STAGE;
-                auto row_of = [&](int key, int p) {       // (an address inside the cache whatever the page)
-                    const int off = key - (int)(fast_div((uint32_t)key, x.block) * x.block.d);
-                    return ((int64_t)max(p, 0) * a.Hkv + u.hkv) * a.block_size + off;
-                };
+            const unsigned char* const k_lane = kc + row0 * C::ROW + lane % CPR * 16;
+            const unsigned char* const v_lane = vc + row0 * C::ROW + lane % CPR * 16;
+            const unsigned char* const s_lane = scales + srow * C::SROW;
+            bool any_bad = false;                         // a tile with keys that have no page has been met: their bits are looked at
+            auto fetch = [&](int j, uint32_t base) {      // base: the stage's bytes from the ring's start
+                const int left = vis - (j * kQ4Tile + warp * 16);          // keys there are from here on
+                const int64_t tile_from = ALIGNED ? __shfl_sync(0xffffffffu, from[0], (j - looked) & 31) : 0;
+                if (ALIGNED && left >= 16 && tile_from >= 0) {
 #pragma unroll
-                for (int i = 0; i < PASSES; ++i) {
-                    const int r = i * RPP + lane / CPR, c = lane % CPR, p = ALIGNED ? page[0] : page[i];
-                    const bool real = p >= 0 && k0 + r < vis;
-                    const int64_t at = row_of(k0 + r, p) * C::ROW + c * 16;
-                    const uint32_t dst = base + r * C::ROW + (HD == 128 ? (c ^ (r & 2)) * 16 : c * 16);
-                    cp_async_zfill<16>(dst, kc + at, real);
-                    cp_async_zfill<16>(dst + C::OFF_V, vc + at, real);
+                    for (int i = 0; i < PASSES; ++i) {
+                        cp_async_16(dst0 + base + i * RPP * C::ROW, k_lane + tile_from + i * RPP * C::ROW, true);
+                        cp_async_16(dst0 + base + C::OFF_V + i * RPP * C::ROW, v_lane + tile_from + i * RPP * C::ROW, true);
+                    }
+                    cp_async_zfill<C::SROW>(sdst0 + base, s_lane + (tile_from >> 3), true);
+                    if (any_bad && lane == 0) *reinterpret_cast<uint32_t*>(ring + base + C::OFF_BAD) = 0u;
+                } else {                                  // (rows that are not there: zeros, from an address inside the cache)
+#pragma unroll
+                    for (int i = 0; i < PASSES; ++i) {
+                        const int64_t row = ALIGNED ? tile_from : from[i];
+                        const bool real = row >= 0 && row0 + i * RPP < left;
+                        const int64_t at = (real ? (ALIGNED ? row + (row0 + i * RPP) * C::ROW : row) : 0) + lane % CPR * 16;
+                        cp_async_zfill<16>(dst0 + base + i * RPP * C::ROW, kc + at, real);
+                        cp_async_zfill<16>(dst0 + base + C::OFF_V + i * RPP * C::ROW, vc + at, real);
+                    }
+                    const int64_t row = ALIGNED ? tile_from : from[LOOKUPS - 1];
+                    const bool real = row >= 0 && srow < left;
+                    cp_async_zfill<C::SROW>(sdst0 + base, scales + ((real ? (ALIGNED ? row + srow * C::ROW : row) : 0) >> 3), real);
+                    const uint32_t bad = __ballot_sync(0xffffffffu, row == -2 && srow < left) & 0xffffu;
+                    if (bad && lane == 0 && a.status) atomicOr(a.status, STATUS_BAD_BLOCK);
+                    any_bad = any_bad || bad != 0;
+                    if (any_bad && lane == 0) *reinterpret_cast<uint32_t*>(ring + base + C::OFF_BAD) = bad;
                 }
-                const int r = lane & 15, p = ALIGNED ? page[0] : page[PASSES];
-                const int64_t at = row_of(k0 + r, p) * C::SROW;
-                cp_async_zfill<C::SROW>(base + (lane < 16 ? C::OFF_KS : C::OFF_VS) + r * C::SROW, (lane < 16 ? x.kscale : x.vscale) + at, p >= 0 && k0 + r < vis);
                 cp_async_commit();
-                const uint32_t bad = __ballot_sync(0xffffffffu, p == -2 && k0 + r < vis) & 0xffffu;
-                if (lane == 0) *reinterpret_cast<uint32_t*>(ring + stage * C::STAGE + C::OFF_BAD) = bad;
-                if (bad && lane == 0 && a.status) atomicOr(a.status, STATUS_BAD_BLOCK);
             };
 
             // ---- the walk ----
-            look_up(b0);
+            if constexpr (ALIGNED) {
+                from[0] = row_of(b0 * kQ4Tile + warp * 16 + lane * kQ4Tile);
+                from[1] = row_of(b0 * kQ4Tile + warp * 16 + (32 + lane) * kQ4Tile);
+            } else {
+                look_up(b0);
+            }
+            // (a stage's bits of keys without a page are first read after a tile that has some has been met: zero until then)
+            if (lane < C::NSTAGE) *reinterpret_cast<uint32_t*>(ring + lane * C::STAGE + C::OFF_BAD) = 0u;
+            __syncwarp();
 #pragma unroll 1
             for (int k = 0; k < C::NSTAGE - 1; ++k) {
                 if (b0 + k < b1) {
-                    fetch(b0 + k, k);
+                    fetch(b0 + k, k * C::STAGE);
                     if (b0 + k + 1 < b1) look_up(b0 + k + 1);
                 } else {
                     cp_async_commit();
                 }
             }
-            int stage = 0;
+            // row i of the product is key i with the last bit flipped in every second four: the loads of V then hit all banks
+            const int ka = g ^ ((g >> 2) & 1), kb = ka + 8;
+            const int flip = (t >> 1) & 1, v0 = 2 * t + flip, v1 = 2 * t + 1 - flip;
+            const uint32_t k_at = ring_u32 + (HD == 128 ? ka * 64 + ((t ^ (ka & 2)) * 16) : ka * 32 + t * 8);
+            const uint32_t ks_at = ring_u32 + C::OFF_KS + ka * C::SROW + t * (HD / 64);
+            auto v_of = [&](int key) { return ring_u32 + C::OFF_V + key * C::ROW + (HD == 128 ? ((g >> 1) ^ (key & 2)) * 16 + (g & 1) * 8 : g * 4); };
+            const uint32_t va_at = v_of(v0), vb_at = v_of(v1), vs_at = ring_u32 + C::OFF_VS + v0 * C::SROW + (HD == 128 ? g : g >> 1);
+            const int vs_step = (v1 - v0) * C::SROW;
+            uint32_t base = 0, base_ahead = (C::NSTAGE - 1) * C::STAGE;
+            int k0 = b0 * kQ4Tile + warp * 16;
 #pragma unroll 1
-            for (int j = b0; j < b1; ++j) {
+            for (int j = b0; j < b1; ++j, k0 += kQ4Tile) {
                 cp_async_wait<C::NSTAGE - 2>();
                 __syncwarp();                             // every lane's copies have landed, and every lane has left the last stage
-                {
-                    const int ahead = j + C::NSTAGE - 1;
-                    if (ahead < b1) {
-                        fetch(ahead, stage == 0 ? C::NSTAGE - 1 : stage - 1);
-                        if (ahead + 1 < b1) look_up(ahead + 1);
-                    } else {
-                        cp_async_commit();
-                    }
+                const int ahead = j + C::NSTAGE - 1;
+                if (ahead < b1) {
+                    fetch(ahead, base_ahead);
+                    look_up(ahead + 1);
+                } else {
+                    cp_async_commit();
                 }
-                const unsigned char* const s = ring + stage * C::STAGE;
-                if (++stage == C::NSTAGE) stage = 0;
-                const int k0 = j * kQ4Tile + warp * 16;
+                const uint32_t s = base;
+                base_ahead = base;
+                base = base == (C::NSTAGE - 1) * C::STAGE ? 0u : base + C::STAGE;
                 if (k0 >= vis) continue;
-                // row i of the product is key i with the last bit flipped in every second four: the loads of V below then hit all banks
-                const int ka = g ^ ((g >> 2) & 1), kb = ka + 8;
 
                 float c[NT][4];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
                 {
+                    // one tile of rows: two chains of products, so that a step waits for the one before the last
+                    float d[NT][4];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+                        d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
+                    }
                     uint32_t wa[CPT / 8], wb[CPT / 8], sa, sb;
                     if constexpr (HD == 128) {
-                        *reinterpret_cast<uint4*>(wa) = *reinterpret_cast<const uint4*>(s + ka * 64 + ((t ^ (ka & 2)) * 16));
-                        *reinterpret_cast<uint4*>(wb) = *reinterpret_cast<const uint4*>(s + kb * 64 + ((t ^ (kb & 2)) * 16));
-                        sa = from_e4m3x2(*reinterpret_cast<const uint16_t*>(s + C::OFF_KS + ka * 8 + t * 2));
-                        sb = from_e4m3x2(*reinterpret_cast<const uint16_t*>(s + C::OFF_KS + kb * 8 + t * 2));
+                        *reinterpret_cast<uint4*>(wa) = lds128<0>(k_at + s);
+                        *reinterpret_cast<uint4*>(wb) = lds128<8 * C::ROW>(k_at + s);
+                        sa = from_e4m3x2(lds16<0>(ks_at + s));
+                        sb = from_e4m3x2(lds16<8 * C::SROW>(ks_at + s));
                     } else {
-                        *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(s + ka * 32 + t * 8);
-                        *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(s + kb * 32 + t * 8);
-                        sa = from_e4m3x2(s[C::OFF_KS + ka * 4 + t]);
-                        sb = from_e4m3x2(s[C::OFF_KS + kb * 4 + t]);
+                        *reinterpret_cast<uint2*>(wa) = lds64<0>(k_at + s);
+                        *reinterpret_cast<uint2*>(wb) = lds64<8 * C::ROW>(k_at + s);
+                        sa = from_e4m3x2(lds8<0>(ks_at + s));
+                        sb = from_e4m3x2(lds8<8 * C::SROW>(ks_at + s));
                     }
 #pragma unroll
-                    for (int k = 0; k < KS; ++k) {
+                    for (int k = 0; k < KS; k += 2) {     // a word of either key: two steps
                         const uint32_t ya = __byte_perm(sa, sa, k < KS / 2 || HD == 64 ? 0x1010 : 0x3232);
                         const uint32_t yb = __byte_perm(sb, sb, k < KS / 2 || HD == 64 ? 0x1010 : 0x3232);
-                        const uint32_t va = wa[k / 2] >> (k & 1) * 16, vb = wb[k / 2] >> (k & 1) * 16;
-                        const uint32_t frag[4] = {mul_half2(from_e2m1x2(va), ya), mul_half2(from_e2m1x2(vb), yb),
-                                                  mul_half2(from_e2m1x2(va >> 8), ya), mul_half2(from_e2m1x2(vb >> 8), yb)};
+                        uint32_t xa[4], xb[4];
+                        from_e2m1x8(wa[k / 2], xa);
+                        from_e2m1x8(wb[k / 2], xb);
+                        uint4 qq[NT];
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_16816<__half>(c[n], frag, q[n][k][0], q[n][k][1]);
+                        for (int n = 0; n < NT; ++n) {
+                            if constexpr (NT == 1) qq[n] = make_uint4(q[k][0], q[k][1], q[k + 1][0], q[k + 1][1]);
+                            else qq[n] = q_smem[(n * (KS / 2) + k / 2) * 32];
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t frag[4] = {mul_half2(xa[2 * h], ya), mul_half2(xb[2 * h], yb), mul_half2(xa[2 * h + 1], ya), mul_half2(xb[2 * h + 1], yb)};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma_16816<__half>(NT == 1 && h ? d[n] : c[n], frag, h ? qq[n].z : qq[n].x, h ? qq[n].w : qq[n].y);
+                        }
                     }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) c[n][i] += NT == 1 ? d[n][i] : 0.f;
                 }
-                const uint32_t bad = *reinterpret_cast<const uint32_t*>(s + C::OFF_BAD);
+                const uint32_t bad = any_bad ? *reinterpret_cast<const uint32_t*>(ring + s + C::OFF_BAD) : 0u;
                 const bool edge = k0 + 16 > lowest || bad != 0;
-                bool grow = false;
+                if (edge) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) c[n][i] *= factor[n][i & 1];
-                    if (edge) {
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int key = i < 2 ? ka : kb;
                             if (k0 + key >= lim[n][i & 1] || (bad >> key & 1)) c[n][i] = -INFINITY;
                         }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) grow = grow || fmaxf(c[n][i], c[n][i + 2]) > m[n][i] + 7.f;
                 }
+                bool grow = false;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) grow = grow || fmaxf(c[n][i], c[n][i + 2]) * factor[n][i] > m[n][i] + 7.f;
                 if (__any_sync(0xffffffffu, grow)) {      // (rare behind the first tiles) every row's reference becomes its maximum so far
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            float top = fmaxf(m[n][i], fmaxf(c[n][i], c[n][i + 2]));
+                            float top = fmaxf(m[n][i], fmaxf(c[n][i], c[n][i + 2]) * factor[n][i]);
 #pragma unroll
                             for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-                            const float down = top == -INFINITY ? 1.f : exp2_fast(m[n][i] - top);
+                            const float down = exp2_fast(m[n][i] - top);
                             m[n][i] = top;
                             l[n][i] *= down;
 #pragma unroll
@@ -457,7 +561,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) c[n][i] = exp2_fast(c[n][i] - (m[n][i & 1] == -INFINITY ? 0.f : m[n][i & 1]));
+                    for (int i = 0; i < 4; ++i) c[n][i] = exp2_fast(fmaf(c[n][i], factor[n][i & 1], -m[n][i & 1]));
                     l[n][0] += c[n][0] + c[n][2];
                     l[n][1] += c[n][1] + c[n][3];
                     pb[n][0] = movmatrix(pack2<__half>(c[n][0], c[n][1]));
@@ -465,19 +569,22 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
                 }
                 // ---- O^T += V^T P^T: columns of the product are keys 2 t, 2 t + 1 and eight further, in the order of the rows above ----
                 {
-                    const int flip = (t >> 1) & 1, v0 = 2 * t + flip, v1 = 2 * t + 1 - flip;
                     uint32_t w[4][DPT / 8], sc[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = (i & 1 ? v1 : v0) + (i >> 1) * 8;
-                        if constexpr (HD == 128) {
-                            *reinterpret_cast<uint2*>(w[i]) = *reinterpret_cast<const uint2*>(s + C::OFF_V + key * 64 + (((g >> 1) ^ (key & 2)) * 16) + (g & 1) * 8);
-                            sc[i] = s[C::OFF_VS + key * 8 + g];
-                        } else {
-                            w[i][0] = *reinterpret_cast<const uint32_t*>(s + C::OFF_V + key * 32 + g * 4);
-                            sc[i] = s[C::OFF_VS + key * 4 + (g >> 1)];
-                        }
+                    if constexpr (HD == 128) {
+                        *reinterpret_cast<uint2*>(w[0]) = lds64<0>(va_at + s);
+                        *reinterpret_cast<uint2*>(w[1]) = lds64<0>(vb_at + s);
+                        *reinterpret_cast<uint2*>(w[2]) = lds64<8 * C::ROW>(va_at + s);
+                        *reinterpret_cast<uint2*>(w[3]) = lds64<8 * C::ROW>(vb_at + s);
+                    } else {
+                        w[0][0] = lds32<0>(va_at + s);
+                        w[1][0] = lds32<0>(vb_at + s);
+                        w[2][0] = lds32<8 * C::ROW>(va_at + s);
+                        w[3][0] = lds32<8 * C::ROW>(vb_at + s);
                     }
+                    sc[0] = lds8<0>(vs_at + s);
+                    sc[1] = lds8<0>(vs_at + s + vs_step);
+                    sc[2] = lds8<8 * C::SROW>(vs_at + s);
+                    sc[3] = lds8<8 * C::SROW>(vs_at + s + vs_step);
                     if (edge) {
                         // a value that is not a number reaches the rows that see its key, and no others (0 * NaN would)
                         uint32_t odd = 0;
@@ -505,13 +612,15 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
                     const uint32_t ya = from_e4m3x2(sc[0] | sc[1] << 8), yb = from_e4m3x2(sc[2] | sc[3] << 8);
 #pragma unroll
                     for (int h = 0; h < DPT / 8; ++h) {
-                        // byte k: channel 2 k of both keys, and channel 2 k + 1
-                        const uint32_t a0 = (w[0][h] & 0x0f0f0f0fu) | ((w[1][h] << 4) & 0xf0f0f0f0u), a1 = ((w[0][h] >> 4) & 0x0f0f0f0fu) | (w[1][h] & 0xf0f0f0f0u);
-                        const uint32_t b0_ = (w[2][h] & 0x0f0f0f0fu) | ((w[3][h] << 4) & 0xf0f0f0f0u), b1_ = ((w[2][h] >> 4) & 0x0f0f0f0fu) | (w[3][h] & 0xf0f0f0f0u);
+                        // byte k: channel 2 k of both keys (even), channel 2 k + 1 (odd)
+                        uint32_t ae[4], ao[4], be[4], bo[4];
+                        from_e2m1x8((w[0][h] & 0x0f0f0f0fu) | ((w[1][h] << 4) & 0xf0f0f0f0u), ae);
+                        from_e2m1x8(((w[0][h] >> 4) & 0x0f0f0f0fu) | (w[1][h] & 0xf0f0f0f0u), ao);
+                        from_e2m1x8((w[2][h] & 0x0f0f0f0fu) | ((w[3][h] << 4) & 0xf0f0f0f0u), be);
+                        from_e2m1x8(((w[2][h] >> 4) & 0x0f0f0f0fu) | (w[3][h] & 0xf0f0f0f0u), bo);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const uint32_t frag[4] = {mul_half2(from_e2m1x2(a0 >> 8 * k), ya), mul_half2(from_e2m1x2(a1 >> 8 * k), ya),
-                                                      mul_half2(from_e2m1x2(b0_ >> 8 * k), yb), mul_half2(from_e2m1x2(b1_ >> 8 * k), yb)};
+                            const uint32_t frag[4] = {mul_half2(ae[k], ya), mul_half2(ao[k], ya), mul_half2(be[k], yb), mul_half2(bo[k], yb)};
 #pragma unroll
                             for (int n = 0; n < NT; ++n) mma_16816<__half>(o[n][h * 4 + k], frag, pb[n][0], pb[n][1]);
                         }
@@ -549,15 +658,14 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
             const int r = i / (HD / 4), col = (i - r * (HD / 4)) * 4;
             int s_abs, hq;
             if (!paged_row(a, u, r, &s_abs, &hq)) continue;
-            float M = -INFINITY;
+            float M = -FLT_MAX;
 #pragma unroll
             for (int w = 0; w < kQ4Warps; ++w) M = fmaxf(M, fold_m[w * 8 * NT + r]);
-            const float mu = M == -INFINITY ? 0.f : M;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
             float L = 0.f;
 #pragma unroll
             for (int w = 0; w < kQ4Warps; ++w) {
-                const float wgt = exp2_fast(fold_m[w * 8 * NT + r] - mu);
+                const float wgt = exp2_fast(fold_m[w * 8 * NT + r] - M);
                 const float4 v = *reinterpret_cast<const float4*>(fold + (w * 8 * NT + r) * C::PITCH + col);
                 acc.x = fmaf(v.x, wgt, acc.x);
                 acc.y = fmaf(v.y, wgt, acc.y);
@@ -607,14 +715,14 @@ __global__ void __launch_bounds__(128) q4_mma_merge_kernel(const __grid_constant
     int s_abs, hq;
     if (!paged_row(a, u, row, &s_abs, &hq)) return;
     T* const out = static_cast<T*>(a.out) + u.w * a.o_w + s_abs * a.o_s + hq * a.o_h;
-    float M = -INFINITY, L = 0.f, acc[VEC] = {};
+    float M = -FLT_MAX, L = 0.f, acc[VEC] = {};
     for (int p0 = warp; p0 < count; p0 += 32) {           // eight partials of a warp in flight
         float mp[8], lp[8], v[8][VEC];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const size_t at = ((size_t)(first + p0 + 4 * k) + unit) * kFmaRows + row;
             const bool have = p0 + 4 * k < count;
-            mp[k] = have ? __ldcg(a.ws_m + at) : -INFINITY;
+            mp[k] = have ? __ldcg(a.ws_m + at) : -FLT_MAX;
             lp[k] = have ? __ldcg(a.ws_l + at) : 0.f;
             if constexpr (VEC == 4) {
                 const float4 y = have ? __ldcg(reinterpret_cast<const float4*>(a.ws_o + at * HD + lane * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -627,14 +735,14 @@ __global__ void __launch_bounds__(128) q4_mma_merge_kernel(const __grid_constant
         float top = M;
 #pragma unroll
         for (int k = 0; k < 8; ++k) top = fmaxf(top, mp[k]);
-        const float mu = top == -INFINITY ? 0.f : top, down = exp2_fast(M - mu);
+        const float down = exp2_fast(M - top);
         M = top;
         L *= down;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[i] *= down;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float wgt = exp2_fast(mp[k] - mu);
+            const float wgt = exp2_fast(mp[k] - top);
             L = fmaf(lp[k], wgt, L);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) acc[i] = fmaf(v[k][i], wgt, acc[i]);
@@ -648,13 +756,12 @@ __global__ void __launch_bounds__(128) q4_mma_merge_kernel(const __grid_constant
     for (int i = 0; i < VEC; ++i) sm_o[warp][lane * VEC + i] = acc[i];
     __syncthreads();
     if (warp != 0) return;
-    float top = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
-    const float mu = top == -INFINITY ? 0.f : top;
+    const float top = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
     L = 0.f;
     float r[VEC] = {};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-        const float wgt = exp2_fast(sm_m[w] - mu);
+        const float wgt = exp2_fast(sm_m[w] - top);
         L = fmaf(sm_l[w], wgt, L);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) r[i] = fmaf(sm_o[w][lane * VEC + i], wgt, r[i]);

@@ -359,6 +359,18 @@ def test_large_and_small_queries(A):
             q4_util.check(got, exact)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1e-30, 3.0])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_scales_of_the_scores(A, scale, kernel):
+    gen = torch.Generator().manual_seed(10)
+    cache = [x for pair in zip(*(q4_util.random_cache(gen, 8, 2, 16, 128) for _ in range(2))) for x in pair]
+    q = torch.randn(1, 2, 6, 1, 128, generator=gen).bfloat16()
+    q[0, 0, 1] = 0
+    got, exact = paged(A, q, torch.tensor([[[37], [63]]], dtype=torch.int32), torch.tensor([60], dtype=torch.int32), cache,
+                       torch.arange(8, dtype=torch.int32).reshape(2, 4), scale, kernel=kernel)
+    q4_util.check(got, exact)
+
+
 def test_refusals_of_the_operators(A):
     gen = torch.Generator().manual_seed(9)
     kc, vc, ks, vs = dev(*empty_cache(gen, 4, 2, 16, 64, 64))
