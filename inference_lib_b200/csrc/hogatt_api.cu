@@ -65,8 +65,6 @@ bool pdl_enabled() {
     return on;
 }
 
-namespace {
-
 // HOGATT_DENSE=0 in the environment keeps AUTO away from the tcgen05 kernel (A/B measurements).
 bool dense_disabled() {
     static const bool off = [] {
@@ -75,6 +73,8 @@ bool dense_disabled() {
     }();
     return off;
 }
+
+namespace {
 
 // HOGATT_HOST_PLAN=0 in the environment (read when the library is first used) makes every call derive its
 // tiles on the device even when the caller gave host_lengths: for A/B measurements.
@@ -569,8 +569,7 @@ EncodeTiledFn tensor_map_encoder() {
     return fn;
 }
 
-// A tiled map with the 128-byte swizzle over a dense row-major tensor of 16-bit elements: dims[0] is the contiguous
-// one, box[0] = 64 elements = 128 bytes.
+}  // namespace
 int encode_map(CUtensorMap* out, const void* base, int dtype, int rank, const cuuint64_t* dims, const cuuint32_t* box) {
     EncodeTiledFn fn = tensor_map_encoder();
     if (!fn) return HOGATT_ERR_CUDA;
@@ -590,6 +589,7 @@ int encode_map(CUtensorMap* out, const void* base, int dtype, int rank, const cu
     }
     return HOGATT_OK;
 }
+namespace {
 
 // Fragment maps are cached by (pointer, rows, heads, dtype): preallocated slabs keep their pointers for the whole
 // generation, so a decode step encodes nothing.
@@ -733,6 +733,7 @@ int launch_dense(const hogatt_problem* p, const KernelArgs& args, const Workspac
     d.ctas = std::min(grid, kDenseMaxCtas);
     d.status = args.status;
     d.out = args.out;
+    d.out_scale = 1.f;
     d.world = args.world;
     d.rank = args.rank;
     for (int i = 0; i < args.world; ++i) d.peer_out[i] = args.peer_out[i];
@@ -1078,6 +1079,7 @@ int launch_paged_dense(const hogatt_paged_problem* p, const PagedPlan& pl, int d
     d.ctas = std::min(sms, kDenseMaxCtas);
     d.status = p->device_status;
     d.out = p->out;
+    d.out_scale = 1.f;
     DenseMaps maps;
     memset(&maps, 0, sizeof(maps));
     const cuuint64_t qdims[5] = {128, (cuuint64_t)d.G, (cuuint64_t)d.Hkv, (cuuint64_t)d.total_q, (cuuint64_t)d.F};

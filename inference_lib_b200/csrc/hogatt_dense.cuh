@@ -33,6 +33,8 @@
 #include <cuda.h>
 #include <limits.h>
 
+#include <type_traits>
+
 #include "hogatt_device.cuh"
 #include "hogatt_merge.cuh"
 
@@ -100,17 +102,33 @@ struct DenseArgs {
     void* out;             // [W, Hq, S, 128] or [total_q, Hq, 128]
     int world, rank;       // > 0: every finished row goes to the full-size output of every rank
     void* peer_out[HOGATT_MAX_PEERS];
+    // Pages in 4 bits (hogatt_q4_dense.cuh): [0] keys, [1] values.
+    const unsigned char* codes[2];
+    const unsigned char* scales[2];
+    const float* factor;   // [total_q, Hq]: what a row's products are multiplied with, or nullptr: l2scale for all
+    int num_blocks;
+    uint32_t block_mul, block_shift;       // key / block_size = (umulhi(key, mul) + key) >> shift
+    float out_scale;       // the values' unit (1 elsewhere)
 };
 
-struct DenseCfg {
+template <bool Q4>
+struct DenseCfgOf {
     static constexpr int HD = 128;
     static constexpr int ATOM_BYTES = 128 * 128;            // [128 rows][64 16-bit columns], rows of 128 bytes, swizzled
     static constexpr int TILE_BYTES = 2 * ATOM_BYTES;       // a 128 x 128 operand tile: two column halves
-    static constexpr int NQ = 2, NK = 3, NV = 2;            // rings of query, K and V tiles
+    static constexpr int NQ = 2, NK = Q4 ? 2 : 3, NV = 2;   // rings of query, K and V tiles
     static constexpr int OFF_Q = 0;
     static constexpr int OFF_K = OFF_Q + NQ * TILE_BYTES;
     static constexpr int OFF_V = OFF_K + NK * TILE_BYTES;
-    static constexpr int OFF_BAR = OFF_V + NV * TILE_BYTES;                 // 224 KiB of tiles
+    // Q4: a warp unpacks K tiles and one V tiles; rows as they lie in the cache, 32 keys at a time (for K with the values' scales), a ring for each
+    static constexpr int WARPS = kDenseSoftmaxWarps + 4;
+    // Registers of a softmax thread and of the others.  The warps' shares must not add up to more than what the block is launched with: 96 a
+    // thread (65,536 / 4 for the five warps of an SM's quarter, in steps of 8).  More would wait forever.
+    static constexpr int SOFTMAX_REGS = Q4 ? 96 : 104, OTHER_REGS = Q4 ? 96 : 64;
+    static_assert(kDenseSoftmaxWarps * SOFTMAX_REGS + 4 * OTHER_REGS <= WARPS * 96, "register shares");
+    static constexpr int PACK_BYTES = 32 * (HD / 2 + 2 * HD / 16), NPACK = Q4 ? 6 : 0;
+    static constexpr int OFF_PACK = OFF_V + NV * TILE_BYTES;
+    static constexpr int OFF_BAR = OFF_PACK + 2 * NPACK * PACK_BYTES;       // 224 KiB of tiles
     static constexpr int OFF_STAT = OFF_BAR;                                // [2 groups][2 halves][128 rows]: maxima or sums handed over
     // barriers: q_full[NQ], q_empty[NQ], k_full[NK], k_empty[NK], v_full[NV], v_empty[NV], s_full[2], s_free, p_full[2], o_done[2],
     // segment full / empty
@@ -118,10 +136,13 @@ struct DenseCfg {
     static constexpr int OFF_MBAR = OFF_STAT + 2 * 2 * kDenseRows * 4;
     static constexpr int OFF_SEG = (OFF_MBAR + NBAR * 8 + 15) / 16 * 16;
     static constexpr int OFF_MISC = OFF_SEG + 4 * 32;                       // tmem base
-    static constexpr int OFF_END = OFF_MISC + 16;
+    // Q4: eight key tiles' special keys: which have a page (128 bits), is some value not a number
+    static constexpr int OFF_ODD = OFF_MISC + 16;
+    static constexpr int OFF_END = OFF_ODD + (Q4 ? 256 : 0);
     static constexpr int TMEM_COLS = 512;
     static constexpr int COL_O = 0, COL_S = 256, COL_P = 384;               // O_g at 128 g, P_g at 384 + 64 g
 };
+using DenseCfg = DenseCfgOf<false>;
 
 constexpr size_t kDenseSmemBytes = DenseCfg::OFF_END;       // (227 KiB is all there is: dynamic shared memory starts on a 1 KiB boundary)
 
@@ -637,10 +658,22 @@ __device__ __forceinline__ void dense_fetch(const DenseArgs& a, const CUtensorMa
     }
 }
 
-template <class T, bool PAGED>
-__global__ void __launch_bounds__(kDenseThreads, 1)
+// ---- pages in 4 bits: defined in hogatt_q4_dense.cuh, which only its users include -------------------------------------
+struct Q4Pipe {            // a warp's look at the block table: windows of eight units of 32 keys
+    int64_t rows, next;    // lane 4 u + i: where rows 8 i ... of unit u of the window, and of the one behind it, begin
+    uint32_t none, before; // the same lanes' bits: keys without a page, in the window and in the one in front of it
+};
+template <class C>
+__device__ __forceinline__ void q4_unpack(const DenseArgs& a, int which, int w, int h, int t, int t0, int t1, int len, uint32_t pack,
+                                               uint32_t dst, unsigned char* odd, Q4Pipe& pipe, int lane);
+__device__ __forceinline__ uint32_t q4_odd_groups(const DenseArgs& a, int w, int h, int tok0, int n);
+
+// T: the output's type, and the products' unless Q4 (then fp16: hogatt_q4_dense.cuh).
+template <class T, bool PAGED, bool Q4 = false>
+__global__ void __launch_bounds__(DenseCfgOf<Q4>::WARPS * 32, 1)
 dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constant__ DenseMaps maps) {
-    using C = DenseCfg;
+    using C = DenseCfgOf<Q4>;
+    using M = std::conditional_t<Q4, __half, T>;
     extern __shared__ __align__(1024) unsigned char dense_smem[];       // swizzled tiles start on 1 KiB boundaries
     unsigned char* const base = dense_smem;
     const uint32_t sbase = smem_u32(base);
@@ -689,10 +722,12 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
     bool ok = true;
 
     if (warp >= W_K) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if constexpr (!Q4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
+        [[maybe_unused]] Q4Pipe pipe = {0, 0, 0u, 0u};
         if (warp == W_K) {
             // ============================== query and K copies ==============================
             int stage = 0, q_slot = 0;
+            [[maybe_unused]] int n_tile = 0;
             uint32_t phase = 1, q_phase = 1;         // of k_empty and q_empty: the first round finds every stage free
             const int gs = a.G * a.S;
             const uint32_t q_bytes = (uint32_t)(PAGED ? a.tile_span * a.G : (gs > kDenseRows ? kDenseRows : a.tile_span * gs)) * 256u;
@@ -703,7 +738,13 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
                     ok = mbar_wait_polls(k_empty + 8 * stage, phase, a.status, STATUS_WAIT_EMPTY_TIMEOUT);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    dense_fetch<PAGED>(a, maps.k, d.f, w, d.h, t * kDenseTile, sbase + C::OFF_K + stage * C::TILE_BYTES, k_full + 8 * stage, lane);
+                    if constexpr (Q4) {
+                        q4_unpack<C>(a, 0, w, d.h, t, d.t0, d.t1, max(d.vis0, d.vis1), sbase + C::OFF_PACK, sbase + C::OFF_K + stage * C::TILE_BYTES,
+                                     base + C::OFF_ODD + (n_tile++ & 7) * 32, pipe, lane);
+                        if (lane == 0) mbar_arrive(k_full + 8 * stage);
+                    } else {
+                        dense_fetch<PAGED>(a, maps.k, d.f, w, d.h, t * kDenseTile, sbase + C::OFF_K + stage * C::TILE_BYTES, k_full + 8 * stage, lane);
+                    }
                     if (++stage == C::NK) {
                         stage = 0;
                         phase ^= 1u;
@@ -775,13 +816,20 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
 #pragma unroll 1
             while (ok && more) {
                 const int f = walk.f, h = walk.h, t0 = walk.t0, t1 = walk.t1, w = PAGED ? a.rec[walk.b].x : 0;
+                [[maybe_unused]] const int vlen = max(walk.vis0, walk.vis1);
                 more = publish();
 #pragma unroll 1
                 for (int t = t0; t < t1 && ok; ++t) {
                     ok = mbar_wait_polls(v_empty + 8 * stage, phase, a.status, STATUS_WAIT_EMPTY_TIMEOUT);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    dense_fetch<PAGED>(a, maps.v, f, w, h, t * kDenseTile, sbase + C::OFF_V + stage * C::TILE_BYTES, v_full + 8 * stage, lane);
+                    if constexpr (Q4) {
+                        q4_unpack<C>(a, 1, w, h, t, t0, t1, vlen, sbase + C::OFF_PACK + C::NPACK * C::PACK_BYTES, sbase + C::OFF_V + stage * C::TILE_BYTES,
+                                     nullptr, pipe, lane);
+                        if (lane == 0) mbar_arrive(v_full + 8 * stage);
+                    } else {
+                        dense_fetch<PAGED>(a, maps.v, f, w, h, t * kDenseTile, sbase + C::OFF_V + stage * C::TILE_BYTES, v_full + 8 * stage, lane);
+                    }
                     if (++stage == C::NV) {
                         stage = 0;
                         phase ^= 1u;
@@ -790,7 +838,7 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
             }
         } else if (warp == W_S) {
             // ============================== the S MMAs ==============================
-            constexpr uint32_t IDESC_S = umma_idesc<T>(false, kDenseRows, kDenseTile);
+            constexpr uint32_t IDESC_S = umma_idesc<M>(false, kDenseRows, kDenseTile);
             // (a k-step only moves the descriptor's start-address field: +32 bytes inside a 64-column swizzle atom,
             // +16 KiB to the second atom)
             const uint64_t q_desc = umma_desc(sbase + C::OFF_Q, 16, 1024), k_desc = umma_desc(sbase + C::OFF_K, 16, 1024);
@@ -849,7 +897,7 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
             }
         } else {
             // ============================== the O += P V MMAs ==============================
-            constexpr uint32_t IDESC_O = umma_idesc<T>(true, kDenseRows, C::HD);
+            constexpr uint32_t IDESC_O = umma_idesc<M>(true, kDenseRows, C::HD);
             const uint64_t v_desc = umma_desc(sbase + C::OFF_V, C::ATOM_BYTES, 1024);
             int stage = 0;
             uint32_t v_phase = 0, g_phase = 0, started = 0;      // bit g: parity of P_g; O_g holds something
@@ -859,7 +907,7 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
 #pragma unroll 1
                 for (int t = d.t0; t < d.t1 && ok; ++t) {
                     ok = __all_sync(0xffffffffu, mbar_wait_polls(v_full + 8 * stage, v_phase, a.status, STATUS_WAIT_FULL_TIMEOUT));
-                    if ((t + 1) * kDenseTile > vlen && ok) {
+                    if (!Q4 && (t + 1) * kDenseTile > vlen && ok) {
                         // The tile runs past the keys that any row of the block sees: what follows may hold anything (spare
                         // rows of a slab or cache block).  Those probabilities are exactly zero, but 0 * NaN would poison O.
                         unsigned char* vt = base + C::OFF_V + stage * C::TILE_BYTES;
@@ -906,7 +954,7 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
         }
     } else {
         // ============================== softmax: warps 0-7 group 0, 8-15 group 1; warps w and w + 4 share 32 rows ==============================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        if constexpr (!Q4) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
         constexpr int COLS = kDenseTile / 2;                              // this thread's columns of S, P and O
         const int g = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;            // row of the tile == tensor-memory lane
         const uint32_t lane_base = tmem + (((uint32_t)((warp & 3) * 32)) << 16);
@@ -915,8 +963,10 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
         float* const stat = reinterpret_cast<float*>(base + C::OFF_STAT) + (g * 2 + half) * kDenseRows + row;
         const float* const other = reinterpret_cast<const float*>(base + C::OFF_STAT) + (g * 2 + (half ^ 1)) * kDenseRows + row;
         const int pair_bar = 1 + g * 4 + (warp & 3);                      // hardware barrier of the two warps that share rows
-        const float scale2 = a.l2scale;                        // scores are raw dot products; exp2((s - m) * scale2)
-        const float grow_by = 8.f / scale2;                    // raw-score distance that equals a factor 2^8
+        float scale2 = a.l2scale;                              // scores are raw dot products; exp2((s - m) * scale2)
+        float grow_by = 8.f / scale2;                          // raw-score distance that equals a factor 2^8
+        [[maybe_unused]] uint32_t odd_groups = 0;              // (Q4) groups of the row's channels that are not numbers
+        [[maybe_unused]] int tile_base = 0;                    // (Q4) key tiles of the segments before this one
         float m_run = -INFINITY, l_run = 0.f;                  // running max (raw, the row's) and sum (of this half's columns)
         uint32_t phase = 0;                                    // parity of this group's next S; its last PV has the other one
         bool any = false, ever = false;                        // has worked on a tile of this unit; at all
@@ -933,6 +983,13 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
                 m_run = -INFINITY;
                 l_run = 0.f;
                 any = false;
+                if constexpr (Q4) {
+                    odd_groups = 0;
+                    if (a.factor) {
+                        scale2 = id.valid ? a.factor[(size_t)id.s * a.Hq + d.h * a.G + id.g] : 1.f;
+                        grow_by = 8.f / scale2;
+                    }
+                }
             }
             int lim = 0;                                       // keys of the fragment that the row sees: [0, lim)
             if (id.valid) lim = min(dense_location<PAGED>(a, d.f, id), dense_length<PAGED>(a, d.f, id.w) - 1) + 1;
@@ -946,10 +1003,24 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
                 tmem_ld32(s_addr, *reinterpret_cast<float(*)[32]>(&s[0]));
                 tmem_ld32(s_addr + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
                 tmem_wait_ld();
+                // (Q4) of this half's keys: which have a page (64 bits), is some value not a number
+                [[maybe_unused]] uint32_t there0 = ~0u, there1 = ~0u, odd = 0;
+                if constexpr (Q4) {
+                    const uint32_t at = sbase + C::OFF_ODD + ((tile_base + t - d.t0) & 7) * 32;
+                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(there0), "=r"(there1) : "r"(at + half * 8) : "memory");
+                    asm volatile("ld.shared.b32 %0, [%1+16];" : "=r"(odd) : "r"(at) : "memory");
+                }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_free);            // the next S MMA may overwrite the buffer
                 const int nvis = lim - t * kDenseTile - half * COLS;      // of this thread's keys the row sees [0, nvis)
+                if constexpr (Q4) {                            // (the same for every thread of the warp)
+                    if (odd) odd_groups |= q4_odd_groups(a, a.rec[d.b].x, d.h, t * kDenseTile + half * COLS, min(nvis, COLS));
+                    if ((there0 & there1) != ~0u) {
+#pragma unroll
+                        for (int k = 0; k < COLS; ++k) s[k] = (k < 32 ? there0 : there1) >> (k & 31) & 1 ? s[k] : -INFINITY;
+                    }
+                }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 if (__any_sync(0xffffffffu, nvis < COLS)) {
 #pragma unroll
@@ -1005,7 +1076,7 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
                         x0 = fast_exp2(x0);
                         x1 = fast_exp2(x1);
                         sum[k & 1] = add2(sum[k & 1], pair_f32(x0, x1));
-                        packed[k] = pack2<T>(x0, x1);
+                        packed[k] = pack2<M>(x0, x1);
                     }
                     tmem_st16(p_addr + c * 16, packed);        // P (storage type, two per column): this row's lane
                 }
@@ -1020,6 +1091,7 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
                 any = ever = true;
             }
             if (!ok) break;
+            if constexpr (Q4) tile_base += d.t1 - d.t0;
 
             // ---- end of this CTA's share of the unit: the rows themselves, or a partial result ----
             if (d.last()) {
@@ -1042,6 +1114,15 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
                 if (!ok) break;
                 const float total = half ? *other + l_run : l_run + *other;
                 named_barrier_sync(pair_bar, 64);              // (read before it is written again)
+                [[maybe_unused]] uint32_t odd_here = 0;        // (Q4) bit i: this thread's columns 16 i ... are not numbers
+                if constexpr (Q4) {
+                    if (pair_any(pair_bar, odd_groups != 0)) {
+                        *stat = __uint_as_float(odd_groups);
+                        named_barrier_sync(pair_bar, 64);
+                        odd_here = (odd_groups | __float_as_uint(*other)) >> (half * (COLS / 16)) & ((1u << COLS / 16) - 1u);
+                        named_barrier_sync(pair_bar, 64);
+                    }
+                }
                 const int slot_row = g * kDenseRows + row;
                 const size_t slot = (size_t)blockIdx.x + unit;
                 const float m_own = m_run == -INFINITY ? -INFINITY : m_run * scale2;
@@ -1068,6 +1149,12 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
                             tmem_wait_ld();
 #pragma unroll
                             for (int k = 0; k < 32; ++k) o[k] = any ? o[k] : 0.f;          // (a group that saw nothing never touched its O)
+                            if constexpr (Q4) {
+                                if (odd_here >> (c / 16) & 3) {
+#pragma unroll
+                                    for (int k = 0; k < 32; ++k) o[k] = odd_here >> (c / 16 + k / 16) & 1 ? NAN : o[k];
+                                }
+                            }
 #pragma unroll
                             for (int k = 0; k < 8; ++k) wo[(c / 4 + k) * kDenseBlock] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
                         }
@@ -1127,7 +1214,13 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
                                 for (int k = 0; k < 32; ++k) acc[k] = fmaf(x[k], w, acc[k]);
                             }
                         }
-                        const float inv = den > 0.f ? 1.f / den : 0.f;
+                        if constexpr (Q4) {
+                            if (odd_here >> (c / 16) & 3) {
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) acc[k] = odd_here >> (c / 16 + k / 16) & 1 ? NAN : acc[k];
+                            }
+                        }
+                        const float inv = den > 0.f ? (Q4 ? a.out_scale : 1.f) / den : 0.f;
                         uint32_t v[2][8];
 #pragma unroll
                         for (int k = 0; k < 16; ++k) v[k >> 3][k & 7] = pack2<T>(acc[2 * k] * inv, acc[2 * k + 1] * inv);
@@ -1283,7 +1376,7 @@ __global__ void __launch_bounds__(kDenseMergeWarps * 32, BATCH == 1 ? 4 : 2) den
         }
         const DenseRow id = dense_row<PAGED>(a, 2 * b + r / kDenseRows, r % kDenseRows, rec);
         if (!id.valid) continue;
-        const float inv = den > 0.f ? 1.f / den : 0.f;
+        const float inv = den > 0.f ? a.out_scale / den : 0.f;
         const size_t offset = dense_out_offset<PAGED>(a, id, h) + c4 * 4;
         uint4 v[2];
         uint32_t* out = reinterpret_cast<uint32_t*>(v);

@@ -1,6 +1,7 @@
 // Host helpers that the C ABI's translation units share: errors, device properties, launches.  Defined in hogatt_api.cu where they
 // are more than a line.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -57,6 +58,12 @@ cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
     cfg.numAttrs = pdl_enabled() ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
+
+// A tiled tensor map with the 128-byte swizzle over a dense row-major tensor of 16-bit elements: dims[0] is the contiguous one, box[0] = 64
+// elements = 128 bytes.
+int encode_map(CUtensorMap* out, const void* base, int dtype, int rank, const cuuint64_t* dims, const cuuint32_t* box);
+
+bool dense_disabled();      // HOGATT_DENSE=0: AUTO keeps away from the tcgen05 kernels
 
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 inline size_t dtype_size(int dtype) { return dtype == HOGATT_F32 ? 4 : 2; }

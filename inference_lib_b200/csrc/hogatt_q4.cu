@@ -2,12 +2,15 @@
 // carving and launches, like hogatt_api.cu.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
+#include <type_traits>
 
 #include "hogatt_host.h"
 #include "hogatt_blocks.cuh"
 #include "hogatt_q4.cuh"
 #include "hogatt_q4_mma.cuh"
+#include "hogatt_q4_dense.cuh"
 
 namespace hogatt {
 namespace {
@@ -25,13 +28,51 @@ int cache_shape(int Hkv, int E, int Ev, int block_size, int max_blocks, int num_
     return HOGATT_OK;
 }
 
+// The tcgen05 kernel's workspace for packed queries: the plan, then one slot of 256 rows per (CTA, unit) pair that can meet.
+struct DenseLayout {
+    size_t pre, cost, vis, start, merge, fold, rec, o, m, l, total;
+};
+DenseLayout carve_dense_plan(int64_t blocks, int Hkv, int F, int grid) {
+    const size_t slots = (size_t)grid + (size_t)blocks * Hkv;
+    DenseLayout w;
+    w.pre = 256;
+    w.cost = w.pre + align_up((size_t)(blocks + 1) * sizeof(long long), 256);
+    w.vis = w.cost + align_up((size_t)(blocks + 1) * sizeof(long long), 256);
+    w.start = w.vis + align_up((size_t)blocks * 2 * F * sizeof(int), 256);
+    w.merge = w.start + align_up((size_t)grid * sizeof(int4), 256);
+    w.fold = w.merge + align_up((size_t)blocks * Hkv * sizeof(int4), 256);
+    w.rec = w.fold + align_up((size_t)blocks * Hkv * kDenseFoldInts * sizeof(int), 256);
+    w.o = w.rec + align_up((size_t)blocks * sizeof(int4), 256);
+    w.m = w.o + slots * kDenseBlock * 128 * sizeof(float);
+    w.l = w.m + align_up(slots * kDenseBlock * sizeof(float), 256);
+    w.total = w.l + align_up(slots * kDenseBlock * sizeof(float), 256);
+    return w;
+}
+
 struct Q4Plan {
     int kernel;                     // HOGATT_KERNEL_FMA or HOGATT_KERNEL_MMA
     int tokens_per_group, head_blocks, groups_bound, units, splits;
     int rows;                       // (MMA) query rows of a unit at most
     int ctas;                       // (MMA) shares of the list of tiles; 0: a CTA per unit
     size_t o, m, l, plan, total;
+    int tokens, blocks;             // (DENSE) query tokens per tile, blocks per kv head at most
+    DenseLayout w;                  // (DENSE) its workspace
+    size_t queries, factor;
 };
+
+// Packed queries on the tcgen05 kernel: head size 128, blocks of a multiple of eight rows.
+bool dense_eligible(const hogatt_paged_problem* p) {
+    return p->cu_seqlens_q != nullptr && (p->dtype == HOGATT_F16 || p->dtype == HOGATT_BF16) && p->E == 128 && p->Ev == 128 && p->block_size % 8 == 0 &&
+           p->Hq / p->Hkv <= kDenseRows && (int64_t)p->total_q_tokens * p->Hq * p->F < ((int64_t)1 << 31) && p->scale >= 1e-30f && p->scale <= 1e30f;
+}
+// AUTO takes it where the tokens beyond one per sequence, over as many keys as the block table has room for, would keep the other
+// kernel busy for long (as for 16-bit pages).
+bool dense_wanted(const hogatt_paged_problem* p) {
+    if (dense_disabled()) return false;
+    const int64_t tokens = (int64_t)p->total_q_tokens - p->W;
+    if (tokens * (p->Hq / p->Hkv) < kDenseRows || tokens * p->Hq < 8 * kDenseRows) return false;
+    return (double)tokens * p->Hq * p->max_blocks_per_seq * p->block_size >= 4.5e6;
+}
 
 // Units beyond this many per resident CTA get a CTA each: the list's shares then hold several units, whose ends (the eight warps' fold, the next
 // unit's first copies) do not overlap inside a CTA, and the merge step is saved.
@@ -47,11 +88,27 @@ int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
     if (p->Ev != 32 && p->Ev != 64 && p->Ev != 128 && p->Ev != 256) return HOGATT_ERR_UNSUPPORTED_HEAD_DIM;
     if (p->F > 4096) return HOGATT_ERR_TOO_MANY_FRAGMENTS;
     const bool mma = p->dtype != HOGATT_F32 && p->E == p->Ev && (p->E == 64 || p->E == 128);
-    if (p->kernel != HOGATT_KERNEL_AUTO && p->kernel != HOGATT_KERNEL_FMA && !(p->kernel == HOGATT_KERNEL_MMA && mma)) return HOGATT_ERR_BAD_KERNEL_CHOICE;
+    const bool dense = dense_eligible(p);
+    if (p->kernel != HOGATT_KERNEL_AUTO && p->kernel != HOGATT_KERNEL_FMA && !(p->kernel == HOGATT_KERNEL_MMA && mma) &&
+        !(p->kernel == HOGATT_KERNEL_DENSE && dense))
+        return HOGATT_ERR_BAD_KERNEL_CHOICE;
     pl->kernel = mma && p->kernel != HOGATT_KERNEL_FMA ? HOGATT_KERNEL_MMA : HOGATT_KERNEL_FMA;
+    if (dense && (p->kernel == HOGATT_KERNEL_DENSE || (p->kernel == HOGATT_KERNEL_AUTO && dense_wanted(p)))) pl->kernel = HOGATT_KERNEL_DENSE;
     if (!packed && (int64_t)p->F * p->W * p->S >= ((int64_t)1 << 31)) return HOGATT_ERR_TOO_LARGE;
     if (packed && (int64_t)p->F * std::max(p->total_q_tokens, p->W) >= ((int64_t)1 << 31)) return HOGATT_ERR_TOO_LARGE;
     const int G = p->Hq / p->Hkv, most = G >= 16 ? 1 : 16 / G;
+    if (pl->kernel == HOGATT_KERNEL_DENSE) {
+        pl->tokens = kDenseRows / G;
+        pl->blocks = p->total_q_tokens / (2 * pl->tokens) + p->W;
+        if ((int64_t)pl->blocks * p->Hkv > (1 << 24)) return HOGATT_ERR_TOO_LARGE;
+        pl->ctas = std::min(sms, kDenseMaxCtas);
+        pl->w = carve_dense_plan(pl->blocks, p->Hkv, p->F, pl->ctas);
+        pl->queries = pl->w.total;
+        const size_t rows = (size_t)p->total_q_tokens * p->Hq;
+        pl->factor = pl->queries + (p->dtype == HOGATT_BF16 ? align_up(rows * p->F * 128 * sizeof(__half), 256) : 0);
+        pl->total = pl->factor + align_up(rows * sizeof(float), 256);
+        return HOGATT_OK;
+    }
     // (tokens that a sequence is likely to have: a group of more would be empty rows; one of fewer is another reader of the same keys)
     const int64_t tokens = packed ? ((int64_t)p->total_q_tokens + p->W - 1) / p->W : p->S;
     pl->tokens_per_group = pl->kernel == HOGATT_KERNEL_MMA ? (int)std::max<int64_t>(1, std::min<int64_t>(most, tokens)) : most;
@@ -143,6 +200,95 @@ int launch_q4(const Q4Args& x, const Q4Plan& pl, int dev, int smem_optin, cudaSt
     }
 }
 
+// The limits of the bounded waits in this translation unit's kernels (hogatt_api.cu sets its own; see hogatt_device.cuh).
+int ensure_wait_limits(int dev) {
+    static std::atomic<bool> done[kMaxDevices];
+    if (done[dev].load(std::memory_order_acquire)) return HOGATT_OK;
+    if (const char* ms = getenv("HOGATT_WAIT_LIMIT_MS")) {
+        const unsigned int polls = (unsigned int)std::min(std::max(1ll, atoll(ms)), 1000000ll) * kPollsPerMs;
+        HOGATT_CUDA_OK(cudaMemcpyToSymbol(g_wait_polls, &polls, sizeof(polls)));
+    }
+    done[dev].store(true, std::memory_order_release);
+    return HOGATT_OK;
+}
+
+template <class T>
+int launch_q4_dense(const hogatt_paged_q4_problem* x, const Q4Plan& pl, int dev, int smem_optin, cudaStream_t stream) {
+    const hogatt_paged_problem* p = &x->paged;
+    int rc = ensure_wait_limits(dev);
+    if (rc != HOGATT_OK) return rc;
+    unsigned char* const ws = static_cast<unsigned char*>(p->workspace);
+    DenseArgs d;
+    memset(&d, 0, sizeof(d));
+    d.F = p->F; d.W = p->W; d.Hq = p->Hq; d.Hkv = p->Hkv; d.G = p->Hq / p->Hkv;
+    d.tiles = 2 * pl.blocks;
+    d.blocks = pl.blocks;
+    d.tile_span = pl.tokens;
+    d.total_q = p->total_q_tokens;
+    d.block_size = p->block_size;
+    d.max_blocks = p->max_blocks_per_seq;
+    d.l2scale = (float)((double)p->scale * 1.4426950408889634 * x->key_unit);
+    d.loc = p->locations;
+    d.flen = p->fragment_lengths;
+    d.cu = p->cu_seqlens_q;
+    d.block_table = p->block_table;
+    d.nmerge = reinterpret_cast<int*>(ws);
+    d.start = reinterpret_cast<int4*>(ws + pl.w.start);
+    d.merge = reinterpret_cast<int4*>(ws + pl.w.merge);
+    d.fold = reinterpret_cast<int*>(ws + pl.w.fold);
+    d.pre = reinterpret_cast<long long*>(ws + pl.w.pre);
+    d.cost = reinterpret_cast<long long*>(ws + pl.w.cost);
+    d.vis = reinterpret_cast<int*>(ws + pl.w.vis);
+    d.rec = reinterpret_cast<int4*>(ws + pl.w.rec);
+    d.ws_o = reinterpret_cast<float4*>(ws + pl.w.o);
+    d.ws_m = reinterpret_cast<float*>(ws + pl.w.m);
+    d.ws_l = reinterpret_cast<float*>(ws + pl.w.l);
+    d.ctas = pl.ctas;
+    d.status = p->device_status;
+    d.out = p->out;
+    d.codes[0] = static_cast<const unsigned char*>(p->key_cache);
+    d.codes[1] = static_cast<const unsigned char*>(p->value_cache);
+    d.scales[0] = static_cast<const unsigned char*>(x->key_scales);
+    d.scales[1] = static_cast<const unsigned char*>(x->value_scales);
+    d.num_blocks = p->num_blocks;
+    const FastDiv by_block = fast_div_by((uint32_t)p->block_size);
+    d.block_mul = by_block.mul;
+    d.block_shift = by_block.shift;
+    d.out_scale = x->value_unit;
+    constexpr bool convert = std::is_same<T, __nv_bfloat16>::value;
+    const void* q = p->queries;
+    if (convert) {
+        d.factor = reinterpret_cast<float*>(ws + pl.factor);
+        q = ws + pl.queries;
+    }
+    DenseMaps maps;
+    memset(&maps, 0, sizeof(maps));
+    const cuuint64_t qdims[5] = {128, (cuuint64_t)d.G, (cuuint64_t)d.Hkv, (cuuint64_t)d.total_q, (cuuint64_t)d.F};
+    const cuuint32_t qbox[5] = {64, (cuuint32_t)d.G, 1, (cuuint32_t)d.tile_span, 1};
+    rc = encode_map(&maps.q, q, HOGATT_F16, 5, qdims, qbox);
+    if (rc != HOGATT_OK) return rc;
+    HOGATT_CUDA_OK(launch_kernel(dense_plan_kernel<true>, dim3(1), dim3(kDensePlanThreads), 0, stream, d));
+    if constexpr (convert) {
+        const int rows = p->total_q_tokens * p->Hq;
+        HOGATT_CUDA_OK(launch_kernel(q4_dense_queries_kernel, dim3((rows + 7) / 8), dim3(256), 0, stream, static_cast<const __nv_bfloat16*>(p->queries),
+                                     reinterpret_cast<__half*>(ws + pl.queries), reinterpret_cast<float*>(ws + pl.factor), p->F, rows, d.l2scale));
+    }
+    static std::atomic<size_t> granted[kMaxDevices];
+    constexpr size_t smem = DenseCfgOf<true>::OFF_END;
+    if (smem > (size_t)smem_optin) return HOGATT_ERR_CUDA;
+    rc = ensure_smem_limit(dense_attention_kernel<T, true, true>, dev, smem, granted);
+    if (rc != HOGATT_OK) return rc;
+    HOGATT_CUDA_OK(launch_kernel(dense_attention_kernel<T, true, true>, dim3(d.ctas), dim3(DenseCfgOf<true>::WARPS * 32), smem, stream, d, maps));
+    // (as for 16-bit pages: few units have many partials, whose eight warps share a row's)
+    const int64_t units = (int64_t)d.blocks * d.Hkv, resident = 2 * (int64_t)d.ctas;
+    const dim3 block(kDenseMergeWarps * 32);
+    if (d.ctas <= 8 * units)
+        HOGATT_CUDA_OK(launch_kernel(dense_merge_kernel<T, true, false, kDenseMergeBatch>, dim3((unsigned)std::min(8 * units, resident)), block, 0, stream, d));
+    else
+        HOGATT_CUDA_OK(launch_kernel(dense_merge_kernel<T, true, true, 1>, dim3((unsigned)(64 * units)), block, 0, stream, d));
+    return HOGATT_OK;
+}
+
 // Bookkeeping runs as one cluster; the copies follow on the whole GPU.
 int launch_copies(const hogatt_block_tensors* t, const int* count, const int* pairs, int64_t most, int sms, cudaStream_t stream) {
     for (int first = 0; first < t->count; first += kMaxPageTensors) {
@@ -227,6 +373,8 @@ int hogatt_paged_q4_sdpa_launch(const hogatt_paged_q4_problem* x, hogatt_stream_
     if (rc != HOGATT_OK) return rc;
     if (p->workspace_bytes < pl.total) return HOGATT_ERR_WORKSPACE_TOO_SMALL;
 
+    if (pl.kernel == HOGATT_KERNEL_DENSE)
+        return p->dtype == HOGATT_F16 ? launch_q4_dense<__half>(x, pl, dev, smem_optin, stream) : launch_q4_dense<__nv_bfloat16>(x, pl, dev, smem_optin, stream);
     Q4Args args;
     memset(&args, 0, sizeof(args));
     PagedArgs& a = args.p;

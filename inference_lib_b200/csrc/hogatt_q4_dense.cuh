@@ -1,0 +1,179 @@
+// Packed prompt chunks over 4-bit pages on the tcgen05 kernel (hogatt_dense.cuh with Q4): head size 128, blocks of a multiple of eight rows.
+//
+// The tensor cores take both operands in one 16-bit type from swizzled shared memory, so what the TMA does for 16-bit pages a warp does
+// here: two warps unpack K tiles, two V tiles, 64 keys each.  A key is a row of 64 bytes of codes and 8 of scales, copied 32 keys at a time by
+// cp.async, two units ahead (rings of three; the K ring of tiles gives one of its three places for them), converted two values
+// per instruction, multiplied by their scales -- exact in fp16 -- and stored where the 128-byte swizzle wants them.  That is 1,600
+// instructions a step of the four warps together beside 5,600 of the softmax warps.  Unpacking into 16-bit pages in the workspace
+// first would take four times the cache's memory.
+//
+// fp16 for both products: six significant bits times a probability; bf16 queries become fp16 once per call, a power of two per (token, head)
+// taken out (q4_dense_queries_kernel), which the softmax multiplies back in.
+//
+// Values that are not numbers are stored as zeros, keys without a page as zeros too; what is special about a tile travels to the softmax
+// warps in a ring of eight words (K tiles are at most three ahead of the scores that are read), and only for such tiles they look
+// the scales and the block table up again: a row that sees such a value has NaN in that group's channels.
+#pragma once
+#include "hogatt_dense.cuh"
+#include "hogatt_q4_mma.cuh"
+
+namespace hogatt {
+
+// row (of all pages and heads) of key `key` of sequence w; -1 behind the keys, -2 a key without a page
+__device__ __forceinline__ int64_t q4_dense_row(const DenseArgs& a, int w, int h, int key, int len) {
+    if (key >= len) return -1;
+    const int at = (int)fast_div((uint32_t)key, {a.block_mul, a.block_shift, 0u});
+    const int p = at < a.max_blocks ? a.block_table[(size_t)w * a.max_blocks + at] : -1;
+    if (p < 0 || p >= a.num_blocks) return -2;
+    return ((int64_t)p * a.Hkv + h) * a.block_size + (key - at * a.block_size);
+}
+
+// Tile t (128 keys) of sequence w's K (which 0) or V (1), kv head h, into the tile at `dst`; `len` keys are seen by anybody, the segment's
+// tiles are t0 ... t1 - 1.  Whole warp.  `pack`: the warp's ring of packed units of 32 keys, all but one of which are under way.  (A copy takes
+// two microseconds here: with two under way a tile took four.  One unit's loads are in front of its conversions: with each load in front of
+// its own, a tile took four as well.)
+template <class C>
+__device__ __forceinline__ void q4_unpack(const DenseArgs& a, int which, int w, int h, int t, int t0, int t1, int len, uint32_t pack, uint32_t dst,
+                                          unsigned char* odd, Q4Pipe& pipe, int lane) {
+    constexpr int AHEAD = C::NPACK - 1;
+    const int r = lane >> 2, q = lane & 3;
+    const unsigned char* const codes = a.codes[which] + r * 64 + q * 16;
+    // scales, two rows a lane: K's or V's by lanes 0-15; behind K's the values', to see what is special about them
+    const bool second = lane >= 16;
+    const unsigned char* const scales = a.scales[second ? 1 : which] + q * 16;
+    auto look_up = [&](int window) { return q4_dense_row(a, w, h, window * 256 + lane * 8, len); };
+    // the next unit's turn: its window, and its copies if it belongs to the segment: 4 groups of 8 rows (a group lies in one block), a row's four
+    // 16-byte pieces by four lanes
+    auto fetch = [&](int unit) {
+        if ((unit & 7) == 0 && unit != 4 * t0) {
+            pipe.rows = pipe.next;
+            pipe.next = look_up((unit >> 3) + 1);
+            pipe.before = pipe.none;
+            pipe.none = __ballot_sync(0xffffffffu, pipe.rows == -2);
+            if (which == 0 && pipe.none && lane == 0 && a.status) atomicOr(a.status, STATUS_BAD_BLOCK);
+        }
+        if (unit < 4 * t1) {
+            const int left = len - unit * 32, from = (unit & 7) * 4;
+            const uint32_t at = pack + (uint32_t)(unit % C::NPACK) * C::PACK_BYTES;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t row0 = __shfl_sync(0xffffffffu, pipe.rows, from + i);
+                const bool real = row0 >= 0 && i * 8 + r < left;
+                cp_async_zfill<16>(at + (i * 8 + r) * 64 + q * 16, codes + (real ? row0 * 64 : 0), real);
+            }
+            const int64_t row0 = __shfl_sync(0xffffffffu, pipe.rows, from + (r & 3));
+            const int rows = row0 >= 0 ? max(0, min(2, left - (lane & 15) * 2)) : 0;
+            if (!second || which == 0)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + 2048 + lane * 16), "l"(scales + (rows > 0 ? row0 * 8 : 0)), "r"(rows * 8) : "memory");
+        }
+        cp_async_commit();
+    };
+    if (t == t0) {
+        __syncwarp();
+        pipe.rows = look_up(4 * t >> 3);
+        pipe.next = look_up((4 * t >> 3) + 1);
+        pipe.none = __ballot_sync(0xffffffffu, pipe.rows == -2);
+        if (which == 0 && pipe.none && lane == 0 && a.status) atomicOr(a.status, STATUS_BAD_BLOCK);
+#pragma unroll 1
+        for (int k = 0; k < AHEAD; ++k) fetch(4 * t + k);
+    }
+    // where the four words (32 channels) of a lane's row go: the pair of words that is stored first differs between the column halves, so that
+    // eight lanes hit all banks
+    const int p0 = q >> 1;
+    const uint32_t to = dst + (uint32_t)((q >> 1) * C::ATOM_BYTES + r * 128 + ((((q & 1) * 4 + 2 * p0) ^ r) * 16));      // (word k: the address ^ 16 k)
+    const uint32_t sel0 = p0 ? 0x3232 : 0x1010, sel1 = p0 ? 0x1010 : 0x3232;
+    bool special = false;
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) {
+        const int unit = 4 * t + k;
+        __syncwarp();                                     // (every lane has left the unit whose place is next)
+        fetch(unit + AHEAD);
+        cp_async_wait<AHEAD>();
+        __syncwarp();
+        const uint32_t at = pack + (uint32_t)(unit % C::NPACK) * C::PACK_BYTES, from = at + r * 64 + q * 16 + p0 * 8, sfrom = at + 2048 + r * 8 + q * 2;
+        const uint32_t put = to + k * 32 * 128;
+        uint2 w0[4], w1[4];
+        uint32_t sc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w0[i] = i == 0 ? lds64<0>(from) : i == 1 ? lds64<512>(from) : i == 2 ? lds64<1024>(from) : lds64<1536>(from);
+            w1[i] = i == 0 ? lds64<0>(from ^ 8u) : i == 1 ? lds64<512>(from ^ 8u) : i == 2 ? lds64<1024>(from ^ 8u) : lds64<1536>(from ^ 8u);
+            sc[i] = i == 0 ? lds16<0>(sfrom) : i == 1 ? lds16<64>(sfrom) : i == 2 ? lds16<128>(sfrom) : lds16<192>(sfrom);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t s = sc[i];
+            if (which == 1) {                             // a NaN scale becomes zero (0x7f + 1 reaches the sign bit)
+                const uint32_t bits = ((s & 0x7f7fu) + 0x0101u) & 0x8080u;
+                s &= ~(bits | (bits - (bits >> 7)));
+            }
+            s = from_e4m3x2(s);
+            const uint32_t y0 = __byte_perm(s, s, sel0), y1 = __byte_perm(s, s, sel1);
+            const uint32_t words[4] = {w0[i].x, w0[i].y, w1[i].x, w1[i].y};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t x[4];
+                const uint32_t y = j < 2 ? y0 : y1;
+                from_e2m1x8(words[j], x);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"((put ^ (16 * j)) + i * 1024), "r"(mul_half2(x[0], y)), "r"(mul_half2(x[1], y)),
+                             "r"(mul_half2(x[2], y)), "r"(mul_half2(x[3], y)) : "memory");
+            }
+        }
+        if (which == 0) {
+            const uint4 v = lds128<2304>(at + (lane & 15) * 16);
+            const uint32_t nan = ((v.x & 0x7f7f7f7fu) + 0x01010101u) | ((v.y & 0x7f7f7f7fu) + 0x01010101u) | ((v.z & 0x7f7f7f7fu) + 0x01010101u) |
+                                 ((v.w & 0x7f7f7f7fu) + 0x01010101u);
+            special = special || __any_sync(0xffffffffu, (nan & 0x80808080u) != 0);
+            // four bits, one per eight keys, to bits of the unit's keys
+            const uint32_t g = ~((unit >> 3 == (unit + AHEAD) >> 3 ? pipe.none : pipe.before) >> (unit & 7) * 4);
+            if (lane == 0) *reinterpret_cast<volatile uint32_t*>(odd + k * 4) = ((g & 1u) | (g & 2u) << 7 | (g & 4u) << 14 | (g & 8u) << 21) * 0xffu;
+        }
+    }
+    if (which == 0 && lane == 0) *reinterpret_cast<volatile uint32_t*>(odd + 16) = special;
+    fence_proxy_async_smem();                             // generic-proxy writes before the MMA's async-proxy reads
+    __syncwarp();
+}
+
+// Groups of channels in which some value of keys tok0 ... tok0 + n - 1 is not a number.
+__device__ __forceinline__ uint32_t q4_odd_groups(const DenseArgs& a, int w, int h, int tok0, int n) {
+    uint32_t odd = 0;
+#pragma unroll 1
+    for (int k = 0; k < n; ++k) {
+        const int64_t row = q4_dense_row(a, w, h, tok0 + k, INT_MAX);
+        if (row < 0) continue;
+#pragma unroll 1
+        for (int g = 0; g < 8; ++g)
+            if (is_nan_e4m3(a.scales[1][row * 8 + g])) odd |= 1u << g;
+    }
+    return odd;
+}
+
+// bf16 queries as fp16, each (token, head)'s largest magnitude (over the fragments) brought to [2^14, 2^15); factor: what brings its scores
+// back, with the scale.  A row with an infinity or a NaN becomes NaN.  One warp per (token, head), four channels per lane.  It starts beside the
+// plan kernel, which is behind everything that may still write the queries, and ends after it.
+__global__ void __launch_bounds__(256) q4_dense_queries_kernel(const __nv_bfloat16* q, __half* out, float* factor, int F, int rows, float l2scale) {
+    const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row < rows) {
+        uint32_t top = 0;
+        for (int f = 0; f < F; ++f) {
+            const uint2 v = *reinterpret_cast<const uint2*>(q + ((size_t)f * rows + row) * 128 + lane * 4);
+            top = max(max(top, max(v.x & 0x7fff0000u, (v.x & 0x7fffu) << 16)), max(v.y & 0x7fff0000u, (v.y & 0x7fffu) << 16));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const bool finite = top < 0x7f800000u;
+        const int e = min(120, 14 - ((int)(top >> 23) - 127));
+        const float up = finite ? __int_as_float((e + 127) << 23) : NAN;
+        if (lane == 0) factor[row] = finite ? fmaxf(l2scale * __int_as_float((127 - e) << 23), 1e-36f) : l2scale;
+        for (int f = 0; f < F; ++f) {
+            const size_t at = ((size_t)f * rows + row) * 128 + lane * 4;
+            const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(q + at);
+            *reinterpret_cast<uint2*>(out + at) = make_uint2(pack2<__half>(__low2float(v[0]) * up, __high2float(v[0]) * up),
+                                                             pack2<__half>(__low2float(v[1]) * up, __high2float(v[1]) * up));
+        }
+    }
+    pdl_wait();
+    pdl_trigger();
+}
+
+}  // namespace hogatt

@@ -198,12 +198,14 @@ def paged(A, q, loc, lens, cache, table, scale, units=(1.0, 1.0), cu=None, out=N
     return got, exact
 
 
-KERNELS = [None, 1, 2]                                       # the operator; by name on the CUDA cores; mma.sync
+KERNELS = [None, 1, 2, 4]                                    # the operator; by name on the CUDA cores; mma.sync; tcgen05
 
 
-def skip_unless_eligible(kernel, dtype, E, Ev):
+def skip_unless_eligible(kernel, dtype, E, Ev, packed=False, bs=8):
     if kernel == 2 and (dtype == torch.float32 or E != Ev or E not in (64, 128)):
         pytest.skip("not for this type and head size")
+    if kernel == 4 and (dtype == torch.float32 or E != 128 or Ev != 128 or not packed or bs % 8):
+        pytest.skip("not for this type, head size or layout")
 
 
 SHAPES = [
@@ -249,6 +251,8 @@ PACKED = [
     (torch.bfloat16, [40, 1, 0, 2], 1, 7, 128, 8, 1, 301, (1.0, 2.0)),
     (torch.float16, [0, 150, 1, 33], 1, 8, 128, 32, 2, 200, (1.0, 1.0)),
     (torch.bfloat16, [129], 2, 1, 128, 128, 1, 129, (1.0, 1.0)),
+    (torch.bfloat16, [200, 1, 70], 2, 4, 128, 24, 1, 700, (0.25, 4.0)),
+    (torch.float16, [65, 3, 0, 64], 2, 2, 128, 16, 3, 260, (1.0, 2.0 ** -12)),
     (torch.float32, [2, 3], 1, 20, 128, 16, 1, 50, (1.0, 1.0)),
 ]
 
@@ -258,7 +262,7 @@ PACKED = [
 @pytest.mark.parametrize("kernel", KERNELS)
 def test_packed_attention(A, case, causal, kernel):
     dtype, counts, Hkv, G, E, bs, F, keys, units = case
-    skip_unless_eligible(kernel, dtype, E, E)
+    skip_unless_eligible(kernel, dtype, E, E, True, bs)
     gen, rng = torch.Generator().manual_seed(keys), np.random.default_rng(keys)
     W, T, width = len(counts), sum(counts), -(-keys // bs) + 1
     blocks = W * width + 1
@@ -292,7 +296,7 @@ def odd_scales(rng, cache, table, bs, spots):
 @pytest.mark.parametrize("kernel", KERNELS)
 def test_numbers_that_are_not(A, dtype, E, counts, bs, kernel):
     """A NaN key is the whole row's, a NaN value its channels', and only of rows that see it; behind the lengths there may be anything."""
-    skip_unless_eligible(kernel, dtype, E, E)
+    skip_unless_eligible(kernel, dtype, E, E, True, bs)
     gen, rng = torch.Generator().manual_seed(5), np.random.default_rng(5)
     Hkv, G, keys, W, T = 2, 4, 150, len(counts), sum(counts)
     width = -(-keys // bs)
@@ -331,6 +335,28 @@ def test_keys_without_a_page_are_not_seen(A, dtype, E, G, kernel, bs):
     assert int(st) == 1024 and bool((got.reshape(W, 2, -1)[2] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_packed_chunks_over_tables_with_holes(A, dtype, kernel):
+    """Keys without a page and values that are not numbers in the middle of chunks, over several fragments; rows that see nothing."""
+    gen, rng = torch.Generator().manual_seed(12), np.random.default_rng(12)
+    Hkv, G, E, bs, counts, keys, F = 2, 4, 128, 8, [150, 1, 33, 40], 320, 2
+    W, T, width, cu = len(counts), sum(counts), keys // bs, torch.tensor([0, 150, 151, 184, 224], dtype=torch.int32)
+    (kc, ks), (vc, vs) = (q4_util.random_cache(gen, W * width, Hkv, bs, E) for _ in range(2))
+    table = table_of(rng, W, width, W * width)
+    cache = [kc, vc, ks, vs]
+    odd_scales(rng, cache, table, bs, [(0, 200, 1, 0, 7), (0, 210, 1, 1, 2), (0, 3, 1, 0, 0), (2, 310, 1, 1, 5), (2, 300, 0, 0, 1)])
+    table[0, 25], table[0, 12], table[1, :], table[2, 39], table[3, 3] = -1, W * width, -1, 1 << 30, -2        # (25: the page of the first odd value)
+    lens = torch.tensor([[320, 320, 320, 0], [100, 7, 320, 33]], dtype=torch.int32)
+    loc = torch.from_numpy(rng.integers(-1, keys + 5, (F, T)).astype(np.int32))
+    loc[0, :150] = torch.arange(170, 320)
+    q = torch.randn(F, T, Hkv * G, E, generator=gen).to(dtype)
+    st = status()
+    got, exact = paged(A, q, loc, lens, cache, table, E ** -0.5, cu=cu, st=st, kernel=kernel)
+    q4_util.check(got, exact)
+    assert int(st) == 1024
+
+
 def test_rows_that_see_nothing_are_zero(A):
     gen = torch.Generator().manual_seed(7)
     cache = [x for pair in zip(*(q4_util.random_cache(gen, 8, 2, 16, 128) for _ in range(2))) for x in pair]
@@ -362,6 +388,7 @@ def test_large_and_small_queries(A):
 @pytest.mark.parametrize("scale", [0.0, -0.1, 1e-30, 3.0])
 @pytest.mark.parametrize("kernel", KERNELS)
 def test_scales_of_the_scores(A, scale, kernel):
+    skip_unless_eligible(kernel, torch.bfloat16, 128, 128)
     gen = torch.Generator().manual_seed(10)
     cache = [x for pair in zip(*(q4_util.random_cache(gen, 8, 2, 16, 128) for _ in range(2))) for x in pair]
     q = torch.randn(1, 2, 6, 1, 128, generator=gen).bfloat16()
