@@ -660,7 +660,7 @@ __device__ __forceinline__ void dense_fetch(const DenseArgs& a, const CUtensorMa
 
 // ---- pages in 4 bits: defined in hogatt_q4_dense.cuh, which only its users include -------------------------------------
 struct Q4Pipe {            // a warp's look at the block table: windows of eight units of 32 keys
-    int64_t rows, next;    // lane 4 u + i: where rows 8 i ... of unit u of the window, and of the one behind it, begin
+    int rows, next;        // lane 4 u + i: where rows 8 i ... of unit u of the window, and of the one behind it, begin
     uint32_t none, before; // the same lanes' bits: keys without a page, in the window and in the one in front of it
 };
 template <class C>

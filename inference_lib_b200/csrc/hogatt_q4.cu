@@ -63,7 +63,8 @@ struct Q4Plan {
 // Packed queries on the tcgen05 kernel: head size 128, blocks of a multiple of eight rows.
 bool dense_eligible(const hogatt_paged_problem* p) {
     return p->cu_seqlens_q != nullptr && (p->dtype == HOGATT_F16 || p->dtype == HOGATT_BF16) && p->E == 128 && p->Ev == 128 && p->block_size % 8 == 0 &&
-           p->Hq / p->Hkv <= kDenseRows && (int64_t)p->total_q_tokens * p->Hq * p->F < ((int64_t)1 << 31) && p->scale >= 1e-30f && p->scale <= 1e30f;
+           p->Hq / p->Hkv <= kDenseRows && (int64_t)p->num_blocks * p->Hkv * p->block_size < ((int64_t)1 << 31) &&
+           (int64_t)p->total_q_tokens * p->Hq * p->F < ((int64_t)1 << 31) && p->scale >= 1e-30f && p->scale <= 1e30f;
 }
 // AUTO takes it where the tokens beyond one per sequence, over as many keys as the block table has room for, would keep the other
 // kernel busy for long (as for 16-bit pages).

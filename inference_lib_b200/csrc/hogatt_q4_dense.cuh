@@ -19,13 +19,13 @@
 
 namespace hogatt {
 
-// row (of all pages and heads) of key `key` of sequence w; -1 behind the keys, -2 a key without a page
-__device__ __forceinline__ int64_t q4_dense_row(const DenseArgs& a, int w, int h, int key, int len) {
+// row (of all pages and heads: fewer than 2^31, 64 bytes each) of key `key` of sequence w; -1 behind the keys, -2 a key without a page
+__device__ __forceinline__ int q4_dense_row(const DenseArgs& a, int w, int h, int key, int len) {
     if (key >= len) return -1;
     const int at = (int)fast_div((uint32_t)key, {a.block_mul, a.block_shift, 0u});
     const int p = at < a.max_blocks ? a.block_table[(size_t)w * a.max_blocks + at] : -1;
     if (p < 0 || p >= a.num_blocks) return -2;
-    return ((int64_t)p * a.Hkv + h) * a.block_size + (key - at * a.block_size);
+    return (p * a.Hkv + h) * a.block_size + (key - at * a.block_size);
 }
 
 // Tile t (128 keys) of sequence w's K (which 0) or V (1), kv head h, into the tile at `dst`; `len` keys are seen by anybody, the segment's
@@ -36,11 +36,13 @@ template <class C>
 __device__ __forceinline__ void q4_unpack(const DenseArgs& a, int which, int w, int h, int t, int t0, int t1, int len, uint32_t pack, uint32_t dst,
                                           unsigned char* odd, Q4Pipe& pipe, int lane) {
     constexpr int AHEAD = C::NPACK - 1;
-    const int r = lane >> 2, q = lane & 3;
+    // a lane's row of eight and quarter of it: eight lanes in a row are four rows and one half of their channels, which all stores below take to
+    // different banks; in the ring the halves of every second pair of rows change places, for the loads
+    const int r = (lane >> 4) * 4 + ((lane >> 1) & 3), q = ((lane >> 3) & 1) * 2 + (lane & 1), in_ring = r * 64 + (q ^ (r & 2)) * 16;
     const unsigned char* const codes = a.codes[which] + r * 64 + q * 16;
     // scales, two rows a lane: K's or V's by lanes 0-15; behind K's the values', to see what is special about them
     const bool second = lane >= 16;
-    const unsigned char* const scales = a.scales[second ? 1 : which] + q * 16;
+    const unsigned char* const scales = a.scales[second ? 1 : which] + (lane & 3) * 16;
     auto look_up = [&](int window) { return q4_dense_row(a, w, h, window * 256 + lane * 8, len); };
     // the next unit's turn: its window, and its copies if it belongs to the segment: 4 groups of 8 rows (a group lies in one block), a row's four
     // 16-byte pieces by four lanes
@@ -55,16 +57,25 @@ __device__ __forceinline__ void q4_unpack(const DenseArgs& a, int which, int w, 
         if (unit < 4 * t1) {
             const int left = len - unit * 32, from = (unit & 7) * 4;
             const uint32_t at = pack + (uint32_t)(unit % C::NPACK) * C::PACK_BYTES;
+            if (left >= 32 && (pipe.none >> from & 0xfu) == 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int64_t row0 = __shfl_sync(0xffffffffu, pipe.rows, from + i);
-                const bool real = row0 >= 0 && i * 8 + r < left;
-                cp_async_zfill<16>(at + (i * 8 + r) * 64 + q * 16, codes + (real ? row0 * 64 : 0), real);
+                for (int i = 0; i < 4; ++i)
+                    cp_async_16(at + i * 512 + in_ring, codes + (int64_t)__shfl_sync(0xffffffffu, pipe.rows, from + i) * 64, true);
+                const int64_t row0 = __shfl_sync(0xffffffffu, pipe.rows, from + ((lane >> 2) & 3));
+                if (!second || which == 0) cp_async_16(at + 2048 + lane * 16, scales + row0 * 8, true);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row0 = __shfl_sync(0xffffffffu, pipe.rows, from + i);
+                    const bool real = row0 >= 0 && i * 8 + r < left;
+                    cp_async_zfill<16>(at + i * 512 + in_ring, codes + (real ? (int64_t)row0 * 64 : 0), real);
+                }
+                const int row0 = __shfl_sync(0xffffffffu, pipe.rows, from + ((lane >> 2) & 3));
+                const int rows = row0 >= 0 ? max(0, min(2, left - (lane & 15) * 2)) : 0;
+                if (!second || which == 0)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + 2048 + lane * 16), "l"(scales + (rows > 0 ? (int64_t)row0 * 8 : 0)), "r"(rows * 8)
+                                 : "memory");
             }
-            const int64_t row0 = __shfl_sync(0xffffffffu, pipe.rows, from + (r & 3));
-            const int rows = row0 >= 0 ? max(0, min(2, left - (lane & 15) * 2)) : 0;
-            if (!second || which == 0)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + 2048 + lane * 16), "l"(scales + (rows > 0 ? row0 * 8 : 0)), "r"(rows * 8) : "memory");
         }
         cp_async_commit();
     };
@@ -77,11 +88,7 @@ __device__ __forceinline__ void q4_unpack(const DenseArgs& a, int which, int w, 
 #pragma unroll 1
         for (int k = 0; k < AHEAD; ++k) fetch(4 * t + k);
     }
-    // where the four words (32 channels) of a lane's row go: the pair of words that is stored first differs between the column halves, so that
-    // eight lanes hit all banks
-    const int p0 = q >> 1;
-    const uint32_t to = dst + (uint32_t)((q >> 1) * C::ATOM_BYTES + r * 128 + ((((q & 1) * 4 + 2 * p0) ^ r) * 16));      // (word k: the address ^ 16 k)
-    const uint32_t sel0 = p0 ? 0x3232 : 0x1010, sel1 = p0 ? 0x1010 : 0x3232;
+    const uint32_t to = dst + (uint32_t)((q >> 1) * C::ATOM_BYTES + r * 128 + ((((q & 1) * 4) ^ r) * 16));       // (word k of a row: this address ^ 16 k)
     bool special = false;
 #pragma unroll 1
     for (int k = 0; k < 4; ++k) {
@@ -90,16 +97,10 @@ __device__ __forceinline__ void q4_unpack(const DenseArgs& a, int which, int w, 
         fetch(unit + AHEAD);
         cp_async_wait<AHEAD>();
         __syncwarp();
-        const uint32_t at = pack + (uint32_t)(unit % C::NPACK) * C::PACK_BYTES, from = at + r * 64 + q * 16 + p0 * 8, sfrom = at + 2048 + r * 8 + q * 2;
+        const uint32_t at = pack + (uint32_t)(unit % C::NPACK) * C::PACK_BYTES, from = at + in_ring, sfrom = at + 2048 + r * 8 + q * 2;
         const uint32_t put = to + k * 32 * 128;
-        uint2 w0[4], w1[4];
-        uint32_t sc[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            w0[i] = i == 0 ? lds64<0>(from) : i == 1 ? lds64<512>(from) : i == 2 ? lds64<1024>(from) : lds64<1536>(from);
-            w1[i] = i == 0 ? lds64<0>(from ^ 8u) : i == 1 ? lds64<512>(from ^ 8u) : i == 2 ? lds64<1024>(from ^ 8u) : lds64<1536>(from ^ 8u);
-            sc[i] = i == 0 ? lds16<0>(sfrom) : i == 1 ? lds16<64>(sfrom) : i == 2 ? lds16<128>(sfrom) : lds16<192>(sfrom);
-        }
+        const uint4 w[4] = {lds128<0>(from), lds128<512>(from), lds128<1024>(from), lds128<1536>(from)};
+        const uint32_t sc[4] = {lds16<0>(sfrom), lds16<64>(sfrom), lds16<128>(sfrom), lds16<192>(sfrom)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             uint32_t s = sc[i];
@@ -108,8 +109,8 @@ __device__ __forceinline__ void q4_unpack(const DenseArgs& a, int which, int w, 
                 s &= ~(bits | (bits - (bits >> 7)));
             }
             s = from_e4m3x2(s);
-            const uint32_t y0 = __byte_perm(s, s, sel0), y1 = __byte_perm(s, s, sel1);
-            const uint32_t words[4] = {w0[i].x, w0[i].y, w1[i].x, w1[i].y};
+            const uint32_t y0 = __byte_perm(s, s, 0x1010), y1 = __byte_perm(s, s, 0x3232);
+            const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t x[4];
@@ -139,11 +140,11 @@ __device__ __forceinline__ uint32_t q4_odd_groups(const DenseArgs& a, int w, int
     uint32_t odd = 0;
 #pragma unroll 1
     for (int k = 0; k < n; ++k) {
-        const int64_t row = q4_dense_row(a, w, h, tok0 + k, INT_MAX);
+        const int row = q4_dense_row(a, w, h, tok0 + k, INT_MAX);
         if (row < 0) continue;
 #pragma unroll 1
         for (int g = 0; g < 8; ++g)
-            if (is_nan_e4m3(a.scales[1][row * 8 + g])) odd |= 1u << g;
+            if (is_nan_e4m3(a.scales[1][(int64_t)row * 8 + g])) odd |= 1u << g;
     }
     return odd;
 }
