@@ -64,7 +64,7 @@ struct Q4MmaCfg {
 };
 template <int HD>
 __host__ __device__ inline size_t q4_mma_smem_bytes(int nt, int W, int groups, bool list) {
-    return Q4MmaCfg<HD>::work_bytes(nt) + (list ? ((size_t)W + 1 + groups + 1) * sizeof(int) : 0);
+    return Q4MmaCfg<HD>::work_bytes(nt) + (list ? ((size_t)W + 1 + 2 * groups + 1) * sizeof(int) : 0);
 }
 
 // the 8x8 matrix of 16-bit elements that the warp holds (row lane / 4, columns 2 (lane % 4) and + 1), transposed
@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
     const uint32_t ring_u32 = smem_u32(ring);
     int* const first_group = reinterpret_cast<int*>(smem_raw + C::work_bytes(NT));      // [W + 1]
     int* const pre = first_group + a.W + 1;                                              // [groups + 1]
+    int* const seen = pre + a.groups_bound + 1;                                          // [groups]: the group's visible keys, of the last fragment
     const unsigned char* const kc = static_cast<const unsigned char*>(a.kcache);
     const unsigned char* const vc = static_cast<const unsigned char*>(a.vcache);
     const int per_group = a.Hkv * a.head_blocks;          // units of a group of query tokens
@@ -190,12 +191,18 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
     int groups = 0;
     if (x.ctas) {
         int before = 0;
-        for (int w0 = 0; w0 < a.W; w0 += kQ4Threads) {
-            int start, n = 0, total;
-            if (w0 + tid < a.W) n = (tokens_of(a, w0 + tid, &start) + a.tokens_per_group - 1) / a.tokens_per_group;
-            const int at = before + block_exclusive(n, &total);
-            if (w0 + tid < a.W) first_group[w0 + tid] = at;
-            before += total;
+        if (a.cu_seqlens) {
+            for (int w0 = 0; w0 < a.W; w0 += kQ4Threads) {
+                int start, n = 0, total;
+                if (w0 + tid < a.W) n = (tokens_of(a, w0 + tid, &start) + a.tokens_per_group - 1) / a.tokens_per_group;
+                const int at = before + block_exclusive(n, &total);
+                if (w0 + tid < a.W) first_group[w0 + tid] = at;
+                before += total;
+            }
+        } else {
+            const int each = (a.S + a.tokens_per_group - 1) / a.tokens_per_group;
+            for (int w = tid; w < a.W; w += kQ4Threads) first_group[w] = w * each;
+            before = a.W * each;
         }
         groups = min(before, a.groups_bound);
         if (tid == 0) first_group[a.W] = before;
@@ -213,7 +220,12 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
                 }
                 int start;
                 const int tokens = tokens_of(a, lo, &start), s0 = (e - first_group[lo]) * a.tokens_per_group;
-                for (int f = 0; f < a.F; ++f) n += ceil_div(group_visible(a, f, lo, start, s0, min(tokens, s0 + a.tokens_per_group)), kQ4Tile);
+                int vis = 0;
+                for (int f = 0; f < a.F; ++f) {
+                    vis = group_visible(a, f, lo, start, s0, min(tokens, s0 + a.tokens_per_group));
+                    n += ceil_div(vis, kQ4Tile);
+                }
+                seen[e] = vis;
             }
             const int at = before + block_exclusive(n, &total);
             if (e < groups) pre[e] = at;
@@ -286,82 +298,12 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
         bool whole = true;                                // this CTA has all of the unit's tiles
         for (int f = 0; f < a.F; ++f) {
             // ---- this fragment's tiles of the share ----
-            const int vis = group_visible(a, f, u.w, u.s_base, u.s_begin, u.s_end);
+            const int vis = x.ctas && a.F == 1 ? seen[grp] : group_visible(a, f, u.w, u.s_base, u.s_begin, u.s_end);
             const int tiles = ceil_div(vis, kQ4Tile);
             const int b0 = max(j0, tiles_before) - tiles_before, b1 = min(j1, tiles_before + tiles) - tiles_before;
             whole = whole && (tiles == 0 || (b0 == 0 && b1 == tiles));
             tiles_before += tiles;
             if (b0 >= b1) continue;
-
-            // ---- its query rows as B fragments: thread (g, t) has channels CPT t ... of row g of each eight ----
-            uint32_t q[NT == 1 ? KS : 1][2];
-            uint4* const q_smem = reinterpret_cast<uint4*>(smem_raw + C::ring_bytes(NT)) + lane;
-            if (NT == 2 && f > 0) __syncthreads();        // (every warp has left the last fragment)
-            float factor[NT][2];                          // what a product of columns 2 t, 2 t + 1 is multiplied with: log2 e * scale / row's power
-            int lim[NT][2], lowest = INT_MAX;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                int s_abs, hq;
-                const bool real = paged_row(a, u, n * 8 + g, &s_abs, &hq);
-                uint4 raw[CPT / 8];
-#pragma unroll
-                for (int k = 0; k < CPT / 8; ++k) raw[k] = make_uint4(0u, 0u, 0u, 0u);
-                if (real) {
-                    const T* src = static_cast<const T*>(a.q) + f * a.q_f + u.w * a.q_w + s_abs * a.q_s + hq * a.q_h + t * CPT;
-#pragma unroll
-                    for (int k = 0; k < CPT / 8; ++k) {
-                        const int4 v = load_16(src + k * 8);
-                        raw[k] = make_uint4(v.x, v.y, v.z, v.w);
-                    }
-                }
-                float mine = fabsf(a.l2scale);
-                uint32_t* r = reinterpret_cast<uint32_t*>(raw);
-                if constexpr (!std::is_same<T, __half>::value) {
-                    uint32_t top = 0;                     // the largest magnitude's bits: bf16 in the upper half
-#pragma unroll
-                    for (int k = 0; k < CPT / 2; ++k) top = max(top, max(r[k] & 0x7fff0000u, (r[k] & 0x7fffu) << 16));
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    // times 2^e so that the largest lies in [2^14, 2^15); an infinity or a NaN makes the row NaN
-                    const int e = min(120, 14 - ((int)(top >> 23) - 127));
-                    const float up = top >= 0x7f800000u ? NAN : __int_as_float((e + 127) << 23);
-                    mine *= top >= 0x7f800000u ? NAN : __int_as_float((127 - e) << 23);
-#pragma unroll
-                    for (int k = 0; k < CPT / 2; ++k) {
-                        const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&r[k]);
-                        r[k] = pack2<__half>(__low2float(v) * up, __high2float(v) * up);
-                    }
-                }
-                mine = fmaxf(mine, FLT_MIN);              // (a masked score is -inf and has to stay it; scores this small are none)
-                if (a.l2scale < 0.f) {                    // (the row's maximum is taken before the factor)
-#pragma unroll
-                    for (int k = 0; k < CPT / 2; ++k) r[k] ^= 0x80008000u;
-                }
-                if constexpr (NT == 1) {
-#pragma unroll
-                    for (int k = 0; k < KS; ++k) {
-                        q[k][0] = r[2 * k];
-                        q[k][1] = r[2 * k + 1];
-                    }
-                } else if (warp == 0) {
-#pragma unroll
-                    for (int k = 0; k < KS / 2; ++k) q_smem[(n * (KS / 2) + k) * 32] = raw[k];
-                }
-                int mylim = INT_MAX;                      // (a row that is not there is never masked, nor stored)
-                if (real) {
-                    const int loc = a.loc[(size_t)f * a.loc_f + (size_t)u.w * a.loc_w + s_abs];
-                    mylim = max(0, min(loc, a.flen[f * a.len_f + u.w * a.len_w] - 1) + 1);
-                }
-                lowest = min(lowest, mylim);
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {             // row 2 t + c is lane 8 t + 4 c's
-                    lim[n][c] = __shfl_sync(0xffffffffu, mylim, 8 * t + 4 * c);
-                    factor[n][c] = __shfl_sync(0xffffffffu, mine, 8 * t + 4 * c);
-                }
-            }
-#pragma unroll
-            for (int k = 4; k < 32; k <<= 1) lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, k));
-            if (NT == 2) __syncthreads();
 
             // ---- copies of 16 keys: rows of 4 (2) 16-byte chunks, dealt over the lanes; scales of K by lanes 0-15, of V by 16-31 ----
             constexpr int CPR = C::ROW / 16, PASSES = 16 * CPR / 32, RPP = 32 / CPR;
@@ -451,6 +393,76 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
                     cp_async_commit();
                 }
             }
+            // ---- the query rows as B fragments (the first copies are under way): thread (g, t) has channels CPT t ... of row g of each eight ----
+            uint32_t q[NT == 1 ? KS : 1][2];
+            uint4* const q_smem = reinterpret_cast<uint4*>(smem_raw + C::ring_bytes(NT)) + lane;
+            if (NT == 2 && f > 0) __syncthreads();        // (every warp has left the last fragment)
+            float factor[NT][2];                          // what a product of columns 2 t, 2 t + 1 is multiplied with: log2 e * scale / row's power
+            int lim[NT][2], lowest = INT_MAX;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                int s_abs, hq;
+                const bool real = paged_row(a, u, n * 8 + g, &s_abs, &hq);
+                uint4 raw[CPT / 8];
+#pragma unroll
+                for (int k = 0; k < CPT / 8; ++k) raw[k] = make_uint4(0u, 0u, 0u, 0u);
+                if (real) {
+                    const T* src = static_cast<const T*>(a.q) + f * a.q_f + u.w * a.q_w + s_abs * a.q_s + hq * a.q_h + t * CPT;
+#pragma unroll
+                    for (int k = 0; k < CPT / 8; ++k) {
+                        const int4 v = load_16(src + k * 8);
+                        raw[k] = make_uint4(v.x, v.y, v.z, v.w);
+                    }
+                }
+                float mine = fabsf(a.l2scale);
+                uint32_t* r = reinterpret_cast<uint32_t*>(raw);
+                if constexpr (!std::is_same<T, __half>::value) {
+                    uint32_t top = 0;                     // the largest magnitude's bits: bf16 in the upper half
+#pragma unroll
+                    for (int k = 0; k < CPT / 2; ++k) top = max(top, max(r[k] & 0x7fff0000u, (r[k] & 0x7fffu) << 16));
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    // times 2^e so that the largest lies in [2^14, 2^15); an infinity or a NaN makes the row NaN
+                    const int e = min(120, 14 - ((int)(top >> 23) - 127));
+                    const float up = top >= 0x7f800000u ? NAN : __int_as_float((e + 127) << 23);
+                    mine *= top >= 0x7f800000u ? NAN : __int_as_float((127 - e) << 23);
+#pragma unroll
+                    for (int k = 0; k < CPT / 2; ++k) {
+                        const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&r[k]);
+                        r[k] = pack2<__half>(__low2float(v) * up, __high2float(v) * up);
+                    }
+                }
+                mine = fmaxf(mine, FLT_MIN);              // (a masked score is -inf and has to stay it; scores this small are none)
+                if (a.l2scale < 0.f) {                    // (the row's maximum is taken before the factor)
+#pragma unroll
+                    for (int k = 0; k < CPT / 2; ++k) r[k] ^= 0x80008000u;
+                }
+                if constexpr (NT == 1) {
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        q[k][0] = r[2 * k];
+                        q[k][1] = r[2 * k + 1];
+                    }
+                } else if (warp == 0) {
+#pragma unroll
+                    for (int k = 0; k < KS / 2; ++k) q_smem[(n * (KS / 2) + k) * 32] = raw[k];
+                }
+                int mylim = INT_MAX;                      // (a row that is not there is never masked, nor stored)
+                if (real) {
+                    const int loc = a.loc[(size_t)f * a.loc_f + (size_t)u.w * a.loc_w + s_abs];
+                    mylim = max(0, min(loc, a.flen[f * a.len_f + u.w * a.len_w] - 1) + 1);
+                }
+                lowest = min(lowest, mylim);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {             // row 2 t + c is lane 8 t + 4 c's
+                    lim[n][c] = __shfl_sync(0xffffffffu, mylim, 8 * t + 4 * c);
+                    factor[n][c] = __shfl_sync(0xffffffffu, mine, 8 * t + 4 * c);
+                }
+            }
+#pragma unroll
+            for (int k = 4; k < 32; k <<= 1) lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, k));
+            if (NT == 2) __syncthreads();
+
             // row i of the product is key i with the last bit flipped in every second four: the loads of V then hit all banks
             const int ka = g ^ ((g >> 2) & 1), kb = ka + 8;
             const int flip = (t >> 1) & 1, v0 = 2 * t + flip, v1 = 2 * t + 1 - flip;
@@ -698,9 +710,10 @@ __global__ void __launch_bounds__(128) q4_mma_merge_kernel(const __grid_constant
     __shared__ float sm_m[4], sm_l[4], sm_o[4][HD];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, unit = blockIdx.x, row = blockIdx.y;
     const int per_group = a.Hkv * a.head_blocks, grp = unit / per_group;
+    PagedUnit u;
     pdl_wait();
     pdl_trigger();
-    PagedUnit u;
+    const bool there = locate_unit(a, unit, &u);          // (its loads beside the plan's)
     const int before = __ldcg(x.plan + grp), n = __ldcg(x.plan + grp + 1) - before;
     const int64_t N = (int64_t)__ldcg(x.plan + a.groups_bound) * per_group;
     int first = 0, count = 0;
@@ -711,9 +724,8 @@ __global__ void __launch_bounds__(128) q4_mma_merge_kernel(const __grid_constant
         count = cta_of_tile(start + n - 1, N, shares) - first + 1;
         if (count == 1) return;
     }
-    if (!locate_unit(a, unit, &u)) return;
     int s_abs, hq;
-    if (!paged_row(a, u, row, &s_abs, &hq)) return;
+    if (!there || !paged_row(a, u, row, &s_abs, &hq)) return;
     T* const out = static_cast<T*>(a.out) + u.w * a.o_w + s_abs * a.o_s + hq * a.o_h;
     float M = -FLT_MAX, L = 0.f, acc[VEC] = {};
     for (int p0 = warp; p0 < count; p0 += 32) {           // eight partials of a warp in flight
