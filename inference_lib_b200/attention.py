@@ -37,10 +37,14 @@ _VARLEN_PAGED_SDPA = torch.ops.libhogatt.hogwild_varlen_paged_sdpa.default
 _COPY_TO_BLOCKS = torch.ops.libhogatt.copy_to_blocks.default
 _PAGED_SDPA_Q4 = torch.ops.libhogatt.hogwild_paged_sdpa_q4.default
 _VARLEN_PAGED_SDPA_Q4 = torch.ops.libhogatt.hogwild_varlen_paged_sdpa_q4.default
+_PAGED_SDPA_Q4_NEW = torch.ops.libhogatt.hogwild_paged_sdpa_q4.new
+_VARLEN_PAGED_SDPA_Q4_NEW = torch.ops.libhogatt.hogwild_varlen_paged_sdpa_q4.new
 _COPY_TO_BLOCKS_Q4 = torch.ops.libhogatt.copy_to_blocks_q4.default
-_COPY_FROM_BLOCKS_Q4 = torch.ops.libhogatt.copy_from_blocks_q4.default
+_COPY_FROM_BLOCKS_Q4_NEW = torch.ops.libhogatt.copy_from_blocks_q4.new
 _STEP_BLOCKS = torch.ops.libhogatt.step_blocks.default
+_STEP_BLOCKS_NEW = torch.ops.libhogatt.step_blocks.new
 _COMPACT_BLOCKS = torch.ops.libhogatt.compact_blocks.default
+_COMPACT_BLOCKS_NEW = torch.ops.libhogatt.compact_blocks.new
 fragment_append = torch.ops.libhogatt.fragment_append.default              # FragmentCache.update's two steps
 fragment_step_plan = torch.ops.libhogatt.fragment_step_plan.default
 
@@ -147,7 +151,8 @@ def hogwild_paged_sdpa_q4(queries: torch.Tensor, locations: torch.Tensor, key_ca
                           value_unit: float = 1.0, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`hogwild_paged_sdpa` over a 4-bit cache: ``queries [F,W,Hq,S,E]`` (rotated) and ``out [W,Hq,S,Ev]`` in fp32, fp16 or bf16."""
     if out is None:
-        out = torch.empty((queries.size(1), queries.size(2), queries.size(3), value_cache.size(3) * 2), dtype=queries.dtype, device=queries.device)
+        return _PAGED_SDPA_Q4_NEW(scale, locations, queries.contiguous(), fragment_lengths, key_cache, value_cache, key_scales, value_scales,
+                                  block_table, key_unit, value_unit, status)
     _PAGED_SDPA_Q4(out, scale, locations, queries.contiguous(), fragment_lengths, key_cache, value_cache, key_scales, value_scales,
                    block_table, key_unit, value_unit, status)
     return out
@@ -160,7 +165,8 @@ def hogwild_varlen_paged_sdpa_q4(queries: torch.Tensor, locations: torch.Tensor,
     """:func:`hogwild_varlen_paged_sdpa` over a 4-bit cache: ``queries [F,total_q,Hq,E]``, ``locations [F,total_q]``,
     ``fragment_lengths [F,W]``, ``cu_seqlens_q [W+1]``.  Rows of ``out`` behind the last sequence are left as they are."""
     if out is None:
-        out = torch.empty((queries.size(1), queries.size(2), value_cache.size(3) * 2), dtype=queries.dtype, device=queries.device)
+        return _VARLEN_PAGED_SDPA_Q4_NEW(scale, locations, queries.contiguous(), fragment_lengths, key_cache, value_cache, key_scales,
+                                         value_scales, block_table, cu_seqlens_q, key_unit, value_unit, status)
     _VARLEN_PAGED_SDPA_Q4(out, scale, locations, queries.contiguous(), fragment_lengths, key_cache, value_cache, key_scales, value_scales,
                           block_table, cu_seqlens_q, key_unit, value_unit, status)
     return out
@@ -184,11 +190,8 @@ def copy_from_blocks_q4(key_cache: torch.Tensor, value_cache: torch.Tensor, key_
                         status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The numbers that a 4-bit cache holds: rows ``first_rows[b]`` ... ``first_rows[b] + rows - 1`` of every sequence of ``block_table``,
     as keys ``[B,Hkv,rows,E]`` and values ``[B,Hkv,rows,Ev]``.  Rows without a page are NaN."""
-    shape = (block_table.size(0), key_cache.size(1), int(rows))
-    keys = torch.empty(shape + (key_cache.size(3) * 2,), dtype=dtype, device=key_cache.device)
-    values = torch.empty(shape + (value_cache.size(3) * 2,), dtype=dtype, device=key_cache.device)
-    _COPY_FROM_BLOCKS_Q4(keys, values, key_cache, value_cache, key_scales, value_scales, block_table, first_rows, key_unit, value_unit, status)
-    return keys, values
+    return _COPY_FROM_BLOCKS_Q4_NEW(key_cache, value_cache, key_scales, value_scales, block_table, first_rows, rows, dtype, key_unit, value_unit,
+                                    status)
 
 
 # ---- the pages of a paged cache of any type (no counterpart in the reference) ------------------------------------------
@@ -206,9 +209,7 @@ def step_blocks(block_refs: torch.Tensor, block_table: torch.Tensor, seq_lengths
     ``room[w]`` = ``new_tokens[w]`` where the row has its pages, otherwise 0 (rows are served in order until the pool is empty).  ``out`` may
     hold the inputs themselves where there is no ``source``; ``block_refs`` always.  Nothing is read back from the device."""
     if out is None:
-        rows = seq_lengths.size(0) if source is None else source.size(0)
-        out = (torch.empty_like(block_refs), torch.empty((rows, block_table.size(-1)), dtype=torch.int32, device=block_table.device),
-               torch.empty(rows, dtype=torch.int32, device=block_table.device), torch.empty(rows, dtype=torch.int32, device=block_table.device))
+        return _STEP_BLOCKS_NEW(block_refs, block_table, seq_lengths, source, new_tokens, block_size, caches, status)
     refs, table, lengths, room = out
     _STEP_BLOCKS(block_refs, block_table, seq_lengths, source, new_tokens, block_size, caches, refs, table, lengths, room, status)
     return refs, table, lengths, room
@@ -220,7 +221,9 @@ def compact_blocks(block_refs: torch.Tensor, block_table: torch.Tensor, caches: 
     """Moves the held pages to the front of ``caches`` (in place) and returns ``(block_refs, block_table, moved)`` in new tensors or in
     ``out`` (which may hold the inputs): ``moved[p]`` is page ``p``'s new number, -1 for a free one.  The pages that are held end up as
     ``0 .. n-1``; one that was there already stays."""
-    refs, table, moved = out if out is not None else (torch.empty_like(block_refs), torch.empty_like(block_table), torch.empty_like(block_refs))
+    if out is None:
+        return _COMPACT_BLOCKS_NEW(block_refs, block_table, caches, status)
+    refs, table, moved = out
     _COMPACT_BLOCKS(block_refs, block_table, caches, refs, table, moved, status)
     return refs, table, moved
 

@@ -54,7 +54,10 @@ __device__ __forceinline__ StepRow step_row(const StepBlocksArgs& a, int w) {
     if (bad || r.from < 0) r.from = -1;
     r.length = r.from >= 0 ? max(0, __ldcg(a.lengths_in + r.from)) : 0;
     r.add = a.new_tokens ? max(0, a.new_tokens[w]) : 0;
-    const int64_t kept = ((int64_t)r.length + a.block_size - 1) / a.block_size, want = ((int64_t)r.length + r.add + a.block_size - 1) / a.block_size;
+    // (a length and a block size are below 2^31: the sum fits 32 bits without sign; with new tokens it may not)
+    const uint32_t bs = (uint32_t)a.block_size;
+    const int64_t kept = ((uint32_t)r.length + bs - 1) / bs, all = (int64_t)r.length + r.add + bs - 1;
+    const int64_t want = all >> 32 ? all / bs : (int64_t)((uint32_t)all / bs);
     r.kept = (int)min(kept, (int64_t)a.max_blocks);
     r.over = bad || kept > a.max_blocks || want > a.max_blocks;
     r.want = r.over ? r.kept : (int)want;
@@ -62,7 +65,7 @@ __device__ __forceinline__ StepRow step_row(const StepBlocksArgs& a, int w) {
 }
 
 // grid = one cluster
-__global__ void __launch_bounds__(kBlocksThreads) step_blocks_kernel(const __grid_constant__ StepBlocksArgs a) {
+__global__ void __launch_bounds__(kBlocksThreads, 1) step_blocks_kernel(const __grid_constant__ StepBlocksArgs a) {
     const int rank = cluster_ctarank(), ctas = cluster_nctarank(), tid = threadIdx.x;
     const int64_t gtid = (int64_t)rank * kBlocksThreads + tid, gthreads = (int64_t)ctas * kBlocksThreads;
     int* const rows_ws = a.ws + kStepHead;
@@ -83,18 +86,30 @@ __global__ void __launch_bounds__(kBlocksThreads) step_blocks_kernel(const __gri
             const int p = a.table_in[i];
             if (p >= 0 && p < a.num_blocks) atomicAdd(a.refs_out + p, -1);
         }
-    for (int64_t i = gtid; i < (int64_t)a.rows_out * a.max_blocks; i += gthreads) {
-        const int w = (int)floor_div(i, a.max_blocks), c = (int)(i - (int64_t)w * a.max_blocks);
+    // (a warp takes 128 entries of a row at a time: what the row is, once for all of them)
+    const int pieces = (a.max_blocks + 127) / 128;
+    for (int64_t i = gtid >> 5; i < (int64_t)a.rows_out * pieces; i += gthreads >> 5) {
+        const int w = (int)floor_div(i, pieces), c0 = (int)(i - (int64_t)w * pieces) * 128 + (tid & 31);
+        const int64_t row = (int64_t)w * a.max_blocks;
+        const int from = a.source ? a.source[w] : w;
+        int p[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            p[k] = from >= 0 && from < a.rows_in && c0 + 32 * k < a.max_blocks ? a.table_in[(int64_t)from * a.max_blocks + c0 + 32 * k] : -1;
         const StepRow r = step_row(a, w);
-        int p = r.from >= 0 ? a.table_in[(int64_t)r.from * a.max_blocks + c] : -1;
-        const bool there = p >= 0 && p < a.num_blocks, kept = c < r.kept;
-        if (kept && !there) flags |= STATUS_BAD_BLOCK;
-        if (a.source) {
-            if (kept && there) atomicAdd(a.refs_out + p, 1);
-        } else if (!kept && there) {
-            atomicAdd(a.refs_out + p, -1);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int c = c0 + 32 * k;
+            if (c >= a.max_blocks) break;
+            const bool there = p[k] >= 0 && p[k] < a.num_blocks, kept = c < r.kept;
+            if (kept && !there) flags |= STATUS_BAD_BLOCK;
+            if (a.source) {
+                if (kept && there) atomicAdd(a.refs_out + p[k], 1);
+            } else if (!kept && there) {
+                atomicAdd(a.refs_out + p[k], -1);
+            }
+            a.table_out[row + c] = kept && there ? p[k] : -1;
         }
-        a.table_out[i] = kept && there ? p : -1;
     }
     cluster_sync_all();
 
@@ -203,7 +218,7 @@ __host__ __device__ inline int64_t compact_blocks_ints(int64_t blocks) { return 
 
 // n live pages: the k-th live page at or behind place n (lowest first) goes to the k-th free place in front of it.  No page is both, so
 // the copies can run in any order.
-__global__ void __launch_bounds__(kBlocksThreads) compact_blocks_kernel(const __grid_constant__ CompactBlocksArgs a) {
+__global__ void __launch_bounds__(kBlocksThreads, 1) compact_blocks_kernel(const __grid_constant__ CompactBlocksArgs a) {
     const int rank = cluster_ctarank(), ctas = cluster_nctarank(), tid = threadIdx.x;
     const int64_t gtid = (int64_t)rank * kBlocksThreads + tid, gthreads = (int64_t)ctas * kBlocksThreads;
     int* const pairs = a.ws + kCompactHead;

@@ -21,8 +21,15 @@ bool unit_ok(float u) {
     return u > 0.f && std::isfinite(u) && std::frexp(u, &e) == 0.5f && e >= -63 && e <= 65;
 }
 
+FastDiv fast_div_by(uint32_t d) {
+    uint32_t shift = 0;
+    while (shift < 32 && ((uint64_t)1 << shift) < d) ++shift;
+    return {(uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1), shift, d};
+}
+
 int cache_shape(int Hkv, int E, int Ev, int block_size, int max_blocks, int num_blocks, int dtype) {
     if (Hkv <= 0 || E <= 0 || Ev <= 0 || block_size <= 0 || max_blocks <= 0 || num_blocks <= 0) return HOGATT_ERR_BAD_SHAPE;
+    if (Hkv > 65535) return HOGATT_ERR_TOO_LARGE;
     if (dtype != HOGATT_F32 && dtype != HOGATT_F16 && dtype != HOGATT_BF16) return HOGATT_ERR_UNSUPPORTED_DTYPE;
     if (E % kGroup != 0 || Ev % kGroup != 0 || E > 256 || Ev > 256) return HOGATT_ERR_UNSUPPORTED_HEAD_DIM;
     return HOGATT_OK;
@@ -137,12 +144,6 @@ int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
     pl->plan = pl->l + align_up(slots * sizeof(float), 256);
     pl->total = pl->plan + align_up(((size_t)pl->groups_bound + 1) * sizeof(int), 256);
     return HOGATT_OK;
-}
-
-FastDiv fast_div_by(uint32_t d) {
-    uint32_t shift = 0;
-    while (shift < 32 && ((uint64_t)1 << shift) < d) ++shift;
-    return {(uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1), shift, d};
 }
 
 template <class T, int HD, int NT, bool ALIGNED>
@@ -290,6 +291,12 @@ int launch_q4_dense(const hogatt_paged_q4_problem* x, const Q4Plan& pl, int dev,
     return HOGATT_OK;
 }
 
+// (rows x groups, kv heads, sequences), eight CTAs of 256 threads per SM at most
+dim3 rows_grid(int64_t rows, int64_t groups, int Hkv, int B, int sms) {
+    const int64_t z = std::min(B, 65535), per = std::max<int64_t>(1, (int64_t)sms * 8 / (Hkv * z));
+    return dim3((unsigned)std::min((rows * groups + 255) / 256, per), (unsigned)Hkv, (unsigned)z);
+}
+
 // Bookkeeping runs as one cluster; the copies follow on the whole GPU.
 int launch_copies(const hogatt_block_tensors* t, const int* count, const int* pairs, int64_t most, int sms, cudaStream_t stream) {
     for (int first = 0; first < t->count; first += kMaxPageTensors) {
@@ -312,15 +319,20 @@ int launch_copies(const hogatt_block_tensors* t, const int* count, const int* pa
     return HOGATT_OK;
 }
 
+// CTAs of the bookkeeping cluster by what there is to read (pages' counts and table entries): a barrier over several costs more than it
+// saves where one has little to do.  us per call, copies included, with 1 / 2 / 4 / 8: compaction of 512 pages 9.6 / 9.8 / 10.1 / 12.0; a fork of 8 rows
+// into 32, 2,048 pages, 6,000 entries 20.2 / 18.4 / 18.7 / 19.1; 64 rows of 250 entries, 20,480 pages 15.9 / 12.4 / 10.5 / 10.4.
+int cluster_ctas(int64_t cells) { return cells <= 2048 ? 1 : cells <= 8192 ? 2 : cells <= 65536 ? 4 : kBlocksCluster; }
+
 template <class Args>
-cudaError_t launch_cluster(void (*kernel)(Args), cudaStream_t stream, const Args& args) {
+cudaError_t launch_cluster(void (*kernel)(Args), int ctas, cudaStream_t stream, const Args& args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kBlocksCluster);
+    cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kBlocksThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kBlocksCluster;
+    attr[0].val.clusterDim.x = ctas;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -428,7 +440,9 @@ int hogatt_copy_to_blocks_q4_launch(const hogatt_q4_append* p, hogatt_stream_t s
     Q4AppendArgs a;
     memset(&a, 0, sizeof(a));
     a.B = p->B; a.Hkv = p->Hkv; a.S = p->S; a.E = p->E; a.Ev = p->Ev;
-    a.block_size = p->block_size; a.max_blocks = p->max_blocks; a.num_blocks = p->num_blocks;
+    a.max_blocks = p->max_blocks; a.num_blocks = p->num_blocks;
+    a.block = fast_div_by((uint32_t)p->block_size);
+    a.groups = fast_div_by((uint32_t)(std::max(p->E, p->Ev) / kGroup));
     a.packed_tokens = packed ? p->S : 0;
     const int vec = 16 / (int)dtype_size(p->dtype);
     bool vectorised = aligned16(p->keys) && aligned16(p->values);
@@ -444,8 +458,7 @@ int hogatt_copy_to_blocks_q4_launch(const hogatt_q4_append* p, hogatt_stream_t s
     a.table = p->block_table; a.lengths = p->seq_lengths; a.cu = p->cu_seqlens; a.new_rows = p->new_rows; a.status = p->device_status;
     int dev, sms, smem_optin;
     if (const int rc = current_device_info(&dev, &sms, &smem_optin)) return rc;
-    const int64_t total = (packed ? (int64_t)p->S : (int64_t)p->B * p->S) * p->Hkv * ((p->E + p->Ev) / kGroup);
-    const dim3 grid((unsigned)std::min<int64_t>((total + 255) / 256, (int64_t)sms * 8));
+    const dim3 grid = rows_grid(p->S, a.groups.d, p->Hkv, packed ? 1 : p->B, sms);
     cudaError_t err;
     switch (p->dtype) {
         case HOGATT_F32: err = launch_kernel(q4_append_kernel<float>, grid, dim3(256), 0, stream, a, (int)vectorised); break;
@@ -471,7 +484,9 @@ int hogatt_copy_from_blocks_q4_launch(const hogatt_q4_read* p, hogatt_stream_t s
     Q4ReadArgs a;
     memset(&a, 0, sizeof(a));
     a.B = p->B; a.Hkv = p->Hkv; a.S = p->S; a.E = p->E; a.Ev = p->Ev;
-    a.block_size = p->block_size; a.max_blocks = p->max_blocks; a.num_blocks = p->num_blocks;
+    a.max_blocks = p->max_blocks; a.num_blocks = p->num_blocks;
+    a.block = fast_div_by((uint32_t)p->block_size);
+    a.groups = fast_div_by((uint32_t)(std::max(p->E, p->Ev) / kGroup));
     a.key_unit = p->key_unit; a.value_unit = p->value_unit;
     a.k = p->keys; a.v = p->values;
     a.codes[0] = static_cast<const unsigned char*>(p->key_cache); a.codes[1] = static_cast<const unsigned char*>(p->value_cache);
@@ -479,8 +494,7 @@ int hogatt_copy_from_blocks_q4_launch(const hogatt_q4_read* p, hogatt_stream_t s
     a.table = p->block_table; a.first = p->first_rows; a.status = p->device_status;
     int dev, sms, smem_optin;
     if (const int rc = current_device_info(&dev, &sms, &smem_optin)) return rc;
-    const int64_t total = (int64_t)p->B * p->S * p->Hkv * ((p->E + p->Ev) / kGroup);
-    const dim3 grid((unsigned)std::min<int64_t>((total + 255) / 256, (int64_t)sms * 8));
+    const dim3 grid = rows_grid(p->S, a.groups.d, p->Hkv, p->B, sms);
     cudaError_t err;
     switch (p->dtype) {
         case HOGATT_F32: err = launch_kernel(q4_read_kernel<float>, grid, dim3(256), 0, stream, a); break;
@@ -516,7 +530,7 @@ int hogatt_step_blocks_launch(const hogatt_step_blocks* p, hogatt_stream_t strea
     a.refs_out = p->refs_out; a.table_out = p->table_out; a.lengths_out = p->lengths_out; a.room = p->room;
     a.ws = static_cast<int*>(p->workspace);
     a.status = p->device_status;
-    HOGATT_CUDA_OK(launch_cluster(step_blocks_kernel, stream, a));
+    HOGATT_CUDA_OK(launch_cluster(step_blocks_kernel, cluster_ctas(p->num_blocks + (int64_t)p->rows_out * p->max_blocks), stream, a));
     if (p->new_tokens == nullptr) return HOGATT_OK;                 // (nobody writes: nothing is copied)
     return launch_copies(&p->caches, a.ws, a.ws + step_blocks_pairs(p->rows_out), p->rows_out, sms, stream);
 }
@@ -541,7 +555,7 @@ int hogatt_compact_blocks_launch(const hogatt_compact_blocks* p, hogatt_stream_t
     a.refs_in = p->refs_in; a.table_in = p->table_in; a.refs_out = p->refs_out; a.table_out = p->table_out; a.moved = p->moved;
     a.ws = static_cast<int*>(p->workspace);
     a.status = p->device_status;
-    HOGATT_CUDA_OK(launch_cluster(compact_blocks_kernel, stream, a));
+    HOGATT_CUDA_OK(launch_cluster(compact_blocks_kernel, cluster_ctas(p->num_blocks + p->table_entries), stream, a));
     return launch_copies(&p->caches, a.ws, a.ws + kCompactHead, p->num_blocks / 2 + 1, sms, stream);
 }
 

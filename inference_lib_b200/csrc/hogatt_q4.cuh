@@ -61,7 +61,20 @@ __device__ __forceinline__ float from_e4m3(uint32_t byte) {
 __device__ __forceinline__ bool is_nan_e4m3(uint32_t byte) { return (byte & 0x7fu) == 0x7fu; }
 __device__ __forceinline__ float2 half2_of(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 
+// n / d for 0 <= n < 2^31
+struct FastDiv {
+    uint32_t mul, shift, d;
+};
+__device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv& f) { return (__umulhi(n, f.mul) + n) >> f.shift; }
+
 // Row `pos` of a sequence in the cache (rows of all pages and heads are numbered through), or -1: no page there.
+__device__ __forceinline__ long long paged_row_at(const int* table, int pos, const FastDiv& block, int max_blocks, int num_blocks, int Hkv, int h) {
+    const int at = (int)fast_div((uint32_t)pos, block);
+    if (pos < 0 || at >= max_blocks) return -1;
+    const int page = table[at];
+    if (page < 0 || page >= num_blocks) return -1;
+    return ((long long)page * Hkv + h) * block.d + (pos - at * (int)block.d);
+}
 __device__ __forceinline__ long long paged_row_at(const int* table, int pos, int block_size, int max_blocks, int num_blocks, int Hkv, int h) {
     const int at = pos / block_size;
     if (pos < 0 || at >= max_blocks) return -1;
@@ -97,8 +110,9 @@ __device__ __forceinline__ int block_exclusive(int x, int* total) {
     return inc - x + (warp ? warp_sum[warp - 1] : 0);
 }
 struct Q4AppendArgs {
-    int B, Hkv, S, E, Ev, block_size, max_blocks, num_blocks;
+    int B, Hkv, S, E, Ev, max_blocks, num_blocks;
     int packed_tokens;            // packed layout: rows of the source; fixed layout: 0
+    FastDiv block, groups;        // block size; max(E, Ev) / 16
     long long ks[3], vs[3];       // element strides of (sequence, kv head, token)
     float key_unit, value_unit;
     const void* k;
@@ -140,60 +154,73 @@ __device__ __forceinline__ void load_group(const T* src, bool vectorised, float 
     }
 }
 
+// A group's scale and codes.  x / step is the correctly rounded quotient, from a correctly rounded reciprocal r of the step and one
+// correction, q + (x - q step) r (Markstein, IBM J. Res. Dev. 34, 1990).  It stays below 10 unless the scale is the largest; then a first
+// quotient beyond 8 is taken for 8, so that nothing overflows into a NaN, and its correction only takes it further out.  A group
+// whose scale is zero or not a number has codes of zero.  (A division per channel: 12,000 rows of 4 groups 9.3 us.)
+__device__ __forceinline__ void quantise_group(const float (&x)[kGroup], float unit, uint32_t (&code)[2], uint32_t* scale) {
+    uint32_t top = 0;                                     // largest magnitude, as bits: NaN > infinity > every number
+#pragma unroll
+    for (int e = 0; e < kGroup; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    *scale = top >= 0x7f800000u ? 0x7fu : to_e4m3(__fdiv_rn(__uint_as_float(top), 6.f * unit));
+    const float step = from_e4m3(*scale) * unit, r = __fdiv_rn(1.f, step);
+    float q[kGroup];
+#pragma unroll
+    for (int e = 0; e < kGroup; ++e) q[e] = x[e] * r;
+    if (*scale == 0x7eu) {
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e) q[e] = fminf(fmaxf(q[e], -8.f), 8.f);
+    }
+#pragma unroll
+    for (int e = 0; e < kGroup; ++e) q[e] = fmaf(fmaf(q[e], -step, x[e]), r, q[e]);
+    code[0] = code[1] = 0u;
+#pragma unroll
+    for (int e = 0; e < kGroup; e += 2) code[e / 8] |= to_e2m1x2(q[e], q[e + 1]) << (e % 8 * 4);
+    if (!(step > 0.f)) code[0] = code[1] = 0u;
+}
+
+// A thread: one group of a key row and of the value row beside it.  grid: (groups of rows, kv heads, sequences), packed layout one "sequence".
 template <class T>
 __global__ void __launch_bounds__(256) q4_append_kernel(const __grid_constant__ Q4AppendArgs a, const int vectorised) {
-    const int gk = a.E / kGroup, gv = a.Ev / kGroup, per_row = gk + gv;
-    const int64_t rows = (int64_t)(a.cu ? a.packed_tokens : a.B * (int64_t)a.S) * a.Hkv;
-    const int64_t total = rows * per_row;
+    const int gk = a.E / kGroup, gv = a.Ev / kGroup, h = blockIdx.y;
     pdl_wait();
     pdl_trigger();
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t row = floor_div(i, per_row);
-        const int c = (int)(i - row * per_row);
-        const int64_t tok = floor_div(row, a.Hkv);
-        const int h = (int)(row - tok * a.Hkv);
-        int b, t;
-        if (a.cu) {
-            b = packed_sequence(a.cu, a.B, (int)tok);
-            if (b < 0) continue;
-            t = (int)tok - a.cu[b];
-        } else {
-            b = (int)floor_div(tok, a.S);
-            t = (int)(tok - (int64_t)b * a.S);
-        }
-        const bool value = c >= gk;
-        const int g = value ? c - gk : c;
-        const long long* st = value ? a.vs : a.ks;
-        const T* src = static_cast<const T*>(value ? a.v : a.k) + (a.cu ? tok : (int64_t)t) * st[2] + (a.cu ? 0 : b * st[0]) + h * st[1] + g * kGroup;
-        float x[kGroup];
-        load_group<T>(src, vectorised, x);
-        if (a.new_rows && t >= a.new_rows[b]) continue;
-        const long long dst = paged_row_at(a.table + (size_t)b * a.max_blocks, a.lengths[b] + t, a.block_size, a.max_blocks, a.num_blocks, a.Hkv, h);
-        if (dst < 0) {
-            if (a.status && c == 0) atomicOr(a.status, STATUS_BAD_BLOCK);
-            continue;
-        }
-        uint32_t top = 0;                                 // largest magnitude, as bits: NaN > infinity > every number
+    for (int z = blockIdx.z; z < (a.cu ? 1 : a.B); z += gridDim.z) {
+        const int rows = a.cu ? a.packed_tokens : a.S;
+        for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (int64_t)rows * a.groups.d; i += (int64_t)gridDim.x * blockDim.x) {
+            const int row = i < INT_MAX ? (int)fast_div((uint32_t)i, a.groups) : (int)(i / a.groups.d), g = (int)(i - (int64_t)row * a.groups.d);
+            // both rows' loads first: where they go takes two more round trips
+            float x[2][kGroup];
+            if (g < gk) load_group<T>(static_cast<const T*>(a.k) + z * a.ks[0] + h * a.ks[1] + row * a.ks[2] + g * kGroup, vectorised, x[0]);
+            if (g < gv) load_group<T>(static_cast<const T*>(a.v) + z * a.vs[0] + h * a.vs[1] + row * a.vs[2] + g * kGroup, vectorised, x[1]);
+            int b = z, t = row;
+            if (a.cu) {
+                b = packed_sequence(a.cu, a.B, row);
+                if (b < 0) continue;
+                t = row - a.cu[b];
+            }
+            if (a.new_rows && t >= a.new_rows[b]) continue;
+            const long long dst = paged_row_at(a.table + (size_t)b * a.max_blocks, a.lengths[b] + t, a.block, a.max_blocks, a.num_blocks, a.Hkv, h);
+            if (dst < 0) {
+                if (a.status && g == 0) atomicOr(a.status, STATUS_BAD_BLOCK);
+                continue;
+            }
 #pragma unroll
-        for (int e = 0; e < kGroup; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-        const float unit = value ? a.value_unit : a.key_unit;
-        const uint32_t scale = top >= 0x7f800000u ? 0x7fu : to_e4m3(__fdiv_rn(__uint_as_float(top), 6.f * unit));
-        const float step = from_e4m3(scale) * unit;
-        const bool some = step > 0.f;                     // (all smaller than half of the smallest scale, or not a number: zeros)
-        uint32_t code[2] = {0u, 0u};
-#pragma unroll
-        for (int e = 0; e < kGroup; e += 2) {
-            const float lo = some ? __fdiv_rn(x[e], step) : copysignf(0.f, x[e]), hi = some ? __fdiv_rn(x[e + 1], step) : copysignf(0.f, x[e + 1]);
-            code[e / 8] |= to_e2m1x2(lo, hi) << (e % 8 * 4);
+            for (int v = 0; v < 2; ++v) {
+                const int groups = v ? gv : gk;
+                if (g >= groups) continue;
+                uint32_t code[2], scale;
+                quantise_group(x[v], v ? a.value_unit : a.key_unit, code, &scale);
+                *reinterpret_cast<uint2*>(a.codes[v] + ((size_t)dst * groups + g) * (kGroup / 2)) = make_uint2(code[0], code[1]);
+                a.scales[v][(size_t)dst * groups + g] = (unsigned char)scale;
+            }
         }
-        const int groups = value ? gv : gk;
-        *reinterpret_cast<uint2*>(a.codes[value] + ((size_t)dst * groups + g) * (kGroup / 2)) = make_uint2(code[0], code[1]);
-        a.scales[value][(size_t)dst * groups + g] = (unsigned char)scale;
     }
 }
 
 struct Q4ReadArgs {
-    int B, Hkv, S, E, Ev, block_size, max_blocks, num_blocks;
+    int B, Hkv, S, E, Ev, max_blocks, num_blocks;
+    FastDiv block, groups;
     float key_unit, value_unit;
     void* k;                      // [B, Hkv, S, E]
     void* v;
@@ -204,39 +231,50 @@ struct Q4ReadArgs {
     int* status;
 };
 
-// Rows first[b] ... first[b] + S - 1 of every sequence as numbers; a row without a page is NaN.
+// Rows first[b] ... first[b] + S - 1 of every sequence as numbers; a row without a page is NaN.  Threads and grid as above.
 template <class T>
 __global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ Q4ReadArgs a) {
-    const int gk = a.E / kGroup, gv = a.Ev / kGroup, per_row = gk + gv;
-    const int64_t total = (int64_t)a.B * a.Hkv * a.S * per_row;
+    const int gk = a.E / kGroup, gv = a.Ev / kGroup, h = blockIdx.y;
     pdl_wait();
     pdl_trigger();
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t row = floor_div(i, per_row), bh = floor_div(row, a.S);
-        const int c = (int)(i - row * per_row), t = (int)(row - bh * a.S);
-        const int b = (int)floor_div(bh, a.Hkv), h = (int)(bh - (int64_t)b * a.Hkv);
-        const bool value = c >= gk;
-        const int g = value ? c - gk : c, groups = value ? gv : gk;
-        const long long src = paged_row_at(a.table + (size_t)b * a.max_blocks, a.first[b] + t, a.block_size, a.max_blocks, a.num_blocks, a.Hkv, h);
-        uint2 code = make_uint2(0u, 0u);
-        uint32_t scale = 0x7fu;
-        if (src >= 0) {
-            code = *reinterpret_cast<const uint2*>(a.codes[value] + ((size_t)src * groups + g) * (kGroup / 2));
-            scale = a.scales[value][(size_t)src * groups + g];
-        } else if (a.status && c == 0) {
-            atomicOr(a.status, STATUS_BAD_BLOCK);
-        }
-        const float step = from_e4m3(scale) * (value ? a.value_unit : a.key_unit);
-        T* dst = static_cast<T*>(value ? a.v : a.k) + ((size_t)row * groups + g) * kGroup;
-        __align__(16) T out[kGroup];
+    for (int b = blockIdx.z; b < a.B; b += gridDim.z) {
+        const int first = a.first[b];
+        for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (int64_t)a.S * a.groups.d; i += (int64_t)gridDim.x * blockDim.x) {
+            const int t = i < INT_MAX ? (int)fast_div((uint32_t)i, a.groups) : (int)(i / a.groups.d), g = (int)(i - (int64_t)t * a.groups.d);
+            const long long src = paged_row_at(a.table + (size_t)b * a.max_blocks, first + t, a.block, a.max_blocks, a.num_blocks, a.Hkv, h);
+            if (src < 0 && a.status && g == 0) atomicOr(a.status, STATUS_BAD_BLOCK);
+            const size_t row = ((size_t)b * a.Hkv + h) * a.S + t;
+            uint2 code[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+            uint32_t scale[2] = {0x7fu, 0x7fu};
 #pragma unroll
-        for (int e = 0; e < kGroup; e += 2) {
-            const float2 x = half2_of(from_e2m1x2((e < 8 ? code.x : code.y) >> (e % 8 * 4)));
-            out[e] = Scalar<T>::from_float(x.x * step);
-            out[e + 1] = Scalar<T>::from_float(x.y * step);
-        }
+            for (int v = 0; v < 2; ++v)
+                if (src >= 0 && g < (v ? gv : gk)) {
+                    const size_t at = (size_t)src * (v ? gv : gk) + g;
+                    code[v] = *reinterpret_cast<const uint2*>(a.codes[v] + at * (kGroup / 2));
+                    scale[v] = a.scales[v][at];
+                }
 #pragma unroll
-        for (int k = 0; k < (int)(kGroup * sizeof(T) / 16); ++k) reinterpret_cast<uint4*>(dst)[k] = reinterpret_cast<const uint4*>(out)[k];
+            for (int v = 0; v < 2; ++v) {
+                const int groups = v ? gv : gk;
+                if (g >= groups) continue;
+                const float step = from_e4m3(scale[v]) * (v ? a.value_unit : a.key_unit);
+                __align__(16) T out[kGroup];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t x[4];
+                    from_e2m1x8(e ? code[v].y : code[v].x, x);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 y = half2_of(x[k]);
+                        out[e * 8 + 2 * k] = Scalar<T>::from_float(y.x * step);
+                        out[e * 8 + 2 * k + 1] = Scalar<T>::from_float(y.y * step);
+                    }
+                }
+                uint4* const dst = reinterpret_cast<uint4*>(static_cast<T*>(v ? a.v : a.k) + (row * groups + g) * kGroup);
+#pragma unroll
+                for (int k = 0; k < (int)(kGroup * sizeof(T) / 16); ++k) dst[k] = reinterpret_cast<const uint4*>(out)[k];
+            }
+        }
     }
 }
 

@@ -31,12 +31,6 @@ namespace hogatt {
 
 constexpr int kQ4Warps = 8, kQ4Threads = kQ4Warps * 32, kQ4Tile = kQ4Warps * 16, kQ4Ctas = 2;
 
-// n / d for 0 <= n < 2^31
-struct FastDiv {
-    uint32_t mul, shift, d;
-};
-__device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv& f) { return (__umulhi(n, f.mul) + n) >> f.shift; }
-
 struct Q4MmaArgs {
     PagedArgs p;                  // kcache / vcache: the codes; splits: unused; groups_bound: entries of the prefix
     const unsigned char* kscale;

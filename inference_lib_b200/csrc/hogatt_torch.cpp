@@ -7,7 +7,9 @@
 // call into the C ABI on the current stream of the tensors' device.
 #include <ATen/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
 #include <Python.h>
+#include <c10/core/Allocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/util/SmallVector.h>
@@ -15,6 +17,7 @@
 
 #include <algorithm>
 #include <optional>
+#include <tuple>
 #include <vector>
 
 #include "../../include/hogatt.h"
@@ -492,6 +495,10 @@ const int32_t* int_vector(const char* what, const char* name, const std::optiona
     return t.has_value() ? int_vector(what, name, *t, n, device) : nullptr;
 }
 
+// Scratch memory for one call, from torch's caching allocator on the current stream (without a tensor around it, which costs the host more
+// than the memory).
+c10::DataPtr scratch(size_t bytes) { return c10::GetAllocator(c10::kCUDA)->allocate(bytes); }
+
 void run_paged_q4(const char* what, at::Tensor& out, double scale, const at::Tensor& locations, const at::Tensor& queries,
                   const at::Tensor& fragment_lengths, const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& key_scales,
                   const at::Tensor& value_scales, const at::Tensor& block_table, const at::Tensor* cu_seqlens_q, double key_unit,
@@ -556,8 +563,8 @@ void run_paged_q4(const char* what, at::Tensor& out, double scale, const at::Ten
     const size_t need = hogatt_paged_q4_workspace_bytes(&x);
     TORCH_CHECK(need > 0, what, ": unsupported problem (head sizes ", p.E, "/", p.Ev, ", Hq ", p.Hq, ", Hkv ", p.Hkv, ", ", c.num_blocks, " blocks of ",
                 c.block_size, ")");
-    at::Tensor workspace = at::empty({(int64_t)need}, out.options().dtype(at::kByte));
-    p.workspace = workspace.data_ptr();
+    const c10::DataPtr workspace = scratch(need);
+    p.workspace = workspace.get();
     p.workspace_bytes = need;
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream();
     check_status(hogatt_paged_q4_sdpa_launch(&x, reinterpret_cast<hogatt_stream_t>(stream)), what);
@@ -577,6 +584,29 @@ void hogwild_varlen_paged_attention_q4(at::Tensor& out, double scale, const at::
                                        const at::Tensor& cu_seqlens_q, double key_unit, double value_unit, const std::optional<at::Tensor>& status) {
     run_paged_q4("hogwild_varlen_paged_sdpa_q4", out, scale, locations, queries, fragment_lengths, key_cache, value_cache, key_scales, value_scales,
                  block_table, &cu_seqlens_q, key_unit, value_unit, status);
+}
+
+// The same into a new tensor: made here, an output costs the host less than through Python.
+at::Tensor hogwild_paged_attention_q4_new(double scale, const at::Tensor& locations, const at::Tensor& queries, const at::Tensor& fragment_lengths,
+                                          const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& key_scales,
+                                          const at::Tensor& value_scales, const at::Tensor& block_table, double key_unit, double value_unit,
+                                          const std::optional<at::Tensor>& status) {
+    TORCH_CHECK(queries.dim() == 5 && value_cache.dim() == 4, "hogwild_paged_sdpa_q4: queries [F,W,Hq,S,E], caches [NumBlocks,Hkv,bs,E/2]");
+    at::Tensor out = at::empty({queries.size(1), queries.size(2), queries.size(3), 2 * value_cache.size(3)}, queries.options());
+    hogwild_paged_attention_q4(out, scale, locations, queries, fragment_lengths, key_cache, value_cache, key_scales, value_scales, block_table, key_unit,
+                               value_unit, status);
+    return out;
+}
+
+at::Tensor hogwild_varlen_paged_attention_q4_new(double scale, const at::Tensor& locations, const at::Tensor& queries, const at::Tensor& fragment_lengths,
+                                                 const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& key_scales,
+                                                 const at::Tensor& value_scales, const at::Tensor& block_table, const at::Tensor& cu_seqlens_q,
+                                                 double key_unit, double value_unit, const std::optional<at::Tensor>& status) {
+    TORCH_CHECK(queries.dim() == 4 && value_cache.dim() == 4, "hogwild_varlen_paged_sdpa_q4: queries [F,total_q,Hq,E], caches [NumBlocks,Hkv,bs,E/2]");
+    at::Tensor out = at::empty({queries.size(1), queries.size(2), 2 * value_cache.size(3)}, queries.options());
+    hogwild_varlen_paged_attention_q4(out, scale, locations, queries, fragment_lengths, key_cache, value_cache, key_scales, value_scales, block_table,
+                                      cu_seqlens_q, key_unit, value_unit, status);
+    return out;
 }
 
 void copy_to_blocks_q4(const at::Tensor& key_states, const at::Tensor& value_states, at::Tensor& key_cache, at::Tensor& value_cache,
@@ -662,6 +692,19 @@ void copy_from_blocks_q4(at::Tensor& keys, at::Tensor& values, const at::Tensor&
     check_status(hogatt_copy_from_blocks_q4_launch(&p, reinterpret_cast<hogatt_stream_t>(stream)), what);
 }
 
+std::tuple<at::Tensor, at::Tensor> copy_from_blocks_q4_new(const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& key_scales,
+                                                            const at::Tensor& value_scales, const at::Tensor& block_table, const at::Tensor& first_rows,
+                                                            int64_t rows, at::ScalarType dtype, double key_unit, double value_unit,
+                                                            const std::optional<at::Tensor>& status) {
+    TORCH_CHECK(key_cache.dim() == 4 && value_cache.dim() == 4 && block_table.dim() == 2 && rows >= 0,
+                "copy_from_blocks_q4: caches [NumBlocks,Hkv,bs,E/2], block_table [B,max_blocks], rows not negative");
+    const at::TensorOptions like = key_cache.options().dtype(dtype);
+    at::Tensor keys = at::empty({block_table.size(0), key_cache.size(1), rows, 2 * key_cache.size(3)}, like);
+    at::Tensor values = at::empty({block_table.size(0), key_cache.size(1), rows, 2 * value_cache.size(3)}, like);
+    copy_from_blocks_q4(keys, values, key_cache, value_cache, key_scales, value_scales, block_table, first_rows, key_unit, value_unit, status);
+    return {keys, values};
+}
+
 struct BlockTensors {
     c10::SmallVector<void*, 64> data;
     c10::SmallVector<int64_t, 64> bytes;
@@ -714,8 +757,8 @@ void step_blocks(const at::Tensor& block_refs, const at::Tensor& block_table, co
     p.device_status = status_word(what, status, device);
     const size_t need = hogatt_step_blocks_workspace_bytes((int32_t)rows_out);
     TORCH_CHECK(need > 0, what, ": no rows");
-    at::Tensor workspace = at::empty({(int64_t)need}, block_refs.options().dtype(at::kByte));
-    p.workspace = workspace.data_ptr();
+    const c10::DataPtr workspace = scratch(need);
+    p.workspace = workspace.get();
     p.workspace_bytes = need;
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream();
     check_status(hogatt_step_blocks_launch(&p, reinterpret_cast<hogatt_stream_t>(stream)), what);
@@ -744,11 +787,32 @@ void compact_blocks(const at::Tensor& block_refs, const at::Tensor& block_table,
     p.device_status = status_word(what, status, device);
     const size_t need = hogatt_compact_blocks_workspace_bytes(p.num_blocks);
     TORCH_CHECK(need > 0, what, ": no blocks");
-    at::Tensor workspace = at::empty({(int64_t)need}, block_refs.options().dtype(at::kByte));
-    p.workspace = workspace.data_ptr();
+    const c10::DataPtr workspace = scratch(need);
+    p.workspace = workspace.get();
     p.workspace_bytes = need;
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream();
     check_status(hogatt_compact_blocks_launch(&p, reinterpret_cast<hogatt_stream_t>(stream)), what);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> step_blocks_new(const at::Tensor& block_refs, const at::Tensor& block_table,
+                                                                            const at::Tensor& seq_lengths, const std::optional<at::Tensor>& source,
+                                                                            const std::optional<at::Tensor>& new_tokens, int64_t block_size,
+                                                                            at::TensorList caches, const std::optional<at::Tensor>& status) {
+    TORCH_CHECK(block_table.dim() == 2 && (!source.has_value() || source->dim() == 1), "step_blocks: block_table [W,max_blocks], source [W']");
+    const int64_t rows = source.has_value() ? source->size(0) : block_table.size(0);
+    const at::TensorOptions like = block_refs.options().dtype(at::kInt);
+    at::Tensor refs = at::empty(block_refs.sizes(), like), table = at::empty({rows, block_table.size(1)}, like), lengths = at::empty({rows}, like),
+               room = at::empty({rows}, like);
+    step_blocks(block_refs, block_table, seq_lengths, source, new_tokens, block_size, caches, refs, table, lengths, room, status);
+    return {refs, table, lengths, room};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> compact_blocks_new(const at::Tensor& block_refs, const at::Tensor& block_table, at::TensorList caches,
+                                                                   const std::optional<at::Tensor>& status) {
+    const at::TensorOptions like = block_refs.options().dtype(at::kInt);
+    at::Tensor refs = at::empty(block_refs.sizes(), like), table = at::empty(block_table.sizes(), like), moved = at::empty(block_refs.sizes(), like);
+    compact_blocks(block_refs, block_table, caches, refs, table, moved, status);
+    return {refs, table, moved};
 }
 
 }  // namespace
@@ -798,6 +862,20 @@ TORCH_LIBRARY(libhogatt, m) {
           "float value_unit, Tensor(e!)? status) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
     m.def("copy_from_blocks_q4(Tensor(a!) keys, Tensor(b!) values, Tensor key_cache, Tensor value_cache, Tensor key_scales, Tensor value_scales, "
           "Tensor block_table, Tensor first_rows, float key_unit, float value_unit, Tensor(c!)? status) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
+    // (into new tensors)
+    m.def("hogwild_paged_sdpa_q4.new(float scale, Tensor locations, Tensor queries, Tensor fragment_lengths, Tensor key_cache, Tensor value_cache, "
+          "Tensor key_scales, Tensor value_scales, Tensor block_table, float key_unit, float value_unit, Tensor(a!)? status) -> Tensor",
+          tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("hogwild_varlen_paged_sdpa_q4.new(float scale, Tensor locations, Tensor queries, Tensor fragment_lengths, Tensor key_cache, "
+          "Tensor value_cache, Tensor key_scales, Tensor value_scales, Tensor block_table, Tensor cu_seqlens_q, float key_unit, float value_unit, "
+          "Tensor(a!)? status) -> Tensor", tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("copy_from_blocks_q4.new(Tensor key_cache, Tensor value_cache, Tensor key_scales, Tensor value_scales, Tensor block_table, "
+          "Tensor first_rows, int rows, ScalarType dtype, float key_unit, float value_unit, Tensor(a!)? status) -> (Tensor, Tensor)",
+          tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("step_blocks.new(Tensor block_refs, Tensor block_table, Tensor seq_lengths, Tensor? source, Tensor? new_tokens, int block_size, "
+          "Tensor(a!)[] caches, Tensor(b!)? status) -> (Tensor, Tensor, Tensor, Tensor)", tags, torch::_RegisterOrVerify::REGISTER);
+    m.def("compact_blocks.new(Tensor block_refs, Tensor block_table, Tensor(a!)[] caches, Tensor(b!)? status) -> (Tensor, Tensor, Tensor)",
+          tags, torch::_RegisterOrVerify::REGISTER);
     // ... and the pages of a paged cache of any type
     m.def("step_blocks(Tensor block_refs, Tensor block_table, Tensor seq_lengths, Tensor? source, Tensor? new_tokens, int block_size, "
           "Tensor(a!)[] caches, Tensor(b!) refs_out, Tensor(c!) table_out, Tensor(d!) lengths_out, Tensor(e!) room, Tensor(f!)? status) -> ()",
@@ -821,5 +899,10 @@ TORCH_LIBRARY_IMPL(libhogatt, CUDA, m) {
     m.impl("copy_to_blocks_q4", copy_to_blocks_q4);
     m.impl("copy_from_blocks_q4", copy_from_blocks_q4);
     m.impl("step_blocks", step_blocks);
+    m.impl("hogwild_paged_sdpa_q4.new", hogwild_paged_attention_q4_new);
+    m.impl("hogwild_varlen_paged_sdpa_q4.new", hogwild_varlen_paged_attention_q4_new);
+    m.impl("copy_from_blocks_q4.new", copy_from_blocks_q4_new);
+    m.impl("step_blocks.new", step_blocks_new);
+    m.impl("compact_blocks.new", compact_blocks_new);
     m.impl("compact_blocks", compact_blocks);
 }

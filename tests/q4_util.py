@@ -29,7 +29,7 @@ def quantise(x: torch.Tensor, unit: float):
     scale = np.where(ok, E4M3[_nearest(E4M3_VALUE, np.where(ok, top, 0) / 6 / unit)], 127).astype(np.uint8)
     step = np.where(ok, E4M3_VALUE[np.minimum(scale, 126)], 0)[..., None] * unit
     y = np.where(step > 0, np.abs(np.where(ok[..., None], g, 0)) / np.where(step > 0, step, 1), 0)
-    code = (_nearest(E2M1, y) + 8 * np.signbit(g)).astype(np.uint8).reshape(x.shape)
+    code = np.where(step > 0, _nearest(E2M1, y) + 8 * (g < 0), 0).astype(np.uint8).reshape(x.shape)      # (zeros are positive)
     return torch.from_numpy(code[..., 0::2] | code[..., 1::2] << 4), torch.from_numpy(scale)
 
 
