@@ -61,6 +61,7 @@ struct Q4Plan {
     int tokens_per_group, head_blocks, groups_bound, units, splits;
     int rows;                       // (MMA) query rows of a unit at most
     int ctas;                       // (MMA) shares of the list of tiles; 0: a CTA per unit
+    bool small;                     // (MMA) CTAs of four warps
     size_t o, m, l, plan, total;
     int tokens, blocks;             // (DENSE) query tokens per tile, blocks per kv head at most
     DenseLayout w;                  // (DENSE) its workspace
@@ -82,9 +83,6 @@ bool dense_wanted(const hogatt_paged_problem* p) {
     return (double)tokens * p->Hq * p->max_blocks_per_seq * p->block_size >= 4.5e6;
 }
 
-// Units beyond this many per resident CTA get a CTA each: the list's shares then hold several units, whose ends (the eight warps' fold, the next
-// unit's first copies) do not overlap inside a CTA, and the merge step is saved.
-constexpr int kQ4UnitsPerCta = 4;
 
 int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
     if (x == nullptr) return HOGATT_ERR_NULL_POINTER;
@@ -131,7 +129,14 @@ int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
     size_t slots;
     if (pl->kernel == HOGATT_KERNEL_MMA) {
         pl->splits = 0;
-        pl->ctas = pl->units > kQ4UnitsPerCta * kQ4Ctas * sms ? 0 : kQ4Ctas * sms;
+        // With at least as many units as resident CTAs each gets one to itself: shares of the list would hold ends of units (the warps' fold, the next
+        // unit's first copies), which do not overlap inside a CTA, and the merge step is saved.  us per call with shares / without, 8 kv heads
+        // of 5 heads: 24 sequences of 6,000 keys 59.8 / 62.4, 37 of them 72.2 / 62.9, 64 of 2,000 keys 61.5 / 43.5.
+        const int64_t likely = (packed ? std::max<int64_t>(p->W, p->total_q_tokens / pl->tokens_per_group) : groups) * pl->head_blocks * p->Hkv;
+        // Four warps: 100 sequences of 700 keys 33.5 / 29.9 (eight / four), 200 of 1,000 keys 79.3 / 56.6, 148 of 200 keys 36.5 / 23.0; 64 of 4,000
+        // keys (512 units) 64.8 / 75.7.
+        pl->ctas = likely >= kQ4Ctas * sms ? 0 : kQ4Ctas * sms;
+        pl->small = likely >= 2 * kQ4Ctas * sms;
         slots = pl->ctas ? ((size_t)pl->units + pl->ctas) * kFmaRows : 0;
     } else {
         pl->ctas = 0;
@@ -146,22 +151,26 @@ int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
     return HOGATT_OK;
 }
 
-template <class T, int HD, int NT, bool ALIGNED>
+template <class T, int HD, int NT, bool ALIGNED, int WARPS>
 int launch_q4_mma(const Q4MmaArgs& x, const Q4Plan& pl, int dev, int smem_optin, cudaStream_t stream) {
     static std::atomic<size_t> granted[kMaxDevices];
-    const size_t smem = q4_mma_smem_bytes<HD>(NT, x.p.W, pl.groups_bound, x.ctas > 0);
+    const size_t smem = q4_mma_smem_bytes<HD, WARPS>(NT, x.p.W, pl.groups_bound, x.ctas > 0);
     if (smem > (size_t)smem_optin) return HOGATT_ERR_TOO_LARGE;
-    const int rc = ensure_smem_limit(q4_mma_kernel<T, HD, NT, ALIGNED>, dev, smem, granted);
+    const int rc = ensure_smem_limit(q4_mma_kernel<T, HD, NT, ALIGNED, WARPS>, dev, smem, granted);
     if (rc != HOGATT_OK) return rc;
-    HOGATT_CUDA_OK(launch_kernel(q4_mma_kernel<T, HD, NT, ALIGNED>, dim3(x.ctas ? x.ctas : pl.units), dim3(kQ4Threads), smem, stream, x));
+    HOGATT_CUDA_OK(launch_kernel(q4_mma_kernel<T, HD, NT, ALIGNED, WARPS>, dim3(x.ctas ? x.ctas : pl.units), dim3(WARPS * 32), smem, stream, x));
     if (x.ctas) HOGATT_CUDA_OK(launch_kernel(q4_mma_merge_kernel<T, HD>, dim3(pl.units, pl.rows), dim3(128), 0, stream, x));
     return HOGATT_OK;
 }
+template <class T, int HD, int NT>
+int launch_q4_mma_blocks(const Q4MmaArgs& x, const Q4Plan& pl, int dev, int smem_optin, cudaStream_t stream) {
+    if (x.p.block_size % 16 == 0)
+        return pl.small ? launch_q4_mma<T, HD, NT, true, 4>(x, pl, dev, smem_optin, stream) : launch_q4_mma<T, HD, NT, true, 8>(x, pl, dev, smem_optin, stream);
+    return pl.small ? launch_q4_mma<T, HD, NT, false, 4>(x, pl, dev, smem_optin, stream) : launch_q4_mma<T, HD, NT, false, 8>(x, pl, dev, smem_optin, stream);
+}
 template <class T, int HD>
 int launch_q4_mma_rows(const Q4MmaArgs& x, const Q4Plan& pl, int dev, int smem_optin, cudaStream_t stream) {
-    const bool aligned = x.p.block_size % 16 == 0;
-    if (pl.rows <= 8) return aligned ? launch_q4_mma<T, HD, 1, true>(x, pl, dev, smem_optin, stream) : launch_q4_mma<T, HD, 1, false>(x, pl, dev, smem_optin, stream);
-    return aligned ? launch_q4_mma<T, HD, 2, true>(x, pl, dev, smem_optin, stream) : launch_q4_mma<T, HD, 2, false>(x, pl, dev, smem_optin, stream);
+    return pl.rows <= 8 ? launch_q4_mma_blocks<T, HD, 1>(x, pl, dev, smem_optin, stream) : launch_q4_mma_blocks<T, HD, 2>(x, pl, dev, smem_optin, stream);
 }
 
 template <class T>

@@ -16,12 +16,12 @@
 // P goes from the accumulators of the first product to the B operand of the second by movmatrix.
 //
 // Every warp works alone: 16 keys of each 128-key tile, fetched by its own cp.async copies into its own ring, its own running maximum and
-// sum; the eight warps meet only where a unit ends.  Rows are looked up in the block table one tile ahead of their copies.  O is
+// sum; the eight (or four) warps meet only where a unit ends.  Rows are looked up in the block table one tile ahead of their copies.  O is
 // rescaled only when some score exceeds the row's reference by 2^7 (P then stays below 128 in fp16).
 //
 // Split: units (<= 16 query rows that share keys, kv head) are cut into 128-key tiles, all units' tiles are one list, every CTA takes an
-// equal contiguous share (two CTAs per SM).  A share's part of a unit is a partial; q4_mma_merge_kernel adds them up.  With many more units than
-// CTAs each unit gets a CTA of its own, and no merge step.
+// equal contiguous share (two CTAs per SM).  A share's part of a unit is a partial; q4_mma_merge_kernel adds them up.  With as many units as
+// CTAs each unit gets a CTA of its own, and no merge step; with more, CTAs of four warps, four per SM, whose starts and ends overlap.
 #pragma once
 #include <float.h>
 
@@ -29,7 +29,7 @@
 
 namespace hogatt {
 
-constexpr int kQ4Warps = 8, kQ4Threads = kQ4Warps * 32, kQ4Tile = kQ4Warps * 16, kQ4Ctas = 2;
+constexpr int kQ4Ctas = 2;       // resident CTAs of eight warps per SM (four of four warps)
 
 struct Q4MmaArgs {
     PagedArgs p;                  // kcache / vcache: the codes; splits: unused; groups_bound: entries of the prefix
@@ -42,23 +42,24 @@ struct Q4MmaArgs {
     int* plan;                    // [groups_bound + 1]: tiles of a kv head's units in front of every group of query tokens
 };
 
-template <int HD>
+template <int HD, int WARPS>
 struct Q4MmaCfg {
+    static constexpr int THREADS = WARPS * 32, TILE = WARPS * 16;  // keys of a tile: 16 a warp
     static constexpr int ROW = HD / 2, SROW = HD / kGroup;         // bytes of a row's codes and scales
     static constexpr int STAGE = 16 * 2 * (ROW + SROW) + 16;       // K, V, K scales, V scales of 16 keys; which have no page
     static constexpr int OFF_V = 16 * ROW, OFF_KS = 32 * ROW, OFF_VS = OFF_KS + 16 * SROW, OFF_BAD = OFF_VS + 16 * SROW;
     static constexpr int NSTAGE = HD == 128 ? 5 : 8;
-    static constexpr int RING = kQ4Warps * NSTAGE * STAGE;
+    static constexpr int RING = WARPS * NSTAGE * STAGE;
     static constexpr int PITCH = HD + 4;                           // floats between rows of the fold
-    static constexpr int fold_bytes(int rows) { return kQ4Warps * rows * (PITCH + 2) * 4; }
+    static constexpr int fold_bytes(int rows) { return WARPS * rows * (PITCH + 2) * 4; }
     static constexpr int ring_bytes(int nt) { return RING > fold_bytes(8 * nt) ? RING : fold_bytes(8 * nt); }
     // sixteen query rows do not fit in registers beside O: their fragments, the same for every warp, lie in shared memory
     static constexpr int q_bytes(int nt) { return nt == 2 ? nt * (HD / 32) * 512 : 0; }
     static constexpr int work_bytes(int nt) { return ring_bytes(nt) + q_bytes(nt); }
 };
-template <int HD>
+template <int HD, int WARPS>
 __host__ __device__ inline size_t q4_mma_smem_bytes(int nt, int W, int groups, bool list) {
-    return Q4MmaCfg<HD>::work_bytes(nt) + (list ? ((size_t)W + 1 + 2 * groups + 1) * sizeof(int) : 0);
+    return Q4MmaCfg<HD, WARPS>::work_bytes(nt) + (list ? ((size_t)W + 1 + 2 * groups + 1) * sizeof(int) : 0);
 }
 
 // the 8x8 matrix of 16-bit elements that the warp holds (row lane / 4, columns 2 (lane % 4) and + 1), transposed
@@ -127,42 +128,56 @@ __device__ __forceinline__ int tokens_of(const PagedArgs& a, int w, int* start) 
     return a.cu_seqlens ? max(0, min(a.cu_seqlens[w + 1], a.total_q) - *start) : a.S;
 }
 
-// Sequence, tokens and heads of unit x, by a whole warp (32 sequences at a time).
+// Sequence, tokens and heads of unit x, by a whole warp: a lane counts the groups of a run of sequences, its loads all under way at once.
 __device__ __forceinline__ bool locate_unit(const PagedArgs& a, int x, PagedUnit* u) {
     const int lane = threadIdx.x & 31;
     u->hkv = x % a.Hkv;
     const int y = x / a.Hkv;
     u->g0 = (y % a.head_blocks) * 16;
     int grp = y / a.head_blocks;
-    for (int w0 = 0; w0 < a.W; w0 += 32) {
-        const int w = w0 + lane;
-        int start = 0;
-        const int n = w < a.W ? tokens_of(a, w, &start) : 0;
-        const int ng = (n + a.tokens_per_group - 1) / a.tokens_per_group;
-        int inc = ng;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int z = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += z;
-        }
-        const unsigned here = __ballot_sync(0xffffffffu, grp < inc);
-        if (here) {
-            const int src = __ffs(here) - 1;
-            grp -= __shfl_sync(0xffffffffu, inc - ng, src);
-            u->w = w0 + src;
-            u->s_base = __shfl_sync(0xffffffffu, start, src);
-            u->s_begin = grp * a.tokens_per_group;
-            u->s_end = min(__shfl_sync(0xffffffffu, n, src), u->s_begin + a.tokens_per_group);
-            return true;
-        }
-        grp -= __shfl_sync(0xffffffffu, inc, 31);
+    if (a.cu_seqlens == nullptr) {
+        const int each = (a.S + a.tokens_per_group - 1) / a.tokens_per_group;
+        u->w = grp / each;
+        u->s_base = 0;
+        u->s_begin = (grp - u->w * each) * a.tokens_per_group;
+        u->s_end = min(a.S, u->s_begin + a.tokens_per_group);
+        return u->w < a.W;
     }
-    return false;
+    const int run = (a.W + 31) / 32, w0 = min(a.W, lane * run), w1 = min(a.W, w0 + run);
+    auto groups_of = [&](int w) {
+        int start;
+        return (tokens_of(a, w, &start) + a.tokens_per_group - 1) / a.tokens_per_group;
+    };
+    int mine = 0;
+#pragma unroll 8
+    for (int w = w0; w < w1; ++w) mine += groups_of(w);
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int z = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += z;
+    }
+    const unsigned here = __ballot_sync(0xffffffffu, grp < inc);
+    if (!here) return false;
+    const int src = __ffs(here) - 1;
+    grp -= __shfl_sync(0xffffffffu, inc - mine, src);
+    int w = w0;
+    if (lane == src)
+        for (int n; grp >= (n = groups_of(w)); ++w) grp -= n;
+    w = __shfl_sync(0xffffffffu, w, src);
+    grp = __shfl_sync(0xffffffffu, grp, src);
+    int start;
+    const int tokens = tokens_of(a, w, &start);
+    u->w = w;
+    u->s_base = start;
+    u->s_begin = grp * a.tokens_per_group;
+    u->s_end = min(tokens, u->s_begin + a.tokens_per_group);
+    return true;
 }
 
-template <class T, int HD, int NT, bool ALIGNED>
-__global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __grid_constant__ Q4MmaArgs x) {
-    using C = Q4MmaCfg<HD>;
+template <class T, int HD, int NT, bool ALIGNED, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel(const __grid_constant__ Q4MmaArgs x) {
+    using C = Q4MmaCfg<HD, WARPS>;
     constexpr int KS = HD / 16;              // steps of S^T = tiles of O^T
     constexpr int CPT = HD / 4, DPT = HD / 8;        // channels of a key, of a value that a thread holds
     const PagedArgs& a = x.p;
@@ -186,7 +201,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
     if (x.ctas) {
         int before = 0;
         if (a.cu_seqlens) {
-            for (int w0 = 0; w0 < a.W; w0 += kQ4Threads) {
+            for (int w0 = 0; w0 < a.W; w0 += C::THREADS) {
                 int start, n = 0, total;
                 if (w0 + tid < a.W) n = (tokens_of(a, w0 + tid, &start) + a.tokens_per_group - 1) / a.tokens_per_group;
                 const int at = before + block_exclusive(n, &total);
@@ -195,14 +210,14 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
             }
         } else {
             const int each = (a.S + a.tokens_per_group - 1) / a.tokens_per_group;
-            for (int w = tid; w < a.W; w += kQ4Threads) first_group[w] = w * each;
+            for (int w = tid; w < a.W; w += C::THREADS) first_group[w] = w * each;
             before = a.W * each;
         }
         groups = min(before, a.groups_bound);
         if (tid == 0) first_group[a.W] = before;
         __syncthreads();
         before = 0;
-        for (int e0 = 0; e0 < groups; e0 += kQ4Threads) {
+        for (int e0 = 0; e0 < groups; e0 += C::THREADS) {
             const int e = e0 + tid;
             int n = 0, total;
             if (e < groups) {
@@ -217,7 +232,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
                 int vis = 0;
                 for (int f = 0; f < a.F; ++f) {
                     vis = group_visible(a, f, lo, start, s0, min(tokens, s0 + a.tokens_per_group));
-                    n += ceil_div(vis, kQ4Tile);
+                    n += ceil_div(vis, C::TILE);
                 }
                 seen[e] = vis;
             }
@@ -228,7 +243,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
         if (tid == 0) pre[groups] = before;
         __syncthreads();
         if (blockIdx.x == 0)
-            for (int e = tid; e <= a.groups_bound; e += kQ4Threads) x.plan[e] = pre[min(e, groups)];
+            for (int e = tid; e <= a.groups_bound; e += C::THREADS) x.plan[e] = pre[min(e, groups)];
         const int64_t N = (int64_t)before * per_group;
         const int shares = effective_ctas(N, x.ctas);     // none of them empty
         if ((int)blockIdx.x >= shares) return;
@@ -293,7 +308,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
         for (int f = 0; f < a.F; ++f) {
             // ---- this fragment's tiles of the share ----
             const int vis = x.ctas && a.F == 1 ? seen[grp] : group_visible(a, f, u.w, u.s_base, u.s_begin, u.s_end);
-            const int tiles = ceil_div(vis, kQ4Tile);
+            const int tiles = ceil_div(vis, C::TILE);
             const int b0 = max(j0, tiles_before) - tiles_before, b1 = min(j1, tiles_before + tiles) - tiles_before;
             whole = whole && (tiles == 0 || (b0 == 0 && b1 == tiles));
             tiles_before += tiles;
@@ -320,12 +335,12 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
             int64_t from[LOOKUPS];
             int looked = b0;                              // ALIGNED: from[0] has tiles `looked` ..., from[1] the 32 behind them
             auto look_up = [&](int j) {
-                const int k0 = j * kQ4Tile + warp * 16;
+                const int k0 = j * C::TILE + warp * 16;
                 if constexpr (ALIGNED) {
                     if (j - looked == 32) {
                         looked = j;
                         from[0] = from[1];
-                        from[1] = row_of(k0 + (32 + lane) * kQ4Tile);
+                        from[1] = row_of(k0 + (32 + lane) * C::TILE);
                     }
                 } else {
 #pragma unroll
@@ -338,7 +353,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
             const unsigned char* const s_lane = scales + srow * C::SROW;
             bool any_bad = false;                         // a tile with keys that have no page has been met: their bits are looked at
             auto fetch = [&](int j, uint32_t base) {      // base: the stage's bytes from the ring's start
-                const int left = vis - (j * kQ4Tile + warp * 16);          // keys there are from here on
+                const int left = vis - (j * C::TILE + warp * 16);          // keys there are from here on
                 const int64_t tile_from = ALIGNED ? __shfl_sync(0xffffffffu, from[0], (j - looked) & 31) : 0;
                 if (ALIGNED && left >= 16 && tile_from >= 0) {
 #pragma unroll
@@ -370,8 +385,8 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
 
             // ---- the walk ----
             if constexpr (ALIGNED) {
-                from[0] = row_of(b0 * kQ4Tile + warp * 16 + lane * kQ4Tile);
-                from[1] = row_of(b0 * kQ4Tile + warp * 16 + (32 + lane) * kQ4Tile);
+                from[0] = row_of(b0 * C::TILE + warp * 16 + lane * C::TILE);
+                from[1] = row_of(b0 * C::TILE + warp * 16 + (32 + lane) * C::TILE);
             } else {
                 look_up(b0);
             }
@@ -466,9 +481,9 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
             const uint32_t va_at = v_of(v0), vb_at = v_of(v1), vs_at = ring_u32 + C::OFF_VS + v0 * C::SROW + (HD == 128 ? g : g >> 1);
             const int vs_step = (v1 - v0) * C::SROW;
             uint32_t base = 0, base_ahead = (C::NSTAGE - 1) * C::STAGE;
-            int k0 = b0 * kQ4Tile + warp * 16;
+            int k0 = b0 * C::TILE + warp * 16;
 #pragma unroll 1
-            for (int j = b0; j < b1; ++j, k0 += kQ4Tile) {
+            for (int j = b0; j < b1; ++j, k0 += C::TILE) {
                 cp_async_wait<C::NSTAGE - 2>();
                 __syncwarp();                             // every lane's copies have landed, and every lane has left the last stage
                 const int ahead = j + C::NSTAGE - 1;
@@ -640,8 +655,8 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
         // ---- the eight warps' results become one ----
         __syncthreads();                                  // (the fold lies on the rings)
         float* const fold = reinterpret_cast<float*>(smem_raw);
-        float* const fold_m = fold + kQ4Warps * 8 * NT * C::PITCH;
-        float* const fold_l = fold_m + kQ4Warps * 8 * NT;
+        float* const fold_m = fold + WARPS * 8 * NT * C::PITCH;
+        float* const fold_l = fold_m + WARPS * 8 * NT;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -660,17 +675,17 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4Ctas) q4_mma_kernel(const __gri
                 }
             }
         __syncthreads();
-        for (int i = tid; i < 8 * NT * (HD / 4); i += kQ4Threads) {
+        for (int i = tid; i < 8 * NT * (HD / 4); i += C::THREADS) {
             const int r = i / (HD / 4), col = (i - r * (HD / 4)) * 4;
             int s_abs, hq;
             if (!paged_row(a, u, r, &s_abs, &hq)) continue;
             float M = -FLT_MAX;
 #pragma unroll
-            for (int w = 0; w < kQ4Warps; ++w) M = fmaxf(M, fold_m[w * 8 * NT + r]);
+            for (int w = 0; w < WARPS; ++w) M = fmaxf(M, fold_m[w * 8 * NT + r]);
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
             float L = 0.f;
 #pragma unroll
-            for (int w = 0; w < kQ4Warps; ++w) {
+            for (int w = 0; w < WARPS; ++w) {
                 const float wgt = exp2_fast(fold_m[w * 8 * NT + r] - M);
                 const float4 v = *reinterpret_cast<const float4*>(fold + (w * 8 * NT + r) * C::PITCH + col);
                 acc.x = fmaf(v.x, wgt, acc.x);

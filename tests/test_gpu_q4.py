@@ -385,6 +385,26 @@ def test_large_and_small_queries(A):
             q4_util.check(got, exact)
 
 
+@pytest.mark.parametrize("dtype,G,E,bs,W", [(torch.bfloat16, 4, 128, 16, 150), (torch.float16, 2, 64, 8, 330), (torch.bfloat16, 12, 128, 12, 150),
+                                            (torch.float16, 3, 64, 24, 80)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_many_short_sequences(A, dtype, G, E, bs, W, packed):
+    """More units than resident CTAs: each has one to itself."""
+    gen, rng = torch.Generator().manual_seed(W), np.random.default_rng(W)
+    Hkv, keys = 4, 70
+    width = -(-keys // bs)
+    (kc, ks), (vc, vs) = (q4_util.random_cache(gen, 2 * width + 9, Hkv, bs, E) for _ in range(2))
+    table = torch.from_numpy(rng.integers(0, 2 * width + 9, (W, width)).astype(np.int32))              # (pages of many rows)
+    q = torch.randn(1, W, Hkv * G, 1, E, generator=gen).to(dtype)
+    loc = torch.from_numpy(rng.integers(-1, keys, (1, W, 1)).astype(np.int32))
+    if packed:
+        got, exact = paged(A, q[:, :, :, 0].contiguous(), loc[:, :, 0], torch.full((1, W), keys, dtype=torch.int32), (kc, vc, ks, vs), table, E ** -0.5,
+                           cu=torch.arange(W + 1, dtype=torch.int32))
+    else:
+        got, exact = paged(A, q, loc, torch.tensor([keys], dtype=torch.int32), (kc, vc, ks, vs), table, E ** -0.5)
+    q4_util.check(got, exact)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.1, 1e-30, 3.0])
 @pytest.mark.parametrize("kernel", KERNELS)
 def test_scales_of_the_scores(A, scale, kernel):
