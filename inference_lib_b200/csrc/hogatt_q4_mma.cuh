@@ -25,6 +25,8 @@
 #pragma once
 #include <float.h>
 
+#include <type_traits>
+
 #include "hogatt_q4.cuh"
 
 namespace hogatt {
@@ -320,19 +322,21 @@ __global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel
             const uint32_t dst0 = ring_u32 + row0 * C::ROW + (HD == 128 ? ((lane % CPR) ^ (row0 & 2)) * 16 : (lane % CPR) * 16);
             const uint32_t sdst0 = ring_u32 + (lane < 16 ? C::OFF_KS : C::OFF_VS) + srow * C::SROW;
             const unsigned char* const scales = lane < 16 ? x.kscale : x.vscale;
-            // Where key `key`'s row of codes begins in either cache, in bytes (its scales: an eighth of that); -1: behind the keys, -2: a
-            // key without a page.
-            auto row_of = [&](int key) -> int64_t {
+            // Where key `key`'s row is in either cache (rows of all pages and heads numbered through; ALIGNED: sixteens of rows, which 32 bits hold
+            // however large the cache); -1: behind the keys, -2: a key without a page.
+            using Row = std::conditional_t<ALIGNED, int, int64_t>;
+            constexpr int PER = ALIGNED ? 16 : 1;
+            auto row_of = [&](int key) -> Row {
                 if (key >= vis) return -1;
                 const int at = (int)fast_div((uint32_t)key, x.block);
                 const int p = at < a.max_blocks ? table[at] : -1;
                 if (p < 0 || p >= x.num_blocks) return -2;
-                return (((int64_t)p * a.Hkv + u.hkv) * a.block_size + (key - at * (int)x.block.d)) * C::ROW;
+                return ((Row)p * a.Hkv + u.hkv) * (a.block_size / PER) + (key - at * (int)x.block.d) / PER;
             };
             // ALIGNED: the 16 keys of a tile lie in one block, and the lanes look up 32 tiles at a time, the next 32 ahead of their use;
             // otherwise every lane looks its rows of the next tile up
             constexpr int LOOKUPS = ALIGNED ? 2 : PASSES + 1;
-            int64_t from[LOOKUPS];
+            Row from[LOOKUPS];
             int looked = b0;                              // ALIGNED: from[0] has tiles `looked` ..., from[1] the 32 behind them
             auto look_up = [&](int j) {
                 const int k0 = j * C::TILE + warp * 16;
@@ -351,30 +355,33 @@ __global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel
             const unsigned char* const k_lane = kc + row0 * C::ROW + lane % CPR * 16;
             const unsigned char* const v_lane = vc + row0 * C::ROW + lane % CPR * 16;
             const unsigned char* const s_lane = scales + srow * C::SROW;
+            const int whole_tiles = (vis - warp * 16) / C::TILE + ((vis - warp * 16) % C::TILE >= 16);        // tiles of which this warp has all 16 keys
             bool any_bad = false;                         // a tile with keys that have no page has been met: their bits are looked at
             auto fetch = [&](int j, uint32_t base) {      // base: the stage's bytes from the ring's start
-                const int left = vis - (j * C::TILE + warp * 16);          // keys there are from here on
-                const int64_t tile_from = ALIGNED ? __shfl_sync(0xffffffffu, from[0], (j - looked) & 31) : 0;
-                if (ALIGNED && left >= 16 && tile_from >= 0) {
+                const Row tile_from = ALIGNED ? __shfl_sync(0xffffffffu, from[0], j - looked) : 0;       // (the lane: modulo 32)
+                if (ALIGNED && j < whole_tiles && tile_from >= 0) {
+                    const unsigned char* const ks = k_lane + (int64_t)tile_from * (16 * C::ROW);
+                    const unsigned char* const vs = v_lane + (int64_t)tile_from * (16 * C::ROW);
 #pragma unroll
                     for (int i = 0; i < PASSES; ++i) {
-                        cp_async_16(dst0 + base + i * RPP * C::ROW, k_lane + tile_from + i * RPP * C::ROW, true);
-                        cp_async_16(dst0 + base + C::OFF_V + i * RPP * C::ROW, v_lane + tile_from + i * RPP * C::ROW, true);
+                        cp_async_16(dst0 + base + i * RPP * C::ROW, ks + i * RPP * C::ROW, true);
+                        cp_async_16(dst0 + base + C::OFF_V + i * RPP * C::ROW, vs + i * RPP * C::ROW, true);
                     }
-                    cp_async_zfill<C::SROW>(sdst0 + base, s_lane + (tile_from >> 3), true);
+                    cp_async_zfill<C::SROW>(sdst0 + base, s_lane + (int64_t)tile_from * (16 * C::SROW), true);
                     if (any_bad && lane == 0) *reinterpret_cast<uint32_t*>(ring + base + C::OFF_BAD) = 0u;
                 } else {                                  // (rows that are not there: zeros, from an address inside the cache)
+                    const int left = vis - (j * C::TILE + warp * 16);      // keys there are from here on
 #pragma unroll
                     for (int i = 0; i < PASSES; ++i) {
-                        const int64_t row = ALIGNED ? tile_from : from[i];
+                        const Row row = ALIGNED ? tile_from : from[i];
                         const bool real = row >= 0 && row0 + i * RPP < left;
-                        const int64_t at = (real ? (ALIGNED ? row + (row0 + i * RPP) * C::ROW : row) : 0) + lane % CPR * 16;
+                        const int64_t at = (real ? (int64_t)row * PER + (ALIGNED ? row0 + i * RPP : 0) : 0) * C::ROW + lane % CPR * 16;
                         cp_async_zfill<16>(dst0 + base + i * RPP * C::ROW, kc + at, real);
                         cp_async_zfill<16>(dst0 + base + C::OFF_V + i * RPP * C::ROW, vc + at, real);
                     }
-                    const int64_t row = ALIGNED ? tile_from : from[LOOKUPS - 1];
+                    const Row row = ALIGNED ? tile_from : from[LOOKUPS - 1];
                     const bool real = row >= 0 && srow < left;
-                    cp_async_zfill<C::SROW>(sdst0 + base, scales + ((real ? (ALIGNED ? row + srow * C::ROW : row) : 0) >> 3), real);
+                    cp_async_zfill<C::SROW>(sdst0 + base, scales + (real ? (int64_t)row * PER + (ALIGNED ? srow : 0) : 0) * C::SROW, real);
                     const uint32_t bad = __ballot_sync(0xffffffffu, row == -2 && srow < left) & 0xffffu;
                     if (bad && lane == 0 && a.status) atomicOr(a.status, STATUS_BAD_BLOCK);
                     any_bad = any_bad || bad != 0;
