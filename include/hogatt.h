@@ -342,7 +342,9 @@ int hogatt_copy_to_blocks_launch(const void* key_states, const void* value_state
 
 /*
  * Attention over such a cache: hogatt_paged_sdpa_launch with key_cache / value_cache as the codes, and num_blocks given.
- * `kernel`: AUTO or FMA (CUDA cores).  f32 / f16 / bf16 queries and outputs; E <= 256, Ev in {32, 64, 128, 256}.
+ * f32 / f16 / bf16 queries and outputs; E <= 256, Ev in {32, 64, 128, 256}.  `kernel`: AUTO; FMA (CUDA cores: all of those); MMA (mma.sync, f16 / bf16 with
+ * E == Ev == 64 or 128: what AUTO takes there); DENSE (tcgen05, packed queries with E == Ev == 128, blocks of a multiple of 8 rows and a scale from 1e-30 to
+ * 1e30: what AUTO takes for prompt chunks).
  */
 typedef struct hogatt_paged_q4_problem {
     hogatt_paged_problem paged;
@@ -359,7 +361,8 @@ int hogatt_paged_q4_sdpa_launch(const hogatt_paged_q4_problem* p, hogatt_stream_
  *   fixed layout  (cu_seqlens == NULL): element (b, h, t, e) of the source at keys + b*ks[0] + h*ks[1] + t*ks[2] + e, t < S
  *   packed layout (cu_seqlens != NULL): S tokens in all, token i at keys + h*ks[1] + i*ks[2]; those of sequence b are
  *                                       cu_seqlens[b] .. cu_seqlens[b + 1] - 1, tokens behind the last sequence stay out
- * new_rows[b] (or NULL): rows t >= new_rows[b] of sequence b stay out.  Two rows for one position: refused by nobody, either is stored.
+ * new_rows[b] (or NULL): rows t >= new_rows[b] of sequence b stay out.  Where two rows go to
+ * one position, what is stored there is not defined.
  */
 typedef struct hogatt_q4_append {
     int32_t B, Hkv, S, E, Ev, block_size, max_blocks, num_blocks, dtype;

@@ -74,6 +74,15 @@ bool dense_disabled() {
     return off;
 }
 
+// HOGATT_PAGED_MMA=0 in the environment keeps AUTO on the CUDA-core paged kernel (A/B measurements).
+bool paged_mma_disabled() {
+    static const bool off = [] {
+        const char* v = getenv("HOGATT_PAGED_MMA");
+        return v && v[0] == '0';
+    }();
+    return off;
+}
+
 namespace {
 
 // HOGATT_HOST_PLAN=0 in the environment (read when the library is first used) makes every call derive its
@@ -989,15 +998,6 @@ struct PagedPlan {
     size_t o, m, l, total;          // the other kernels' workspace
 };
 
-// HOGATT_PAGED_MMA=0 in the environment keeps AUTO on the CUDA-core paged kernel (A/B measurements).
-bool paged_mma_disabled() {
-    static const bool off = [] {
-        const char* v = getenv("HOGATT_PAGED_MMA");
-        return v && v[0] == '0';
-    }();
-    return off;
-}
-
 // Packed queries on the tcgen05 kernel: 16-bit types, head size 128, cache blocks that tile a 128-key tile in whole
 // 8-row swizzle groups (or hold whole tiles), the number of blocks known (a tensor map needs the extent).  AUTO takes it
 // where the prompt chunks of the batch -- the tokens beyond one per sequence, over as many keys as the block table has room
@@ -1080,6 +1080,7 @@ int launch_paged_dense(const hogatt_paged_problem* p, const PagedPlan& pl, int d
     d.status = p->device_status;
     d.out = p->out;
     d.out_scale = 1.f;
+    d.most_keys = INT_MAX;
     DenseMaps maps;
     memset(&maps, 0, sizeof(maps));
     const cuuint64_t qdims[5] = {128, (cuuint64_t)d.G, (cuuint64_t)d.Hkv, (cuuint64_t)d.total_q, (cuuint64_t)d.F};

@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(kBlocksThreads, 1) step_blocks_kernel(const __
     cluster_sync_all();
 
     // ---- 2: what every row needs (CTA 0), free pages of every share ----
+    __shared__ __align__(16) int last_of[kBlocksThreads];
     if (rank == 0) {
         int before = 0;
         for (int w0 = 0; w0 < a.rows_out; w0 += kBlocksThreads) {
@@ -126,14 +127,22 @@ __global__ void __launch_bounds__(kBlocksThreads, 1) step_blocks_kernel(const __
                 if (!r.over && r.add > 0 && r.length % a.block_size != 0) last = __ldcg(a.table_out + (int64_t)w * a.max_blocks + r.kept - 1);
                 __stcg(rows_ws + 3 * w + 1, last);
             }
+            __syncthreads();                              // (the last chunk's have been read)
+            last_of[tid] = last;
             __syncthreads();
             // a last page that is partly filled and shared: its writers take copies in row order while others still hold it
             bool copy = false;
             if (last >= 0) {
                 const int holders = __ldcg(a.refs_out + last);
                 if (holders > 1) {
-                    int earlier = 0;
-                    for (int v = 0; v < w; ++v) earlier += __ldcg(rows_ws + 3 * v + 1) == last;
+                    int earlier = 0, v = 0;
+                    for (; v + 3 < tid; v += 4) {
+                        const int4 x = *reinterpret_cast<const int4*>(last_of + v);
+                        earlier += (x.x == last) + (x.y == last) + (x.z == last) + (x.w == last);
+                    }
+                    for (; v < tid; ++v) earlier += last_of[v] == last;
+#pragma unroll 8
+                    for (v = 0; v < w0; ++v) earlier += __ldcg(rows_ws + 3 * v + 1) == last;
                     copy = holders - earlier > 1;
                 }
             }

@@ -107,6 +107,7 @@ struct DenseArgs {
     const unsigned char* scales[2];
     const float* factor;   // [total_q, Hq]: what a row's products are multiplied with, or nullptr: l2scale for all
     int num_blocks;
+    int most_keys;         // paged: no sequence is taken for longer
     uint32_t block_mul, block_shift;       // key / block_size = (umulhi(key, mul) + key) >> shift
     float out_scale;       // the values' unit (1 elsewhere)
 };
@@ -323,7 +324,7 @@ __device__ __forceinline__ DenseRow dense_row(const DenseArgs& a, int tile, int 
 // rows of fragment f that hold keys and values (worker w's, when paged)
 template <bool PAGED>
 __device__ __forceinline__ int dense_length(const DenseArgs& a, int f, int w) {
-    if constexpr (PAGED) return a.flen[f * a.W + w];
+    if constexpr (PAGED) return min(a.flen[f * a.W + w], a.most_keys);
     return a.flen ? min(a.cap[f], a.flen[f]) : a.cap[f];
 }
 template <bool PAGED>

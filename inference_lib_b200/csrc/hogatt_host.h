@@ -63,6 +63,7 @@ cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
 // elements = 128 bytes.
 int encode_map(CUtensorMap* out, const void* base, int dtype, int rank, const cuuint64_t* dims, const cuuint32_t* box);
 
+bool paged_mma_disabled();  // HOGATT_PAGED_MMA=0: the paged operators stay on the CUDA cores
 bool dense_disabled();      // HOGATT_DENSE=0: AUTO keeps away from the tcgen05 kernels
 
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }

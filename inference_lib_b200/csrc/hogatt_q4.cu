@@ -1,5 +1,7 @@
 // C ABI of the 4-bit paged cache and of page bookkeeping (declared in include/hogatt.h): argument validation, kernel choice, workspace
 // carving and launches, like hogatt_api.cu.
+#include <limits.h>
+
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
@@ -77,7 +79,7 @@ bool dense_eligible(const hogatt_paged_problem* p) {
 // AUTO takes it where the tokens beyond one per sequence, over as many keys as the block table has room for, would keep the other
 // kernel busy for long (as for 16-bit pages).
 bool dense_wanted(const hogatt_paged_problem* p) {
-    if (dense_disabled()) return false;
+    if (dense_disabled() || paged_mma_disabled()) return false;
     const int64_t tokens = (int64_t)p->total_q_tokens - p->W;
     if (tokens * (p->Hq / p->Hkv) < kDenseRows || tokens * p->Hq < 8 * kDenseRows) return false;
     return (double)tokens * p->Hq * p->max_blocks_per_seq * p->block_size >= 4.5e6;
@@ -98,7 +100,7 @@ int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
     if (p->kernel != HOGATT_KERNEL_AUTO && p->kernel != HOGATT_KERNEL_FMA && !(p->kernel == HOGATT_KERNEL_MMA && mma) &&
         !(p->kernel == HOGATT_KERNEL_DENSE && dense))
         return HOGATT_ERR_BAD_KERNEL_CHOICE;
-    pl->kernel = mma && p->kernel != HOGATT_KERNEL_FMA ? HOGATT_KERNEL_MMA : HOGATT_KERNEL_FMA;
+    pl->kernel = mma && (p->kernel == HOGATT_KERNEL_MMA || (p->kernel == HOGATT_KERNEL_AUTO && !paged_mma_disabled())) ? HOGATT_KERNEL_MMA : HOGATT_KERNEL_FMA;
     if (dense && (p->kernel == HOGATT_KERNEL_DENSE || (p->kernel == HOGATT_KERNEL_AUTO && dense_wanted(p)))) pl->kernel = HOGATT_KERNEL_DENSE;
     if (!packed && (int64_t)p->F * p->W * p->S >= ((int64_t)1 << 31)) return HOGATT_ERR_TOO_LARGE;
     if (packed && (int64_t)p->F * std::max(p->total_q_tokens, p->W) >= ((int64_t)1 << 31)) return HOGATT_ERR_TOO_LARGE;
@@ -262,6 +264,7 @@ int launch_q4_dense(const hogatt_paged_q4_problem* x, const Q4Plan& pl, int dev,
     d.scales[0] = static_cast<const unsigned char*>(x->key_scales);
     d.scales[1] = static_cast<const unsigned char*>(x->value_scales);
     d.num_blocks = p->num_blocks;
+    d.most_keys = (int)std::min<int64_t>((int64_t)p->max_blocks_per_seq * p->block_size + 1, INT_MAX - 4096);
     const FastDiv by_block = fast_div_by((uint32_t)p->block_size);
     d.block_mul = by_block.mul;
     d.block_shift = by_block.shift;

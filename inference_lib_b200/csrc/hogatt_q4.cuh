@@ -279,6 +279,13 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ Q4
 }
 
 // ---- attention -----------------------------------------------------------------------------------------------------------
+// Keys that a row at `loc` of a sequence of `len` sees, as far as the kernels walk: the block table's and one more, which says that there are more
+// than it has pages for (a length that is wrong would be a walk over two billion keys).
+__device__ __forceinline__ int most_visible(const PagedArgs& a, int loc, int len) {
+    const int64_t most = min((int64_t)a.max_blocks * a.block_size + 1, (int64_t)INT_MAX - 4096);
+    return (int)min((int64_t)(max(0, min(loc, len - 1) + 1)), most);
+}
+
 struct Q4Args {
     PagedArgs p;                  // kcache / vcache: the codes
     const unsigned char* kscale;
@@ -325,7 +332,7 @@ __global__ void __launch_bounds__(kFmaThreads) q4_attention_kernel(const __grid_
         if (paged_row(a, u, r, &s_abs, &hq)) {
             const int len = a.flen[f * a.len_f + u.w * a.len_w];
             const int loc = a.loc[(size_t)f * a.loc_f + (size_t)u.w * a.loc_w + s_abs];
-            atomicMax(&vis[f], max(0, min(loc, len - 1) + 1));
+            atomicMax(&vis[f], most_visible(a, loc, len));
         }
     }
     __syncthreads();
@@ -362,7 +369,7 @@ __global__ void __launch_bounds__(kFmaThreads) q4_attention_kernel(const __grid_
                 if (paged_row(a, u, tid, &s_abs, &hq)) {
                     const int len = a.flen[f * a.len_f + u.w * a.len_w];
                     const int loc = a.loc[(size_t)f * a.loc_f + (size_t)u.w * a.loc_w + s_abs];
-                    lim = max(0, min(loc, len - 1) + 1);
+                    lim = most_visible(a, loc, len);
                 }
                 core.lim_s[tid] = lim;
             }

@@ -123,7 +123,7 @@ __device__ __forceinline__ void cp_async_zfill(uint32_t dst, const void* src, bo
 __device__ __forceinline__ int group_visible(const PagedArgs& a, int f, int w, int s_base, int s_begin, int s_end) {
     int top = -1;
     for (int s = s_begin; s < s_end; ++s) top = max(top, a.loc[(size_t)f * a.loc_f + (size_t)w * a.loc_w + s_base + s]);
-    return max(0, min(top, a.flen[f * a.len_f + w * a.len_w] - 1) + 1);
+    return most_visible(a, top, a.flen[f * a.len_f + w * a.len_w]);
 }
 __device__ __forceinline__ int tokens_of(const PagedArgs& a, int w, int* start) {
     *start = a.cu_seqlens ? a.cu_seqlens[w] : 0;
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel
                 int mylim = INT_MAX;                      // (a row that is not there is never masked, nor stored)
                 if (real) {
                     const int loc = a.loc[(size_t)f * a.loc_f + (size_t)u.w * a.loc_w + s_abs];
-                    mylim = max(0, min(loc, a.flen[f * a.len_f + u.w * a.len_w] - 1) + 1);
+                    mylim = most_visible(a, loc, a.flen[f * a.len_f + u.w * a.len_w]);
                 }
                 lowest = min(lowest, mylim);
 #pragma unroll

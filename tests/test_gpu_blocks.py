@@ -128,6 +128,14 @@ def test_one_row_and_many(A):
     run_step(A, refs, table, lengths, None, [int(x) for x in rng.integers(0, 9, W)], 8, [torch.arange(30000 * 16, dtype=torch.int32).reshape(30000, 16)])
 
 
+@pytest.mark.parametrize("W", [1, 300, 1025, 2049])
+def test_everybody_forks_from_one(A, W):
+    """One last page that many rows write: all but the last holder take a copy."""
+    rng = np.random.default_rng(W)
+    refs, table = pool(rng, 2 * W + 20, 8, 4, [13, 5])
+    run_step(A, refs, table, [13, 5], [0] * W, [int(x) for x in rng.integers(0, 3, W)], 8, some_caches(rng, 2 * W + 20))
+
+
 def test_more_caches_than_a_launch_takes(A):
     rng = np.random.default_rng(6)
     caches = [torch.from_numpy(rng.integers(0, 99, (24, 5)).astype(np.int32)) for _ in range(150)]

@@ -418,6 +418,89 @@ def test_scales_of_the_scores(A, scale, kernel):
     q4_util.check(got, exact)
 
 
+CALLS = [
+    # packed?, query tokens, W, G, E, bs, keys: shares of a list, units of their own, tcgen05, CUDA cores
+    (False, 1, 2, 4, 128, 16, 700), (False, 1, 90, 8, 64, 8, 60), (True, 140, 2, 4, 128, 16, 300), (False, 2, 1, 2, 32, 16, 90),
+]
+
+
+@pytest.mark.parametrize("case", CALLS, ids=[str(i) for i in range(len(CALLS))])
+def test_graphs_and_streams(A, case):
+    """Append and attention in a graph that is replayed on other contents; the same twice at once on two streams."""
+    packed, tokens, W, G, E, bs, keys = case
+    gen = torch.Generator().manual_seed(keys)
+    Hkv, width = 4, -(-keys // bs) + 1
+    blocks, T = W * width, tokens * W
+    cu = torch.arange(W + 1, dtype=torch.int32, device=DEV) * tokens
+    table = torch.randperm(blocks, generator=gen).to(torch.int32).reshape(W, width).to(DEV)
+
+    def state(seed):
+        g = torch.Generator().manual_seed(seed)
+        (kc, ks), (vc, vs) = (q4_util.random_cache(g, blocks, Hkv, bs, E) for _ in range(2))
+        new = [torch.randn(T, Hkv, E, generator=g).bfloat16() if packed else torch.randn(W, Hkv, tokens, E, generator=g).bfloat16() for _ in range(2)]
+        q = torch.randn((1, T, Hkv * G, E) if packed else (1, W, Hkv * G, tokens, E), generator=g).bfloat16()
+        have = torch.randint(keys // 2, keys - tokens, (W,), generator=g).to(torch.int32)
+        loc = (have[:, None] + torch.arange(tokens)).to(torch.int32)
+        return dev(kc, vc, ks, vs, *new, q, have, (loc.reshape(1, T) if packed else loc[None]).contiguous())
+
+    def call(s):
+        kc, vc, ks, vs, k, v, q, have, loc = s
+        cache = (kc, vc, ks.view(E4M3), vs.view(E4M3), table)
+        A.copy_to_blocks_q4(k, v, *cache, have, cu_seqlens=cu if packed else None)
+        if packed:
+            return A.hogwild_varlen_paged_sdpa_q4(q, loc, *cache, E ** -0.5, (have + tokens)[None], cu)
+        return A.hogwild_paged_sdpa_q4(q, loc, *cache, E ** -0.5, torch.full((1,), keys, dtype=torch.int32, device=DEV))
+
+    wants = [call(state(s)).clone() for s in range(3)]
+    buffers = state(0)
+    call(buffers)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(buffers)
+    for s in (1, 2, 0):
+        for b, x in zip(buffers, state(s)):
+            b.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, wants[s])
+    streams, states, got = [torch.cuda.Stream() for _ in range(2)], [state(1), state(2)], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(call(states[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, wants[i + 1]) for i in range(2) for x in got[i])
+
+
+@pytest.mark.parametrize("kernel,packed", [(None, False), (1, False), (2, False), (None, True), (4, True)])
+def test_lengths_that_are_wrong_end(A, kernel, packed):
+    """A length of two billion: the keys of the table are seen, the others have no page."""
+    gen = torch.Generator().manual_seed(13)
+    cache = [x for pair in zip(*(q4_util.random_cache(gen, 8, 2, 16, 128) for _ in range(2))) for x in pair]
+    table, huge, st = torch.arange(8, dtype=torch.int32).reshape(2, 4), 2 ** 31 - 1, status()
+    q = torch.randn((1, 140, 8, 128) if packed else (1, 2, 8, 1, 128), generator=gen).bfloat16()
+    loc = torch.full((1, 140) if packed else (1, 2, 1), huge, dtype=torch.int32)
+    cu = torch.tensor([0, 139, 140], dtype=torch.int32) if packed else None
+    lens = torch.tensor([[huge, huge]] if packed else [huge], dtype=torch.int32)
+    seen = paged(A, q, torch.clamp(loc, max=63), torch.clamp(lens, max=64), cache, table, 0.1, cu=cu)[0]
+    dc = dev(*cache)
+    args = (*dev(q, loc), dc[0], dc[1], dc[2].view(E4M3), dc[3].view(E4M3), table.to(DEV), 0.1, lens.to(DEV))
+    if kernel is None:
+        got = A.hogwild_varlen_paged_sdpa_q4(*args, cu.to(DEV), status=st) if packed else A.hogwild_paged_sdpa_q4(*args, status=st)
+    else:
+        from inference_lib_b200 import _cabi
+        got = torch.empty((140, 8, 128) if packed else (2, 8, 1, 128), dtype=q.dtype, device=DEV)
+        x, keep = _cabi.bind_paged_q4(out=got, queries=args[0], locations=args[1], key_cache=args[2], value_cache=args[3], key_scales=args[4],
+                                      value_scales=args[5], block_table=args[6], scale=0.1, fragment_lengths=args[8],
+                                      cu_seqlens_q=cu.to(DEV) if packed else None, kernel=kernel, status=st)
+        assert _cabi.launch_paged_q4(x, torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+    assert int(st) == 1024
+    torch.testing.assert_close(got.reshape(seen.shape).float(), seen.float(), rtol=2 * 2.0 ** -8, atol=2.0 ** -9)      # (other kernels: a rounding apart)
+
+
 def test_refusals_of_the_operators(A):
     gen = torch.Generator().manual_seed(9)
     kc, vc, ks, vs = dev(*empty_cache(gen, 4, 2, 16, 64, 64))
