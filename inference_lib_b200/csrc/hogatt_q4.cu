@@ -161,7 +161,10 @@ int launch_q4_mma(const Q4MmaArgs& x, const Q4Plan& pl, int dev, int smem_optin,
     const int rc = ensure_smem_limit(q4_mma_kernel<T, HD, NT, ALIGNED, WARPS>, dev, smem, granted);
     if (rc != HOGATT_OK) return rc;
     HOGATT_CUDA_OK(launch_kernel(q4_mma_kernel<T, HD, NT, ALIGNED, WARPS>, dim3(x.ctas ? x.ctas : pl.units), dim3(WARPS * 32), smem, stream, x));
-    if (x.ctas) HOGATT_CUDA_OK(launch_kernel(q4_mma_merge_kernel<T, HD>, dim3(pl.units, pl.rows), dim3(128), 0, stream, x));
+    if (!x.ctas) return HOGATT_OK;
+    // a unit's partials: about ctas / units and one more at either end
+    if (x.ctas / pl.units + 2 > 8) HOGATT_CUDA_OK(launch_kernel(q4_mma_merge_kernel<T, HD, true>, dim3(pl.units, pl.rows), dim3(128), 0, stream, x));
+    else HOGATT_CUDA_OK(launch_kernel(q4_mma_merge_kernel<T, HD, false>, dim3(pl.units, (pl.rows + 3) / 4), dim3(128), 0, stream, x));
     return HOGATT_OK;
 }
 template <class T, int HD, int NT>

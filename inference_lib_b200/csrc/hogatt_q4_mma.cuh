@@ -717,14 +717,15 @@ __global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel
     }
 }
 
-// Adds up the partials of one output row (one CTA): warp w takes every fourth, a lane four (two) columns.  Units that one CTA had to
-// itself are stored already; rows that see nothing, of which the list has no tile, are zeros.
-template <class T, int HD>
+// Adds up the partials of an output row, a lane four (two) columns.  WIDE: a CTA per row, warp w takes every fourth partial (few units have many
+// partials each); otherwise a warp per row.  Units that one CTA had to itself are stored already; rows that see nothing, of which the list
+// has no tile, are zeros.
+template <class T, int HD, bool WIDE>
 __global__ void __launch_bounds__(128) q4_mma_merge_kernel(const __grid_constant__ Q4MmaArgs x) {
-    constexpr int VEC = HD / 32;
+    constexpr int VEC = HD / 32, STRIDE = WIDE ? 4 : 1;
     const PagedArgs& a = x.p;
-    __shared__ float sm_m[4], sm_l[4], sm_o[4][HD];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, unit = blockIdx.x, row = blockIdx.y;
+    __shared__ float sm_m[4], sm_l[4], sm_o[WIDE ? 4 : 1][HD];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, unit = blockIdx.x, row = WIDE ? blockIdx.y : blockIdx.y * 4 + warp;
     const int per_group = a.Hkv * a.head_blocks, grp = unit / per_group;
     PagedUnit u;
     pdl_wait();
@@ -744,12 +745,12 @@ __global__ void __launch_bounds__(128) q4_mma_merge_kernel(const __grid_constant
     if (!there || !paged_row(a, u, row, &s_abs, &hq)) return;
     T* const out = static_cast<T*>(a.out) + u.w * a.o_w + s_abs * a.o_s + hq * a.o_h;
     float M = -FLT_MAX, L = 0.f, acc[VEC] = {};
-    for (int p0 = warp; p0 < count; p0 += 32) {           // eight partials of a warp in flight
+    for (int p0 = WIDE ? warp : 0; p0 < count; p0 += 8 * STRIDE) {        // eight partials of a warp in flight
         float mp[8], lp[8], v[8][VEC];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const size_t at = ((size_t)(first + p0 + 4 * k) + unit) * kFmaRows + row;
-            const bool have = p0 + 4 * k < count;
+            const size_t at = ((size_t)(first + p0 + STRIDE * k) + unit) * kFmaRows + row;
+            const bool have = p0 + STRIDE * k < count;
             mp[k] = have ? __ldcg(a.ws_m + at) : -FLT_MAX;
             lp[k] = have ? __ldcg(a.ws_l + at) : 0.f;
             if constexpr (VEC == 4) {
@@ -776,27 +777,30 @@ __global__ void __launch_bounds__(128) q4_mma_merge_kernel(const __grid_constant
             for (int i = 0; i < VEC; ++i) acc[i] = fmaf(v[k][i], wgt, acc[i]);
         }
     }
-    if (lane == 0) {
-        sm_m[warp] = M;
-        sm_l[warp] = L;
-    }
+    if constexpr (WIDE) {
+        if (lane == 0) {
+            sm_m[warp] = M;
+            sm_l[warp] = L;
+        }
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sm_o[warp][lane * VEC + i] = acc[i];
-    __syncthreads();
-    if (warp != 0) return;
-    const float top = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
-    L = 0.f;
-    float r[VEC] = {};
+        for (int i = 0; i < VEC; ++i) sm_o[warp][lane * VEC + i] = acc[i];
+        __syncthreads();
+        if (warp != 0) return;
+        const float top = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
+        L = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float wgt = exp2_fast(sm_m[w] - top);
-        L = fmaf(sm_l[w], wgt, L);
+        for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) r[i] = fmaf(sm_o[w][lane * VEC + i], wgt, r[i]);
+        for (int w = 0; w < 4; ++w) {
+            const float wgt = exp2_fast(sm_m[w] - top);
+            L = fmaf(sm_l[w], wgt, L);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[i] = fmaf(sm_o[w][lane * VEC + i], wgt, acc[i]);
+        }
     }
     const float inv = L == 0.f ? 0.f : x.vunit / L;
-    if constexpr (VEC == 4) store4<T>(out + lane * 4, r[0] * inv, r[1] * inv, r[2] * inv, r[3] * inv);
-    else *reinterpret_cast<uint32_t*>(out + lane * 2) = pack2<T>(r[0] * inv, r[1] * inv);
+    if constexpr (VEC == 4) store4<T>(out + lane * 4, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    else *reinterpret_cast<uint32_t*>(out + lane * 2) = pack2<T>(acc[0] * inv, acc[1] * inv);
 }
 
 }  // namespace hogatt
