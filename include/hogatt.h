@@ -63,7 +63,7 @@ typedef enum hogatt_status {
     HOGATT_ERR_BAD_KERNEL_CHOICE = -9,
     HOGATT_ERR_TOO_LARGE = -10,
     HOGATT_ERR_EXCEEDS_STATIC_SCRATCH = -11, /* hogatt_fused_launch_static: needs more than HOGATT_STATIC_SCRATCH_BYTES */
-    HOGATT_ERR_BAD_UNIT = -12           /* a 4-bit cache's unit is not a power of two between 2^-64 and 2^64 */
+    HOGATT_ERR_BAD_UNIT = -12           /* a 4-bit cache's unit is not a power of two between 2^-64 and 2^64, or scale * log2(e) * key unit is no fp32 number */
 } hogatt_status;
 
 /* Which device code runs.  AUTO picks the tensor-core kernel for f16/bf16 with E == Ev in {64, 128}
@@ -330,7 +330,7 @@ int hogatt_copy_to_blocks_launch(const void* key_states, const void* value_state
  *   scales e4m3  [num_blocks, Hkv, block_size, E/16]   one per 16 consecutive channels
  *   value[e] = e2m1(code[e]) * scale[e / 16] * unit
  * `unit` is a power of two between 2^-64 and 2^64 that the caller keeps for the cache's keys and for its values (HOGATT_ERR_BAD_UNIT
- * otherwise): it moves the range of the scales, 2^-9 to 448, to where the numbers are.  1 suits numbers between 0.1 and 2,688; groups
+ * otherwise, and where attention's scale * log2(e) * key unit leaves fp32): it moves the range of the scales, 2^-9 to 448, to where the numbers are.  1 suits numbers between 0.1 and 2,688; groups
  * whose largest magnitude is below 6 * 2^-6 * unit lose precision, below 3 * 2^-9 * unit they are stored as zeros.
  * Writing: with a = the group's largest magnitude, scale = e4m3(a / (6 unit)), at most 448; code = e2m1(x / (scale unit)), at most 6;
  * all roundings to the nearest, ties to even, divisions in fp32.  A group that holds an infinity or a NaN gets the scale NaN, and every

@@ -85,7 +85,6 @@ bool dense_wanted(const hogatt_paged_problem* p) {
     return (double)tokens * p->Hq * p->max_blocks_per_seq * p->block_size >= 4.5e6;
 }
 
-
 int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
     if (x == nullptr) return HOGATT_ERR_NULL_POINTER;
     const hogatt_paged_problem* p = &x->paged;
@@ -107,8 +106,9 @@ int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
     const int G = p->Hq / p->Hkv, most = G >= 16 ? 1 : 16 / G;
     if (pl->kernel == HOGATT_KERNEL_DENSE) {
         pl->tokens = kDenseRows / G;
-        pl->blocks = p->total_q_tokens / (2 * pl->tokens) + p->W;
-        if ((int64_t)pl->blocks * p->Hkv > (1 << 24)) return HOGATT_ERR_TOO_LARGE;
+        const int64_t blocks = (int64_t)p->total_q_tokens / (2 * pl->tokens) + p->W;
+        if (blocks * p->Hkv > (1 << 24)) return HOGATT_ERR_TOO_LARGE;
+        pl->blocks = (int)blocks;
         pl->ctas = std::min(sms, kDenseMaxCtas);
         pl->w = carve_dense_plan(pl->blocks, p->Hkv, p->F, pl->ctas);
         pl->queries = pl->w.total;
@@ -128,6 +128,8 @@ int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
     if (units > (1 << 24)) return HOGATT_ERR_TOO_LARGE;
     pl->groups_bound = (int)groups;
     pl->units = (int)std::max<int64_t>(units, 1);
+    // tiles are counted in 32 bits, a unit's where it has a CTA to itself, otherwise all units'
+    const int64_t keys = std::min<int64_t>((int64_t)p->max_blocks_per_seq * p->block_size + 1, INT_MAX), tiles = p->F * (keys / 32 + 1);
     size_t slots;
     if (pl->kernel == HOGATT_KERNEL_MMA) {
         pl->splits = 0;
@@ -139,11 +141,13 @@ int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
         // keys (512 units) 64.8 / 75.7.
         pl->ctas = likely >= kQ4Ctas * sms ? 0 : kQ4Ctas * sms;
         pl->small = likely >= 2 * kQ4Ctas * sms;
+        if (tiles > INT_MAX / (pl->ctas ? groups : 1)) return HOGATT_ERR_TOO_LARGE;
         slots = pl->ctas ? ((size_t)pl->units + pl->ctas) * kFmaRows : 0;
     } else {
         pl->ctas = 0;
         pl->splits = std::max(1, std::min(24, (3 * sms + pl->units - 1) / pl->units));      // (24: the merge step's one round trip)
         slots = (size_t)pl->units * pl->splits * kFmaRows;
+        if (tiles > INT_MAX) return HOGATT_ERR_TOO_LARGE;
     }
     pl->o = 0;
     pl->m = pl->o + align_up(slots * p->Ev * sizeof(float), 256);
@@ -387,6 +391,7 @@ int hogatt_paged_q4_sdpa_launch(const hogatt_paged_q4_problem* x, hogatt_stream_
     if (rc != HOGATT_OK) return rc;
     const hogatt_paged_problem* p = &x->paged;
     if (!unit_ok(x->key_unit) || !unit_ok(x->value_unit)) return HOGATT_ERR_BAD_UNIT;
+    if (std::isfinite(p->scale) && !std::isfinite((float)((double)p->scale * 1.4426950408889634 * x->key_unit))) return HOGATT_ERR_BAD_UNIT;
     if (!p->out || !p->queries || !p->locations || !p->fragment_lengths || !p->key_cache || !p->value_cache || !x->key_scales ||
         !x->value_scales || !p->block_table || !p->workspace)
         return HOGATT_ERR_NULL_POINTER;

@@ -54,6 +54,11 @@ def _paged(**kw):
     (dict(key_unit=0.3), UNIT), (dict(value_unit=-1.0), UNIT), (dict(key_unit=0.0), UNIT), (dict(value_unit=float("nan")), UNIT),
     (dict(value_unit=float("inf")), UNIT), (dict(key_unit=2.0 ** 70), UNIT), (dict(key_scales=None), NULL), (dict(workspace=None), NULL),
     (dict(value_scales=4104), ALIGN), (dict(key_cache=4097), ALIGN), (dict(workspace=4112), ALIGN), (dict(W=1 << 30, S=4), LARGE),
+    (dict(scale=1e25, key_unit=2.0 ** 64), UNIT),                          # the scores' factor is no fp32 number
+    (dict(F=4096, max_blocks_per_seq=1 << 20, block_size=1 << 10), LARGE), # more tiles than 32 bits count
+    (dict(F=4096, max_blocks_per_seq=1 << 20, block_size=1 << 10, dtype=_cabi.F32), LARGE),
+    # sequences and tokens whose units do not fit 32 bits: asked of the kernel for chunks
+    (dict(W=2147483392, total_q_tokens=2147483647, Hq=1, Hkv=1, cu_seqlens_q=4096, kernel=4), LARGE),
 ])
 def test_attention_refuses(lib, change, rc):
     assert lib.hogatt_paged_q4_sdpa_launch(C.byref(_paged(**change)), None) == rc
