@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kFmaThreads) q4_attention_kernel(const __grid_
                 float val = 0.f;
                 if (paged_row(a, u, r, &s_abs, &hq))
                     val = Scalar<T>::to_float(q[f * a.q_f + u.w * a.q_w + s_abs * a.q_s + hq * a.q_h + e]);
-                core.Qs[idx] = val;
+                core.Qs[idx] = fabsf(val) == INFINITY ? NAN : val;        // (scores of -infinity would look like keys that are not seen)
             }
             if (tid < kFmaRows) {
                 int s_abs, hq, lim = 0;
@@ -405,8 +405,7 @@ __global__ void __launch_bounds__(kFmaThreads) q4_attention_kernel(const __grid_
             }
         }
         __syncthreads();
-        // keys without a page are seen by nobody: a NaN key product would not be masked away, so their K rows are zeros and the
-        // scores are taken out through the tile's length where they end it, or key by key here
+        // (keys without a page were staged as zeros; compute() takes them out key by key)
         int any = 0;
         for (int k = 0; k < ntok; ++k) any |= odd[k];
         if (any && tid < kFmaRows) {

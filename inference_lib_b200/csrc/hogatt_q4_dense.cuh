@@ -149,28 +149,27 @@ __device__ __forceinline__ uint32_t q4_odd_groups(const DenseArgs& a, int w, int
     return odd;
 }
 
-// bf16 queries as fp16, each (token, head)'s largest magnitude (over the fragments) brought to [2^14, 2^15); factor: what brings its scores
-// back, with the scale.  A row with an infinity or a NaN becomes NaN.  One warp per (token, head), four channels per lane.  It starts beside the
-// plan kernel, which is behind everything that may still write the queries, and ends after it.
+// bf16 queries as fp16, each (token, head)'s largest finite magnitude (over the fragments) brought to [2^14, 2^15); factor: what brings its
+// scores back, with the scale.  A fragment's row with an infinity or a NaN becomes NaN.  One warp per (token, head), four channels per lane.  It
+// starts beside the plan kernel, which is behind everything that may still write the queries, and ends after it.
 __global__ void __launch_bounds__(256) q4_dense_queries_kernel(const __nv_bfloat16* q, __half* out, float* factor, int F, int rows, float l2scale) {
     const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row < rows) {
+        auto load = [&](int f) { return *reinterpret_cast<const uint2*>(q + ((size_t)f * rows + row) * 128 + lane * 4); };
+        auto largest = [](uint2 v) { return max(max(v.x & 0x7fff0000u, (v.x & 0x7fffu) << 16), max(v.y & 0x7fff0000u, (v.y & 0x7fffu) << 16)); };
         uint32_t top = 0;
         for (int f = 0; f < F; ++f) {
-            const uint2 v = *reinterpret_cast<const uint2*>(q + ((size_t)f * rows + row) * 128 + lane * 4);
-            top = max(max(top, max(v.x & 0x7fff0000u, (v.x & 0x7fffu) << 16)), max(v.y & 0x7fff0000u, (v.y & 0x7fffu) << 16));
+            const uint32_t mine = __reduce_max_sync(0xffffffffu, largest(load(f)));
+            if (mine < 0x7f800000u) top = max(top, mine);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const bool finite = top < 0x7f800000u;
         const int e = min(120, 14 - ((int)(top >> 23) - 127));
-        const float up = finite ? __int_as_float((e + 127) << 23) : NAN;
-        if (lane == 0) factor[row] = finite ? fmaxf(l2scale * __int_as_float((127 - e) << 23), 1e-36f) : l2scale;
+        if (lane == 0) factor[row] = fmaxf(l2scale * __int_as_float((127 - e) << 23), 1e-36f);
         for (int f = 0; f < F; ++f) {
-            const size_t at = ((size_t)f * rows + row) * 128 + lane * 4;
-            const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(q + at);
-            *reinterpret_cast<uint2*>(out + at) = make_uint2(pack2<__half>(__low2float(v[0]) * up, __high2float(v[0]) * up),
-                                                             pack2<__half>(__low2float(v[1]) * up, __high2float(v[1]) * up));
+            const uint2 x = load(f);
+            const float up = __any_sync(0xffffffffu, largest(x) >= 0x7f800000u) ? NAN : __int_as_float((e + 127) << 23);
+            const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(&x);
+            *reinterpret_cast<uint2*>(out + ((size_t)f * rows + row) * 128 + lane * 4) =
+                make_uint2(pack2<__half>(__low2float(v[0]) * up, __high2float(v[0]) * up), pack2<__half>(__low2float(v[1]) * up, __high2float(v[1]) * up));
         }
     }
     pdl_wait();

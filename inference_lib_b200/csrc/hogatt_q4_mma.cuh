@@ -432,16 +432,21 @@ __global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel
                 }
                 float mine = fabsf(a.l2scale);
                 uint32_t* r = reinterpret_cast<uint32_t*>(raw);
-                if constexpr (!std::is_same<T, __half>::value) {
-                    uint32_t top = 0;                     // the largest magnitude's bits: bf16 in the upper half
+                // a row with an infinity or a NaN becomes NaN; the factor stays a number, so that a key which the row does not see is -inf times it
+                constexpr bool half = std::is_same<T, __half>::value;
+                uint32_t top = 0;                         // the largest magnitude's bits, in the upper half
 #pragma unroll
-                    for (int k = 0; k < CPT / 2; ++k) top = max(top, max(r[k] & 0x7fff0000u, (r[k] & 0x7fffu) << 16));
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    // times 2^e so that the largest lies in [2^14, 2^15); an infinity or a NaN makes the row NaN
+                for (int k = 0; k < CPT / 2; ++k) top = max(top, max(r[k] & 0x7fff0000u, (r[k] & 0x7fffu) << 16));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const bool finite = top < (half ? 0x7c000000u : 0x7f800000u);
+                if constexpr (half) {
+#pragma unroll
+                    for (int k = 0; k < CPT / 2; ++k) r[k] = finite ? r[k] : 0x7fff7fffu;
+                } else {                                  // times 2^e so that the largest lies in [2^14, 2^15)
                     const int e = min(120, 14 - ((int)(top >> 23) - 127));
-                    const float up = top >= 0x7f800000u ? NAN : __int_as_float((e + 127) << 23);
-                    mine *= top >= 0x7f800000u ? NAN : __int_as_float((127 - e) << 23);
+                    const float up = finite ? __int_as_float((e + 127) << 23) : NAN;
+                    mine *= finite ? __int_as_float((127 - e) << 23) : 1.f;
 #pragma unroll
                     for (int k = 0; k < CPT / 2; ++k) {
                         const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&r[k]);

@@ -369,6 +369,30 @@ def test_rows_that_see_nothing_are_zero(A):
     assert bool((got == 0).all())
 
 
+@pytest.mark.parametrize("dtype,E", [(torch.bfloat16, 128), (torch.float16, 128), (torch.bfloat16, 64), (torch.float32, 64)])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_queries_that_are_no_numbers_and_see_nothing(A, dtype, E, kernel):
+    """Zeros, also beside rows of the same tile that see something and over a fragment more that one of them sees."""
+    skip_unless_eligible(kernel, dtype, E, E, True, 16)
+    gen = torch.Generator().manual_seed(23)
+    cache = [x for pair in zip(*(q4_util.random_cache(gen, 8, 2, 16, E) for _ in range(2))) for x in pair]
+    table = torch.arange(8, dtype=torch.int32).reshape(2, 4)
+    q = torch.randn(2, 8, 8, E, generator=gen).to(dtype)
+    loc = torch.tensor([[30, -1, 40, -1, 20, 50, -1, -1], [10, -1, -1, -1, 63, 50, -1, -1]], dtype=torch.int32)
+    for row, bad in ((1, float("nan")), (3, float("inf")), (6, float("nan")), (7, -float("inf"))):
+        q[:, row, :, 3] = bad
+    q[1, 2] = float("nan")                                                    # (sees keys of the other fragment only)
+    cu, lens = torch.tensor([0, 4, 8], dtype=torch.int32), torch.tensor([[64, 64], [64, 64]], dtype=torch.int32)
+    got, exact = paged(A, q, loc, lens, cache, table, E ** -0.5, cu=cu, kernel=kernel)
+    q4_util.check(got, exact)
+    assert bool((got[[1, 3, 6, 7]] == 0).all()) and not bool(got.isnan().any())
+    if kernel != 4:                                                          # an infinite query of a row that sees one key, whichever sign
+        q[0, 0, :, 3], q[0, 5, :, 3], loc[:, 0], loc[:, 5] = float("inf"), -float("inf"), torch.tensor([0, -1]), torch.tensor([0, -1])
+        got, exact = paged(A, q, loc, lens, cache, table, E ** -0.5, cu=cu, kernel=kernel)
+        q4_util.check(got, exact)
+        assert bool(got[[0, 5]].isnan().all())
+
+
 def test_large_and_small_queries(A):
     """bf16 queries beyond fp16's range, and below it."""
     gen = torch.Generator().manual_seed(8)
