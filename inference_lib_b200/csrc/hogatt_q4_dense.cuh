@@ -1,17 +1,21 @@
 // Packed prompt chunks over 4-bit pages on the tcgen05 kernel (hogatt_dense.cuh with Q4): head size 128, blocks of a multiple of eight rows.
 //
 // The tensor cores take both operands in one 16-bit type from swizzled shared memory, so what the TMA does for 16-bit pages a warp does
-// here: two warps unpack K tiles, two V tiles, 64 keys each.  A key is a row of 64 bytes of codes and 8 of scales, copied 32 keys at a time by
-// cp.async, two units ahead (rings of three; the K ring of tiles gives one of its three places for them), converted two values
-// per instruction, multiplied by their scales -- exact in fp16 -- and stored where the 128-byte swizzle wants them.  That is 1,600
-// instructions a step of the four warps together beside 5,600 of the softmax warps.  Unpacking into 16-bit pages in the workspace
-// first would take four times the cache's memory.
+// here: one unpacks K tiles, one V tiles (128 keys).  A key is a row of 64 bytes of codes and 8 of scales, copied 32 keys at a time by
+// cp.async into a ring of six such units a warp (a third K tile would lie there), converted two values per instruction, multiplied by
+// their scales -- exact in fp16 -- and stored where the 128-byte swizzle wants them.  Unpacking into 16-bit pages in the workspace first would
+// take four times the cache's memory.
+//
+// Bound by those two warps, which share their schedulers with the softmax warps: 2,048 tokens of 4,000 keys, 32 / 8 heads, fp16: 159 us (145
+// without the copies, 120 without the conversions, 106 without either); two chunks of 512 tokens of 6,000 keys beside six single tokens, bf16: 181 us.
+// Slower: four unpacking warps of 24 (registers spill: 220 us); a third one for a quarter of both tiles, both products issued by one warp (219 us).
+// 96 registers for every thread: nothing is left to take from the other warps.
 //
 // fp16 for both products: six significant bits times a probability; bf16 queries become fp16 once per call, a power of two per (token, head)
 // taken out (q4_dense_queries_kernel), which the softmax multiplies back in.
 //
 // Values that are not numbers are stored as zeros, keys without a page as zeros too; what is special about a tile travels to the softmax
-// warps in a ring of eight words (K tiles are at most three ahead of the scores that are read), and only for such tiles they look
+// warps in a ring of eight entries (K tiles are at most three ahead of the scores that are read), and only for such tiles they look
 // the scales and the block table up again: a row that sees such a value has NaN in that group's channels.
 #pragma once
 #include "hogatt_dense.cuh"
