@@ -324,7 +324,7 @@ __device__ __forceinline__ DenseRow dense_row(const DenseArgs& a, int tile, int 
 // rows of fragment f that hold keys and values (worker w's, when paged)
 template <bool PAGED>
 __device__ __forceinline__ int dense_length(const DenseArgs& a, int f, int w) {
-    if constexpr (PAGED) return min(a.flen[f * a.W + w], a.most_keys);
+    if constexpr (PAGED) return max(0, min(a.flen[f * a.W + w], a.most_keys));
     return a.flen ? min(a.cap[f], a.flen[f]) : a.cap[f];
 }
 template <bool PAGED>

@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ Q4
 // than it has pages for (a length that is wrong would be a walk over two billion keys).
 __device__ __forceinline__ int most_visible(const PagedArgs& a, int loc, int len) {
     const int64_t most = min((int64_t)a.max_blocks * a.block_size + 1, (int64_t)INT_MAX - 4096);
-    return (int)min((int64_t)(max(0, min(loc, len - 1) + 1)), most);
+    return (int)min((int64_t)(max(0, min(loc, max(len, 0) - 1) + 1)), most);
 }
 
 struct Q4Args {

@@ -525,6 +525,19 @@ def test_lengths_that_are_wrong_end(A, kernel, packed):
     torch.testing.assert_close(got.reshape(seen.shape).float(), seen.float(), rtol=2 * 2.0 ** -8, atol=2.0 ** -9)      # (other kernels: a rounding apart)
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_lengths_below_zero_are_none(A, kernel):
+    gen = torch.Generator().manual_seed(17)
+    cache = [x for pair in zip(*(q4_util.random_cache(gen, 8, 2, 16, 128) for _ in range(2))) for x in pair]
+    table, st = torch.arange(8, dtype=torch.int32).reshape(4, 2), status()
+    q = torch.randn(1, 6, 8, 128, generator=gen).bfloat16()
+    loc = torch.tensor([[30, 31, 31, 2 ** 31 - 1, -2 ** 31, 31]], dtype=torch.int32)
+    cu, lens = torch.tensor([0, 2, 3, 5, 6], dtype=torch.int32), torch.tensor([[-2 ** 31, -2 ** 31 + 1, -7, 32]], dtype=torch.int32)
+    got, exact = paged(A, q, loc, lens, cache, table, 0.1, cu=cu, st=st, kernel=kernel)
+    q4_util.check(got, exact)
+    assert bool((got[:5] == 0).all()) and bool((got[5] != 0).any()) and int(st) == 0
+
+
 def test_refusals_of_the_operators(A):
     gen = torch.Generator().manual_seed(9)
     kc, vc, ks, vs = dev(*empty_cache(gen, 4, 2, 16, 64, 64))
