@@ -280,3 +280,56 @@ def test_a_batch_from_prompt_to_the_end(A, dtype, E, bs):
         assert np.array_equal(keys[w, :, :len(h[0])].cpu().double().numpy(), want.transpose(1, 0, 2))
     refs, table, lengths, _ = A.step_blocks(refs, table, lengths, flat, bs, source=ints([-1]))          # everything goes back
     assert not bool(refs.any()) and lengths.tolist() == [0] and bool((table == -1).all()) and int(st) & ~1024 == 0
+
+
+def test_caches_of_more_than_four_gigabytes(A):
+    """Pages whose bytes begin behind 2^32: written, read, attended to by every kernel, copied and moved like pages in front."""
+    gen = torch.Generator().manual_seed(31)
+    Hkv, G, bs, E, W, width = 8, 4, 16, 128, 2, 10
+    blocks = 2 ** 19 + 64                                                        # 8 KiB of codes a page
+    small = [torch.zeros(W * width + 2, Hkv, bs, n, dtype=t, device=DEV) for n, t in ((E // 2, torch.uint8), (E // 2, torch.uint8), (E // 16, E4M3), (E // 16, E4M3))]
+    large = [torch.empty(blocks, *c.shape[1:], dtype=c.dtype, device=DEV) for c in small]
+    assert large[0].numel() > 2 ** 32
+    near = torch.arange(W * width, dtype=torch.int32, device=DEV).reshape(W, width)
+    far = blocks - 1 - near
+    k, v = (torch.randn(W, Hkv, width * bs, E, generator=gen).bfloat16().to(DEV) for _ in range(2))
+    start = ints([0] * W)
+    for caches, table in ((small, near), (large, far)):
+        A.copy_to_blocks_q4(k, v, *caches, table, start)
+    for a, b in zip(small, large):
+        assert torch.equal(a.view(torch.uint8)[near.flatten().long()], b.view(torch.uint8)[far.flatten().long()])
+    for a, b in zip(*(A.copy_from_blocks_q4(*c, t, start, width * bs) for c, t in ((small, near), (large, far)))):
+        assert torch.equal(a, b)
+    from inference_lib_b200 import _cabi
+    counts, lens = [130, 1], [150, 157]
+    q = torch.randn(1, sum(counts), Hkv * G, E, generator=gen).bfloat16().to(DEV)
+    loc = ints([[n - c + i for n, c in zip(lens, counts) for i in range(c)]])
+    for kernel in (1, 2, 4):
+        out = []
+        for c, t in ((small, near), (large, far)):
+            out.append(torch.empty_like(q[0]))
+            x, keep = _cabi.bind_paged_q4(out=out[-1], queries=q, locations=loc, key_cache=c[0], value_cache=c[1], key_scales=c[2], value_scales=c[3],
+                                          block_table=t, scale=0.1, fragment_lengths=ints([lens]), cu_seqlens_q=ints([0, 130, 131]), kernel=kernel)
+            assert _cabi.launch_paged_q4(x, torch.cuda.current_stream().cuda_stream) == 0
+            torch.cuda.synchronize()
+        assert torch.equal(*out) and bool(out[0].isfinite().all())
+    # blocks of eight rows (rows looked up one by one), the same bytes
+    small8, large8 = ([t.view(t.shape[0] * 2, Hkv, 8, t.shape[3]) for t in c] for c in (small, large))
+    near8, far8 = (torch.stack([2 * t, 2 * t + 1], -1).reshape(W, 2 * width) for t in (near, far))
+    q1, loc1 = q[:, :W].reshape(1, W, Hkv * G, 1, E).contiguous(), ints([[[150], [157]]])
+    assert torch.equal(*(A.hogwild_paged_sdpa_q4(q1, loc1, *c, t.int(), 0.1, ints([158])) for c, t in ((small8, near8), (large8, far8))))
+    # a fork of a row whose last page lies far behind, onto a free page in front of it; then everything to the front
+    refs = torch.zeros(blocks, dtype=torch.int32, device=DEV)
+    refs[:blocks - 64] = 1                                                       # somebody else's
+    refs[far.flatten().long()] = 1
+    n = ints([width * bs - 3, 8])
+    refs, table, n, room = A.step_blocks(refs, far.contiguous(), n, large, bs, source=ints([0, 0]), new_tokens=ints([1, 1]))
+    copied = int(table[0, width - 1])
+    assert room.tolist() == [1, 1] and copied == blocks - 64 and int(table[1, width - 1]) == int(far[0, width - 1])
+    for c in large:
+        assert torch.equal(c.view(torch.uint8)[copied], c.view(torch.uint8)[int(far[0, width - 1])])
+    refs[:blocks - 64] = 0
+    refs, table, moved = A.compact_blocks(refs, table, large)
+    assert sorted(set(table[table >= 0].tolist())) == list(range(width + 1)) and int((refs != 0).sum()) == width + 1
+    for a, b in zip(A.copy_from_blocks_q4(*small, near[:1], start[:1], width * bs - 3), A.copy_from_blocks_q4(*large, table[:1], start[:1], width * bs - 3)):
+        assert torch.equal(a, b)
