@@ -2,8 +2,8 @@
 //
 // By its bytes bound by HBM: 9/8 byte per (key, channel) of K and V together, 144 bytes per key and kv head at head size 128, against 512 in
 // 16 bits -- so what a key costs on the SM counts: at the full copy rate an SM has to finish one every six cycles.  Bound by instruction issue:
-// 340 instructions of a warp per 16 keys, the schedulers at 62-64 %.  2 sequences of 131,072 keys, 8 kv heads of 4 heads: 75.7 us = 3.99 TB/s;
-// 24 of about 6,000 keys, 5 heads: 43 us; 8 of 16,384 keys, 2 kv heads of 16 heads: 31.6 us, of which the walk is ten.
+// 340 instructions of a warp per 16 keys, the schedulers at 62-64 %.  2 sequences of 131,072 keys, 8 kv heads of 4 heads: 74.4 us = 4.06 TB/s;
+// 24 of about 6,000 keys, 5 heads: 43 us; 8 of 16,384 keys, 2 kv heads of 16 heads: 31.8 us, of which the walk is ten.
 //
 // Both products are taken transposed, keys or value channels as the M of mma.sync m16n8k16 and up to eight query rows as its N:
 //     S^T [16 keys x 8 rows] = K [16 x E] Q^T,      O^T [E x 8 rows] += V^T [E x 16 keys] P^T
@@ -52,7 +52,10 @@ struct Q4MmaCfg {
     static constexpr int ROW = HD / 2, SROW = HD / kGroup;         // bytes of a row's codes and scales
     static constexpr int STAGE = 16 * 2 * (ROW + SROW) + 16;       // K, V, K scales, V scales of 16 keys; which have no page
     static constexpr int OFF_V = 16 * ROW, OFF_KS = 32 * ROW, OFF_VS = OFF_KS + 16 * SROW, OFF_BAD = OFF_VS + 16 * SROW;
-    static constexpr int NSTAGE = HD == 128 ? 5 : 8;
+    // Three tiles of a ring: sixteen warps an SM hide one another's copies, and a shorter prologue comes sooner to its first tile.  us with 5 / 4 / 3 / 2 at
+    // head size 128: 2 sequences of 131,072 keys 75.5 / 74.9 / 74.4 / 74.4, 24 ragged ones 43.5 / 43.1 / 43.0 / 42.8; with 8 / 6 / 5 / 3 at 64:
+    // the latter 32.8 / 32.8 / 32.2 / 31.6.
+    static constexpr int NSTAGE = 3;
     static constexpr int RING = WARPS * NSTAGE * STAGE;
     static constexpr int PITCH = HD + 4;                           // floats between rows of the fold
     static constexpr int fold_bytes(int rows) { return WARPS * rows * (PITCH + 2) * 4; }
