@@ -63,6 +63,7 @@ struct Q4Plan {
     int tokens_per_group, head_blocks, groups_bound, units, splits;
     int rows;                       // (MMA) query rows of a unit at most
     int ctas;                       // (MMA) shares of the list of tiles; 0: a CTA per unit
+    int unit_cost;                  // (MMA) what a unit counts for in the list beside its tiles
     bool small;                     // (MMA) CTAs of four warps
     size_t o, m, l, plan, total;
     int tokens, blocks;             // (DENSE) query tokens per tile, blocks per kv head at most
@@ -129,18 +130,24 @@ int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
     pl->groups_bound = (int)groups;
     pl->units = (int)std::max<int64_t>(units, 1);
     // tiles are counted in 32 bits, a unit's where it has a CTA to itself, otherwise all units'
-    const int64_t keys = std::min<int64_t>((int64_t)p->max_blocks_per_seq * p->block_size + 1, INT_MAX), tiles = p->F * (keys / 32 + 1);
+    const int64_t keys = std::min<int64_t>((int64_t)p->max_blocks_per_seq * p->block_size + 1, INT_MAX), tiles = p->F * (keys / 32 + 1) + 16;
     size_t slots;
     if (pl->kernel == HOGATT_KERNEL_MMA) {
         pl->splits = 0;
         // With at least as many units as resident CTAs each gets one to itself: shares of the list would hold ends of units (the warps' fold, the next
         // unit's first copies), which do not overlap inside a CTA, and the merge step is saved.  us per call with shares / without, 8 kv heads
-        // of 5 heads: 24 sequences of 6,000 keys 59.8 / 62.4, 37 of them 72.2 / 62.9, 64 of 2,000 keys 61.5 / 43.5.
+        // of 5 heads: 24 sequences of 6,000 keys 53.5 / 57.9, 37 of them 65.0 / 58.5, 46 of 2,000 keys 46.0 / 40.0 (40 of 6,000 79 / 93: the second
+        // round of CTAs is short there).
         const int64_t likely = (packed ? std::max<int64_t>(p->W, p->total_q_tokens / pl->tokens_per_group) : groups) * pl->head_blocks * p->Hkv;
-        // Four warps: 100 sequences of 700 keys 33.5 / 29.9 (eight / four), 200 of 1,000 keys 79.3 / 56.6, 148 of 200 keys 36.5 / 23.0; 64 of 4,000
-        // keys (512 units) 64.8 / 75.7.
+        // CTAs of four warps, twice as many resident, from three times as many units: a long unit takes them twice as long, which shows where lengths
+        // differ.  us with eight / four: 200 sequences of 1,000 keys 88 / 67, 148 of 200 keys 35.8 / 22.5; from 6,000 keys down in equal steps 64 of them
+        // 60 / 101, 100 of them 93 / 101, 120 of 5,100 down 98 / 90.
+        // What a unit costs beside its tiles (the fold, the first copies), in tiles: us with 0 / 2 / 4 / 6, 24 sequences of 6,000 keys down to 1,331
+        // 44.0 / 42.2 / 40.7 / 41.6, 30 of 4,000 down to 230 49.1 / 36.7 / 34.9 / 36.3, 20 of 1,500 down to 740 23.5 / 22.9 / 22.7 / 23.4.  Few units have hardly
+        // any ends in a share, but a tile more in it would show.
         pl->ctas = likely >= kQ4Ctas * sms ? 0 : kQ4Ctas * sms;
-        pl->small = likely >= 2 * kQ4Ctas * sms;
+        pl->small = likely >= 3 * kQ4Ctas * sms;
+        pl->unit_cost = 2 * likely > pl->ctas ? 4 : 0;
         if (tiles > INT_MAX / (pl->ctas ? groups : 1)) return HOGATT_ERR_TOO_LARGE;
         slots = pl->ctas ? ((size_t)pl->units + pl->ctas) * kFmaRows : 0;
     } else {
@@ -208,6 +215,7 @@ int launch_q4(const Q4Args& x, const Q4Plan& pl, int dev, int smem_optin, cudaSt
             y.kscale = x.kscale; y.vscale = x.vscale; y.num_blocks = x.num_blocks; y.vunit = x.vunit;
             y.block = fast_div_by((uint32_t)x.p.block_size);
             y.ctas = pl.ctas;
+            y.unit_cost = pl.unit_cost;
             y.plan = x.plan;
             return x.p.E == 128 ? launch_q4_mma_rows<T, 128>(y, pl, dev, smem_optin, stream) : launch_q4_mma_rows<T, 64>(y, pl, dev, smem_optin, stream);
         }

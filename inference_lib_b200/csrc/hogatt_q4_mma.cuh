@@ -22,7 +22,7 @@
 // rescaled only when some score exceeds the row's reference by 2^7 (P then stays below 128 in fp16).
 //
 // Split: units (<= 16 query rows that share keys, kv head) are cut into 128-key tiles, all units' tiles are one list, every CTA takes an
-// equal contiguous share (two CTAs per SM).  A share's part of a unit is a partial; q4_mma_merge_kernel adds them up.  With as many units as
+// equal contiguous share (two CTAs per SM), in which a unit's start and end count as some tiles.  A share's part of a unit is a partial; q4_mma_merge_kernel adds them up.  With as many units as
 // CTAs each unit gets a CTA of its own, and no merge step; with more, CTAs of four warps, four per SM, whose starts and ends overlap.
 #pragma once
 #include <float.h>
@@ -43,7 +43,8 @@ struct Q4MmaArgs {
     float vunit;
     FastDiv block;                // block size
     int ctas;                     // the list's shares; 0: a CTA per unit
-    int* plan;                    // [groups_bound + 1]: tiles of a kv head's units in front of every group of query tokens
+    int unit_cost;                // what a unit counts for in the list beside its tiles
+    int* plan;                    // [groups_bound + 1]: length of the list of one kv head's units in front of every group of query tokens
 };
 
 template <int HD, int WARPS>
@@ -242,6 +243,7 @@ __global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel
                     n += ceil_div(vis, C::TILE);
                 }
                 seen[e] = vis;
+                n += n ? x.unit_cost : 0;
             }
             const int at = before + block_exclusive(n, &total);
             if (e < groups) pre[e] = at;
@@ -280,6 +282,9 @@ __global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel
             j1 = (int)min((int64_t)n, j0 + (item_end - item));
             item += j1 - j0;
             again = item < item_end;
+            j0 = max(0, j0 - x.unit_cost);                // (the tiles stand behind what the unit costs)
+            j1 -= x.unit_cost;
+            if (j0 >= j1) continue;
             int wl = 0, wh = a.W;
             while (wh - wl > 1) {
                 const int mid = (wl + wh) >> 1;
@@ -747,7 +752,7 @@ __global__ void __launch_bounds__(128) q4_mma_merge_kernel(const __grid_constant
     if (n > 0) {
         const int64_t start = (int64_t)before * per_group + (int64_t)(unit - grp * per_group) * n;
         const int shares = effective_ctas(N, x.ctas);
-        first = cta_of_tile(start, N, shares);
+        first = cta_of_tile(start + x.unit_cost, N, shares);
         count = cta_of_tile(start + n - 1, N, shares) - first + 1;
         if (count == 1) return;
     }
