@@ -429,6 +429,24 @@ def test_many_short_sequences(A, dtype, G, E, bs, W, packed):
     q4_util.check(got, exact)
 
 
+@pytest.mark.parametrize("dtype,G,E,bs,W,F,longest", [(torch.bfloat16, 4, 128, 16, 50, 1, 500), (torch.float16, 2, 64, 8, 40, 2, 130), (torch.bfloat16, 12, 128, 32, 60, 1, 300),
+                                                      (torch.float16, 5, 128, 16, 45, 1, 1), (torch.bfloat16, 4, 128, 16, 39, 3, 900)])
+def test_shares_of_many_ragged_units(A, dtype, G, E, bs, W, F, longest):
+    """A list whose units' ends count: units of a few tiles and of none, shares that end in front of a unit's first tile."""
+    gen, rng = torch.Generator().manual_seed(W), np.random.default_rng(W)
+    Hkv, width, pages = 4, -(-longest // bs), 37
+    (kc, ks), (vc, vs) = (q4_util.random_cache(gen, pages, Hkv, bs, E) for _ in range(2))
+    table = torch.from_numpy(rng.integers(0, pages, (W, width)).astype(np.int32))
+    lens = torch.from_numpy(np.where(rng.random((F, W)) < 0.2, 0, rng.integers(1, longest + 1, (F, W))).astype(np.int32))
+    counts = rng.integers(0, 3, W)
+    counts[0] += W - min(W, int(counts.sum()))                              # (a token per sequence on average, at least)
+    cu = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32)
+    T = int(cu[-1])
+    loc = torch.from_numpy(rng.integers(longest - 1 - longest // 4, longest, (F, T)).astype(np.int32))
+    got, exact = paged(A, torch.randn(F, T, Hkv * G, E, generator=gen).to(dtype), loc, lens, (kc, vc, ks, vs), table, E ** -0.5, cu=cu, kernel=2)
+    q4_util.check(got, exact)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.1, 1e-30, 3.0])
 @pytest.mark.parametrize("kernel", KERNELS)
 def test_scales_of_the_scores(A, scale, kernel):
