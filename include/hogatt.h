@@ -321,6 +321,16 @@ int hogatt_copy_to_blocks_launch(const void* key_states, const void* value_state
                                  int32_t S_new, int32_t E, int32_t Ev, int32_t block_size, int32_t max_blocks,
                                  int32_t dtype, hogatt_stream_t stream);
 
+/*
+ * The same for tables whose rows need not have all their pages (hogatt_step_blocks_launch leaves such): rows t >= new_rows[b] (NULL: none)
+ * of sequence b stay out, and rows whose position has no page -- a table entry outside [0, num_blocks), a position behind the table or in
+ * front of it -- are dropped.  hogatt_copy_to_blocks_launch drops rows at negative entries too, but cannot tell entries behind the cache.
+ */
+int hogatt_copy_to_blocks_rows_launch(const void* key_states, const void* value_states, void* key_cache, void* value_cache,
+                                      const int32_t* block_table, const int32_t* seq_lengths, const int32_t* new_rows,
+                                      int32_t B, int32_t Hkv, int32_t S_new, int32_t E, int32_t Ev, int32_t block_size,
+                                      int32_t max_blocks, int32_t num_blocks, int32_t dtype, hogatt_stream_t stream);
+
 /* ---- a paged cache in 4 bits --------------------------------------------------------------------------- */
 
 /*
@@ -411,6 +421,11 @@ int hogatt_copy_from_blocks_q4_launch(const hogatt_q4_read* p, hogatt_stream_t s
  * table entry (a prefix for later) adds one.  A page with refs[p] == 0 is free.  A row of a block table names the pages of its
  * sequence in order, -1 behind the last.  Everything here works for caches of any type: the `caches` are all tensors whose first axis is the
  * page (keys, values and scales of every layer), `block_bytes` what one page of each takes.  Host arrays.
+ *
+ * An empty row, and a row that found no pages, has -1 where its next page would be, and a row that found none may share its last page.  So
+ * what is appended goes by `room`: new_rows of hogatt_copy_to_blocks_rows_launch and of hogatt_q4_append.  And queries see no
+ * further than lengths + room: hogatt_paged_sdpa_launch reads the page of every key that some row sees, which has to be there
+ * (hogatt_paged_q4_sdpa_launch leaves keys without a page out).
  */
 typedef struct hogatt_block_tensors {
     int32_t count;
@@ -428,7 +443,7 @@ typedef struct hogatt_block_tensors {
  *   2. Rows get the pages for new_tokens[w] (NULL: none) tokens behind their length, lowest free page first, in row order.  A row whose last
  *      page is partly filled and shared gets a page of its own with the old one's contents, in all caches, unless it is the last that
  *      still holds it.
- *   room[w] = new_tokens[w] if the row has its pages, else 0 (what hogatt_q4_append takes as new_rows).  A row that does not fit the table gets
+ *   room[w] = new_tokens[w] if the row has its pages, else 0 (what the appends take as new_rows).  A row that does not fit the table gets
  *      none (2048 in *device_status; so does a source row that does not exist).  Rows are served in order until one finds too few free
  *      pages (512): it and all rows behind it get none, and their tables stay as step 1 leaves them.
  * Writes refs_out, table_out [rows_out, max_blocks], lengths_out [rows_out] = the rows' lengths without the new tokens, room [rows_out].  Outputs

@@ -19,7 +19,8 @@ MAX_FRAGMENTS = 128
 
 EXPORTS = ["hogatt_abi_version", "hogatt_status_string", "hogatt_last_cuda_error", "hogatt_workspace_bytes",
            "hogatt_sdpa_launch", "hogatt_fused_launch", "hogatt_fused_launch_static", "hogatt_fused_launch_gather", "hogatt_rope_launch",
-           "hogatt_paged_workspace_bytes", "hogatt_paged_sdpa_launch", "hogatt_copy_to_blocks_launch", "hogatt_plan_describe",
+           "hogatt_paged_workspace_bytes", "hogatt_paged_sdpa_launch", "hogatt_copy_to_blocks_launch", "hogatt_copy_to_blocks_rows_launch",
+           "hogatt_plan_describe",
            "hogatt_plan_ranges", "hogatt_dense_plan", "hogatt_launch_shape", "hogatt_step_plan_launch", "hogatt_append_launch",
            "hogatt_paged_q4_workspace_bytes", "hogatt_paged_q4_sdpa_launch", "hogatt_copy_to_blocks_q4_launch", "hogatt_copy_from_blocks_q4_launch",
            "hogatt_step_blocks_workspace_bytes", "hogatt_step_blocks_launch", "hogatt_compact_blocks_workspace_bytes",
@@ -125,6 +126,8 @@ def load() -> C.CDLL:
         lib.hogatt_paged_sdpa_launch.argtypes = [C.POINTER(PagedProblem), C.c_void_p]
         lib.hogatt_copy_to_blocks_launch.restype = C.c_int
         lib.hogatt_copy_to_blocks_launch.argtypes = [C.c_void_p] * 6 + [C.c_int32] * 8 + [C.c_void_p]
+        lib.hogatt_copy_to_blocks_rows_launch.restype = C.c_int
+        lib.hogatt_copy_to_blocks_rows_launch.argtypes = [C.c_void_p] * 7 + [C.c_int32] * 9 + [C.c_void_p]
         lib.hogatt_step_plan_launch.restype = C.c_int
         lib.hogatt_step_plan_launch.argtypes = [C.POINTER(StepPlan), C.c_void_p]
         lib.hogatt_append_launch.restype = C.c_int

@@ -35,6 +35,7 @@ _FUSED_PLANNED = torch.ops.libhogatt.hogwild_fused_planned.default
 _PAGED_SDPA = torch.ops.libhogatt.hogwild_paged_sdpa.default
 _VARLEN_PAGED_SDPA = torch.ops.libhogatt.hogwild_varlen_paged_sdpa.default
 _COPY_TO_BLOCKS = torch.ops.libhogatt.copy_to_blocks.default
+_COPY_TO_BLOCKS_NEW_ROWS = torch.ops.libhogatt.copy_to_blocks.new_rows
 _PAGED_SDPA_Q4 = torch.ops.libhogatt.hogwild_paged_sdpa_q4.default
 _VARLEN_PAGED_SDPA_Q4 = torch.ops.libhogatt.hogwild_varlen_paged_sdpa_q4.default
 _PAGED_SDPA_Q4_NEW = torch.ops.libhogatt.hogwild_paged_sdpa_q4.new
@@ -133,9 +134,13 @@ def hogwild_varlen_paged_sdpa(queries: torch.Tensor, locations: torch.Tensor, ke
 
 
 def copy_to_blocks(key_states: torch.Tensor, value_states: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
-                   block_table: torch.Tensor, seq_lengths: torch.Tensor) -> None:
+                   block_table: torch.Tensor, seq_lengths: torch.Tensor, *, new_rows: Optional[torch.Tensor] = None) -> None:
     """Append ``key_states / value_states [B,Hkv,S_new,E]`` to the paged caches at ``seq_lengths[b] + t``
-    (``src/binding.cu:370-371``)."""
+    (``src/binding.cu:370-371``).  Rows whose page the table does not name are dropped; ``new_rows [B]``: rows from there on stay out (what
+    :func:`step_blocks` returns as ``room``)."""
+    if new_rows is not None:
+        _COPY_TO_BLOCKS_NEW_ROWS(key_states.contiguous(), value_states.contiguous(), key_cache, value_cache, block_table, seq_lengths, new_rows)
+        return
     _COPY_TO_BLOCKS(key_states.contiguous(), value_states.contiguous(), key_cache, value_cache,
                     block_table, seq_lengths)
 
@@ -195,7 +200,8 @@ def copy_from_blocks_q4(key_cache: torch.Tensor, value_cache: torch.Tensor, key_
 
 
 # ---- the pages of a paged cache of any type (no counterpart in the reference) ------------------------------------------
-# ``block_refs[p]`` counts the block-table entries that name page ``p`` (plus what a caller adds to keep a page); 0: free.
+# ``block_refs[p]`` counts the block-table entries that name page ``p`` (plus what a caller adds to keep a page); 0: free.  A row without
+# pages has -1 in its table: append with ``new_rows=room``, and let queries over 16-bit pages see no further than ``lengths + room``.
 
 def step_blocks(block_refs: torch.Tensor, block_table: torch.Tensor, seq_lengths: torch.Tensor, caches: Sequence[torch.Tensor],
                 block_size: int, *, source: Optional[torch.Tensor] = None, new_tokens: Optional[torch.Tensor] = None,

@@ -1323,13 +1323,13 @@ int hogatt_paged_sdpa_launch(const hogatt_paged_problem* p, hogatt_stream_t stre
     return HOGATT_ERR_UNSUPPORTED_DTYPE;
 }
 
-int hogatt_copy_to_blocks_launch(const void* key_states, const void* value_states, void* key_cache, void* value_cache,
-                                 const int32_t* block_table, const int32_t* seq_lengths, int32_t B, int32_t Hkv,
-                                 int32_t S_new, int32_t E, int32_t Ev, int32_t block_size, int32_t max_blocks,
-                                 int32_t dtype, hogatt_stream_t stream_) {
+int hogatt_copy_to_blocks_rows_launch(const void* key_states, const void* value_states, void* key_cache, void* value_cache,
+                                      const int32_t* block_table, const int32_t* seq_lengths, const int32_t* new_rows,
+                                      int32_t B, int32_t Hkv, int32_t S_new, int32_t E, int32_t Ev, int32_t block_size,
+                                      int32_t max_blocks, int32_t num_blocks, int32_t dtype, hogatt_stream_t stream_) {
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
     if (!key_states || !value_states || !key_cache || !value_cache || !block_table || !seq_lengths) return HOGATT_ERR_NULL_POINTER;
-    if (B <= 0 || Hkv <= 0 || S_new < 0 || E <= 0 || Ev <= 0 || block_size <= 0 || max_blocks <= 0) return HOGATT_ERR_BAD_SHAPE;
+    if (B <= 0 || Hkv <= 0 || S_new < 0 || E <= 0 || Ev <= 0 || block_size <= 0 || max_blocks <= 0 || num_blocks <= 0) return HOGATT_ERR_BAD_SHAPE;
     if (dtype != HOGATT_F32 && dtype != HOGATT_F16 && dtype != HOGATT_BF16) return HOGATT_ERR_UNSUPPORTED_DTYPE;
     const int vec = 16 / (int)dtype_size(dtype);
     if (E % vec != 0 || Ev % vec != 0) return HOGATT_ERR_UNSUPPORTED_HEAD_DIM;
@@ -1342,17 +1342,25 @@ int hogatt_copy_to_blocks_launch(const void* key_states, const void* value_state
     cudaError_t err = cudaSuccess;
     switch (dtype) {
         case HOGATT_F32:
-            err = launch_kernel(copy_to_blocks_kernel<float>, dim3(blocks), dim3(256), 0, stream, (const float*)key_states, (const float*)value_states, (float*)key_cache, (float*)value_cache, block_table, seq_lengths, B, Hkv, S_new, E, Ev, block_size, max_blocks);
+            err = launch_kernel(copy_to_blocks_kernel<float>, dim3(blocks), dim3(256), 0, stream, (const float*)key_states, (const float*)value_states, (float*)key_cache, (float*)value_cache, block_table, seq_lengths, new_rows, B, Hkv, S_new, E, Ev, block_size, max_blocks, num_blocks);
             break;
         case HOGATT_F16:
-            err = launch_kernel(copy_to_blocks_kernel<__half>, dim3(blocks), dim3(256), 0, stream, (const __half*)key_states, (const __half*)value_states, (__half*)key_cache, (__half*)value_cache, block_table, seq_lengths, B, Hkv, S_new, E, Ev, block_size, max_blocks);
+            err = launch_kernel(copy_to_blocks_kernel<__half>, dim3(blocks), dim3(256), 0, stream, (const __half*)key_states, (const __half*)value_states, (__half*)key_cache, (__half*)value_cache, block_table, seq_lengths, new_rows, B, Hkv, S_new, E, Ev, block_size, max_blocks, num_blocks);
             break;
         default:
-            err = launch_kernel(copy_to_blocks_kernel<__nv_bfloat16>, dim3(blocks), dim3(256), 0, stream, (const __nv_bfloat16*)key_states, (const __nv_bfloat16*)value_states, (__nv_bfloat16*)key_cache, (__nv_bfloat16*)value_cache, block_table, seq_lengths, B, Hkv, S_new, E, Ev, block_size, max_blocks);
+            err = launch_kernel(copy_to_blocks_kernel<__nv_bfloat16>, dim3(blocks), dim3(256), 0, stream, (const __nv_bfloat16*)key_states, (const __nv_bfloat16*)value_states, (__nv_bfloat16*)key_cache, (__nv_bfloat16*)value_cache, block_table, seq_lengths, new_rows, B, Hkv, S_new, E, Ev, block_size, max_blocks, num_blocks);
             break;
     }
     HOGATT_CUDA_OK(err);
     return HOGATT_OK;
+}
+
+int hogatt_copy_to_blocks_launch(const void* key_states, const void* value_states, void* key_cache, void* value_cache,
+                                 const int32_t* block_table, const int32_t* seq_lengths, int32_t B, int32_t Hkv,
+                                 int32_t S_new, int32_t E, int32_t Ev, int32_t block_size, int32_t max_blocks,
+                                 int32_t dtype, hogatt_stream_t stream) {
+    return hogatt_copy_to_blocks_rows_launch(key_states, value_states, key_cache, value_cache, block_table, seq_lengths, nullptr, B, Hkv, S_new, E,
+                                             Ev, block_size, max_blocks, INT_MAX, dtype, stream);
 }
 
 int hogatt_fused_launch_gather(const hogatt_problem* p, const hogatt_peers* peers, hogatt_stream_t stream) {

@@ -590,10 +590,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
 // One 16-byte vector per thread; replaces copy_to_blocks_kernel (src/cache.cuh:6-49), where every
 // thread of a (S_new x head-size) block copies a whole row element by element.  A few KB in a decode step: launched beside
 // its predecessor, and its successor beside it (8 sequences of 16 K keys, with the attention call: 37.1 -> 35.0 us).
+// Rows t >= new_rows[b] (where given) and rows whose position has no page stay out: page bookkeeping leaves -1 in the table of a row
+// that found no pages, or that nobody took over.
 template <class T>
 __global__ void __launch_bounds__(256) copy_to_blocks_kernel(const T* k_states, const T* v_states, T* k_cache, T* v_cache,
-                                                             const int* block_table, const int* seq_lengths, int B, int Hkv, int S_new,
-                                                             int E, int Ev, int block_size, int max_blocks) {
+                                                             const int* block_table, const int* seq_lengths, const int* new_rows, int B, int Hkv,
+                                                             int S_new, int E, int Ev, int block_size, int max_blocks, int num_blocks) {
     constexpr int VEC = 16 / sizeof(T);
     const int kvr = E / VEC, vvr = Ev / VEC, per_row = kvr + vvr;
     const int64_t total = (int64_t)B * Hkv * S_new * per_row;
@@ -603,14 +605,17 @@ __global__ void __launch_bounds__(256) copy_to_blocks_kernel(const T* k_states, 
         const int64_t row = floor_div(i, per_row), bh = floor_div(row, S_new);
         const int c = (int)(i - row * per_row), t = (int)(row - bh * S_new);
         const int b = (int)floor_div(bh, Hkv), h = (int)(bh - (int64_t)b * Hkv);
-        const int pos = seq_lengths[b] + t;
-        const size_t blk = (size_t)block_table[(size_t)b * max_blocks + pos / block_size];
-        const size_t dst_row = (blk * Hkv + h) * block_size + pos % block_size;
+        // the row's bytes first: where they go takes two more round trips
         const size_t src_row = ((size_t)b * Hkv + h) * S_new + t;
-        if (c < kvr)
-            reinterpret_cast<int4*>(k_cache + dst_row * E)[c] = load_16(k_states + src_row * E + c * VEC);
-        else
-            reinterpret_cast<int4*>(v_cache + dst_row * Ev)[c - kvr] = load_16(v_states + src_row * Ev + (c - kvr) * VEC);
+        const int4 x = c < kvr ? load_16(k_states + src_row * E + c * VEC) : load_16(v_states + src_row * Ev + (c - kvr) * VEC);
+        if (new_rows && t >= new_rows[b]) continue;
+        const int pos = seq_lengths[b] + t, at = pos / block_size;
+        if (pos < 0 || at >= max_blocks) continue;
+        const int blk = block_table[(size_t)b * max_blocks + at];
+        if (blk < 0 || blk >= num_blocks) continue;
+        const size_t dst_row = ((size_t)blk * Hkv + h) * block_size + (pos - at * block_size);
+        if (c < kvr) reinterpret_cast<int4*>(k_cache + dst_row * E)[c] = x;
+        else reinterpret_cast<int4*>(v_cache + dst_row * Ev)[c - kvr] = x;
     }
 }
 

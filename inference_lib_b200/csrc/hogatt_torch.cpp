@@ -314,8 +314,8 @@ void hogwild_varlen_paged_attention(at::Tensor& out, double scale, const at::Ten
     run_paged(out, scale, locations, queries, fragment_lengths, key_cache, value_cache, block_table, &cu_seqlens_q);
 }
 
-void copy_to_blocks(const at::Tensor& key_states, const at::Tensor& value_states, at::Tensor& key_cache,
-                    at::Tensor& value_cache, const at::Tensor& block_table, const at::Tensor& seq_lengths) {
+void run_copy_to_blocks(const at::Tensor& key_states, const at::Tensor& value_states, at::Tensor& key_cache, at::Tensor& value_cache,
+                        const at::Tensor& block_table, const at::Tensor& seq_lengths, const at::Tensor* new_rows) {
     TORCH_CHECK(key_states.is_cuda(), "libhogatt: tensors must live on a CUDA device");
     const c10::cuda::CUDAGuard guard(key_states.device());
     for (const at::Tensor* t : {&key_states, &value_states, &block_table, &seq_lengths})
@@ -338,13 +338,25 @@ void copy_to_blocks(const at::Tensor& key_states, const at::Tensor& value_states
     TORCH_CHECK_EQ(value_cache.size(2), key_cache.size(2));
     TORCH_CHECK_EQ(block_table.size(0), B);
     TORCH_CHECK_EQ(seq_lengths.size(0), B);
+    TORCH_CHECK(!new_rows || (new_rows->device() == key_states.device() && new_rows->dim() == 1 && new_rows->size(0) == B &&
+                              new_rows->is_contiguous() && new_rows->scalar_type() == at::kInt),
+                "copy_to_blocks: new_rows must be contiguous int32 [B]");
+    const int num_blocks = (int)std::min<int64_t>({key_cache.size(0), value_cache.size(0), INT32_MAX});
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream();
-    check_status(hogatt_copy_to_blocks_launch(key_states.const_data_ptr(), value_states.const_data_ptr(), key_cache.data_ptr(),
-                                              value_cache.data_ptr(), block_table.const_data_ptr<int>(),
-                                              seq_lengths.const_data_ptr<int>(), B, Hkv, S_new, E, Ev, (int)key_cache.size(2),
-                                              (int)block_table.size(1), dtype_code(key_states),
-                                              reinterpret_cast<hogatt_stream_t>(stream)),
+    check_status(hogatt_copy_to_blocks_rows_launch(key_states.const_data_ptr(), value_states.const_data_ptr(), key_cache.data_ptr(),
+                                                   value_cache.data_ptr(), block_table.const_data_ptr<int>(), seq_lengths.const_data_ptr<int>(),
+                                                   new_rows ? new_rows->const_data_ptr<int>() : nullptr, B, Hkv, S_new, E, Ev,
+                                                   (int)key_cache.size(2), (int)block_table.size(1), num_blocks, dtype_code(key_states),
+                                                   reinterpret_cast<hogatt_stream_t>(stream)),
                  "copy_to_blocks");
+}
+void copy_to_blocks(const at::Tensor& key_states, const at::Tensor& value_states, at::Tensor& key_cache,
+                    at::Tensor& value_cache, const at::Tensor& block_table, const at::Tensor& seq_lengths) {
+    run_copy_to_blocks(key_states, value_states, key_cache, value_cache, block_table, seq_lengths, nullptr);
+}
+void copy_to_blocks_new_rows(const at::Tensor& key_states, const at::Tensor& value_states, at::Tensor& key_cache, at::Tensor& value_cache,
+                             const at::Tensor& block_table, const at::Tensor& seq_lengths, const at::Tensor& new_rows) {
+    run_copy_to_blocks(key_states, value_states, key_cache, value_cache, block_table, seq_lengths, &new_rows);
 }
 
 // --- the steps either side of the op (FragmentCache.update) -------------------------------------------------
@@ -850,6 +862,9 @@ TORCH_LIBRARY(libhogatt, m) {
           "Tensor(d!) status) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
     m.def("fragment_step_plan(Tensor order, Tensor fragment_lengths, Tensor inv_freq, Tensor(a!) locations, Tensor(b!) cosines, "
           "Tensor(c!) sines, float attention_scaling, int round_tables_to) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
+    // (rows from new_rows[b] on stay out)
+    m.def("copy_to_blocks.new_rows(Tensor key_states, Tensor value_states, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor block_table, "
+          "Tensor seq_lengths, Tensor new_rows) -> ()", tags, torch::_RegisterOrVerify::REGISTER);
     // a paged cache in 4 bits
     m.def("hogwild_paged_sdpa_q4(Tensor(a!) output, float scale, Tensor locations, Tensor queries, Tensor fragment_lengths, Tensor key_cache, "
           "Tensor value_cache, Tensor key_scales, Tensor value_scales, Tensor block_table, float key_unit, float value_unit, "
@@ -890,6 +905,7 @@ TORCH_LIBRARY_IMPL(libhogatt, CUDA, m) {
     m.impl("hogwild_fused", hogwild_fused);
     m.impl("hogwild_paged_sdpa", hogwild_paged_attention);
     m.impl("copy_to_blocks", copy_to_blocks);
+    m.impl("copy_to_blocks.new_rows", copy_to_blocks_new_rows);
     m.impl("hogwild_varlen_paged_sdpa", hogwild_varlen_paged_attention);
     m.impl("hogwild_fused_planned", hogwild_fused_planned);
     m.impl("fragment_append", fragment_append);

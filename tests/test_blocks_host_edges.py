@@ -1,0 +1,26 @@
+"""What the C ABI refuses of the calls that go with page bookkeeping, without a GPU."""
+import pytest
+
+from inference_lib_b200 import _build, _cabi
+
+OK, NULL, SHAPE, HEAD, DTYPE, ALIGN = 0, -1, -2, -3, -4, -6
+
+
+@pytest.fixture(scope="module")
+def lib():
+    _build.build_cabi()
+    return _cabi.load()
+
+
+@pytest.mark.parametrize("change,rc", [
+    ({}, OK), ({0: None}, NULL), ({4: None}, NULL), ({5: None}, NULL), ({6: None}, OK), ({7: 0}, SHAPE), ({9: -1}, SHAPE), ({14: 0}, SHAPE), ({14: -3}, SHAPE),
+    ({15: 7}, DTYPE), ({10: 60}, HEAD), ({1: 4104}, ALIGN),
+])
+def test_append_of_rows_refuses(lib, change, rc):
+    #         states, caches, table, lengths, new_rows, B, Hkv, S, E, Ev, block size, table width, blocks, dtype
+    args = [4096] * 7 + [2, 2, 0, 64, 64, 16, 4, 9, _cabi.BF16, None]
+    for i, x in change.items():
+        args[i] = x
+    if rc not in (OK, SHAPE):
+        args[9] = 3
+    assert lib.hogatt_copy_to_blocks_rows_launch(*args) == rc
