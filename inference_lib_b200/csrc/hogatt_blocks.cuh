@@ -37,7 +37,7 @@ struct StepBlocksArgs {
     int* status;
 };
 // Workspace, ints: [0] copies listed, [1 .. 8] free pages per CTA, [16 + 3 w] pages of row w that are kept x 2 + takes a copy, its last page,
-// pages that rows before it need; behind them one entry more of the last kind (the total); then the list of copies (from, to).
+// pages that rows before it need (INT_MAX: that or more); behind them one entry more of the last kind (the total); then the list of copies (from, to).
 constexpr int kStepHead = 16;
 __host__ __device__ inline int64_t step_blocks_pairs(int64_t rows) { return kStepHead + 3 * (rows + 1); }
 __host__ __device__ inline int64_t step_blocks_ints(int64_t rows) { return step_blocks_pairs(rows) + 2 * rows; }
@@ -116,7 +116,8 @@ __global__ void __launch_bounds__(kBlocksThreads, 1) step_blocks_kernel(const __
     // ---- 2: what every row needs (CTA 0), free pages of every share ----
     __shared__ __align__(16) int last_of[kBlocksThreads];
     if (rank == 0) {
-        int before = 0;
+        // (65,536 rows may ask for more pages than 32 bits count; more than the pool has is all the same)
+        int64_t before = 0;
         for (int w0 = 0; w0 < a.rows_out; w0 += kBlocksThreads) {
             const int w = w0 + tid;
             StepRow r = {};
@@ -147,15 +148,15 @@ __global__ void __launch_bounds__(kBlocksThreads, 1) step_blocks_kernel(const __
                 }
             }
             const int need = w < a.rows_out ? r.want - r.kept + copy : 0;
-            int total;
-            const int at = block_exclusive(need, &total);
+            int64_t total;
+            const int64_t at = block_exclusive((int64_t)need, &total);
             if (w < a.rows_out) {
                 __stcg(rows_ws + 3 * w, r.kept * 2 + copy);
-                __stcg(rows_ws + 3 * w + 2, before + at);
+                __stcg(rows_ws + 3 * w + 2, (int)min(before + at, (int64_t)INT_MAX));
             }
             before += total;
         }
-        if (tid == 0) __stcg(rows_ws + 3 * a.rows_out + 2, before);
+        if (tid == 0) __stcg(rows_ws + 3 * a.rows_out + 2, (int)min(before, (int64_t)INT_MAX));
     }
     int mine = 0;
     for (int p = begin + tid; p < end; p += kBlocksThreads) mine += __ldcg(a.refs_out + p) == 0;
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(kBlocksThreads, 1) step_blocks_kernel(const __
         const int p = p0 + tid;
         const bool unused = p < end && __ldcg(a.refs_out + p) == 0;
         int total;
-        const int k = base + block_exclusive(unused, &total);
+        const int k = base + block_exclusive((int)unused, &total);
         base += total;
         if (!unused || k >= needed) continue;
         int lo = 0, hi = a.rows_out;                      // the row: the last one whose predecessors need at most k
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(kBlocksThreads, 1) compact_blocks_kernel(const
         const int refs = p < end ? a.refs_in[p] : 0;
         const bool is_hole = p < end && p < n && refs == 0, is_mover = p < end && p >= n && refs != 0;
         int th, tm;
-        const int h = hole + block_exclusive(is_hole, &th), m = mover + block_exclusive(is_mover, &tm);
+        const int h = hole + block_exclusive((int)is_hole, &th), m = mover + block_exclusive((int)is_mover, &tm);
         hole += th;
         mover += tm;
         if (is_hole) __stcg(pairs + 2 * h + 1, p);

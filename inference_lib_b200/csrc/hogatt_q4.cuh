@@ -84,23 +84,24 @@ __device__ __forceinline__ long long paged_row_at(const int* table, int pos, int
 }
 
 // exclusive prefix of `x` over the CTA's threads; the total comes back in *total.  Called by all threads.
-__device__ __forceinline__ int block_exclusive(int x, int* total) {
-    __shared__ int warp_sum[32];
+template <class I>
+__device__ __forceinline__ I block_exclusive(I x, I* total) {
+    __shared__ I warp_sum[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int inc = x;
+    I inc = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, inc, o);
+        const I y = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += y;
     }
     __syncthreads();                                      // (the array may still be in use from the last call)
     if (lane == 31) warp_sum[warp] = inc;
     __syncthreads();
     if (warp == 0) {
-        int s = lane < (int)(blockDim.x >> 5) ? warp_sum[lane] : 0;
+        I s = lane < (int)(blockDim.x >> 5) ? warp_sum[lane] : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, s, o);
+            const I y = __shfl_up_sync(0xffffffffu, s, o);
             if (lane >= o) s += y;
         }
         warp_sum[lane] = s;

@@ -24,3 +24,9 @@ def test_append_of_rows_refuses(lib, change, rc):
     if rc not in (OK, SHAPE):
         args[9] = 3
     assert lib.hogatt_copy_to_blocks_rows_launch(*args) == rc
+
+
+def test_a_pool_beyond_the_count_of_pages_is_refused(lib):
+    import ctypes as C
+    from tests.test_q4_host import _blocks
+    assert lib.hogatt_step_blocks_launch(C.byref(_blocks(_cabi.StepBlocks, num_blocks=2 ** 31 - 1)), None) == -10

@@ -84,3 +84,16 @@ def test_a_batch_over_sixteen_bit_pages(A, dtype, G, E, bs):
             limit = half * want.abs() + (half + 300 * 2.0 ** -23) * (p[:, None] @ vv.abs())[:, 0] * 2
             assert bool(((got[w, :, 0] - want).abs() <= limit).all())
     assert ran_dry >= 2
+
+
+def test_needs_that_32_bits_do_not_hold(A):
+    """65,536 rows that together ask for 2^31 pages and more: those in front get theirs, from the first that finds too few on nobody does."""
+    rows, width, blocks, bs = 65536, 32769, 70000, 4
+    table = torch.full((rows, width), -1, dtype=torch.int32, device=DEV)
+    refs, lengths = ints([0] * blocks), ints([0] * rows)
+    new = torch.full((rows,), width * bs, dtype=torch.int32, device=DEV)
+    st, room = status(), torch.empty(rows, dtype=torch.int32, device=DEV)
+    A.step_blocks(refs, table, lengths, [], bs, new_tokens=new, out=(refs, table, lengths, room), status=st)
+    assert int(st) == 512 and room[:2].tolist() == [width * bs] * 2 and not bool(room[2:].any())
+    assert torch.equal(table[:2].flatten(), torch.arange(2 * width, dtype=torch.int32, device=DEV)) and bool((table[2:] == -1).all())
+    assert bool((refs[:2 * width] == 1).all()) and not bool(refs[2 * width:].any())
