@@ -543,6 +543,7 @@ int hogatt_step_blocks_launch(const hogatt_step_blocks* p, hogatt_stream_t strea
     if (p->num_blocks <= 0 || p->block_size <= 0 || p->max_blocks <= 0 || p->rows_in <= 0 || p->rows_out <= 0 || (!p->source && p->rows_out != p->rows_in))
         return HOGATT_ERR_BAD_SHAPE;
     if (p->rows_in > HOGATT_MAX_BLOCK_ROWS || p->rows_out > HOGATT_MAX_BLOCK_ROWS || p->num_blocks == INT_MAX) return HOGATT_ERR_TOO_LARGE;
+    if (p->max_blocks >= 1 << 30) return HOGATT_ERR_TOO_LARGE;      // (a row's pages travel twice themselves, with a bit behind)
     if (!p->refs_in || !p->table_in || !p->lengths_in || !p->refs_out || !p->table_out || !p->lengths_out || !p->room || !p->workspace)
         return HOGATT_ERR_NULL_POINTER;
     // rows that change places cannot be taken over in place

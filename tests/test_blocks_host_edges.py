@@ -30,3 +30,11 @@ def test_a_pool_beyond_the_count_of_pages_is_refused(lib):
     import ctypes as C
     from tests.test_q4_host import _blocks
     assert lib.hogatt_step_blocks_launch(C.byref(_blocks(_cabi.StepBlocks, num_blocks=2 ** 31 - 1)), None) == -10
+
+
+@pytest.mark.parametrize("width,rc", [(2 ** 30 - 1, -7), (2 ** 30, -10), (2 ** 31 - 1, -10)])
+def test_tables_wider_than_a_row_counts_are_refused(lib, width, rc):
+    """(The one below is refused for the workspace it is given.)"""
+    import ctypes as C
+    from tests.test_q4_host import _blocks
+    assert lib.hogatt_step_blocks_launch(C.byref(_blocks(_cabi.StepBlocks, max_blocks=width, workspace_bytes=8)), None) == rc
