@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kBlocksThreads, 1) step_blocks_kernel(const __
         const bool served = __ldcg(rows_ws + 3 * (w + 1) + 2) <= free_all && !r.over;
         if (!served && !r.over && r.add > 0) flags |= STATUS_NO_BLOCKS;
         a.room[w] = served ? r.add : 0;
-        if (a.lengths_out != a.lengths_in) a.lengths_out[w] = r.length;
+        a.lengths_out[w] = r.length;                      // (in place too: a length below zero is none)
     }
     if (flags && a.status) atomicOr(a.status, flags);
 }

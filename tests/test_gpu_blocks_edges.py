@@ -97,3 +97,10 @@ def test_needs_that_32_bits_do_not_hold(A):
     assert int(st) == 512 and room[:2].tolist() == [width * bs] * 2 and not bool(room[2:].any())
     assert torch.equal(table[:2].flatten(), torch.arange(2 * width, dtype=torch.int32, device=DEV)) and bool((table[2:] == -1).all())
     assert bool((refs[:2 * width] == 1).all()) and not bool(refs[2 * width:].any())
+
+
+def test_a_length_below_zero_in_place(A):
+    """Is none, also where the lengths are written where they are read."""
+    rng = np.random.default_rng(12)
+    refs, table = pool(rng, 20, 4, 5, [7, 0, 9])
+    run_step(A, refs, table, [7, -3, 9], None, [1, 2, 0], 4, some_caches(rng, 20), out=lambda a: (a[0], a[1], a[2], ints([7] * 3)))
