@@ -424,7 +424,8 @@ int hogatt_paged_q4_sdpa_launch(const hogatt_paged_q4_problem* x, hogatt_stream_
     a.block_size = p->block_size; a.max_blocks = p->max_blocks_per_seq;
     a.tokens_per_group = pl.tokens_per_group; a.head_blocks = pl.head_blocks; a.groups_bound = pl.groups_bound;
     a.splits = pl.splits;
-    a.l2scale = (float)((double)p->scale * 1.4426950408889634 * x->key_unit);
+    // (a scale that is no number: every score is inf - inf or 0 * inf, NaN)
+    a.l2scale = std::isfinite(p->scale) ? (float)((double)p->scale * 1.4426950408889634 * x->key_unit) : NAN;
     if (packed) {     // q [F,total_q,Hq,E], out [total_q,Hq,Ev], loc [F,total_q], len [F,W]; s is the packed token index
         a.q_f = (long long)a.total_q * p->Hq * p->E; a.q_w = 0; a.q_s = (long long)p->Hq * p->E; a.q_h = p->E;
         a.o_w = 0; a.o_s = (long long)p->Hq * p->Ev; a.o_h = p->Ev;

@@ -442,14 +442,15 @@ __global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel
                 }
                 float mine = fabsf(a.l2scale);
                 uint32_t* r = reinterpret_cast<uint32_t*>(raw);
-                // a row with an infinity or a NaN becomes NaN; the factor stays a number, so that a key which the row does not see is -inf times it
+                // a row with an infinity or a NaN becomes NaN (every row, if the scale is one); the factor stays a number, so that a key which the
+                // row does not see is -inf times it
                 constexpr bool half = std::is_same<T, __half>::value;
                 uint32_t top = 0;                         // the largest magnitude's bits, in the upper half
 #pragma unroll
                 for (int k = 0; k < CPT / 2; ++k) top = max(top, max(r[k] & 0x7fff0000u, (r[k] & 0x7fffu) << 16));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const bool finite = top < (half ? 0x7c000000u : 0x7f800000u);
+                const bool finite = top < (half ? 0x7c000000u : 0x7f800000u) && fabsf(a.l2scale) <= FLT_MAX;
                 if constexpr (half) {
 #pragma unroll
                     for (int k = 0; k < CPT / 2; ++k) r[k] = finite ? r[k] : 0x7fff7fffu;
@@ -463,7 +464,7 @@ __global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel
                         r[k] = pack2<__half>(__low2float(v) * up, __high2float(v) * up);
                     }
                 }
-                mine = fmaxf(mine, FLT_MIN);              // (a masked score is -inf and has to stay it; scores this small are none)
+                mine = fminf(fmaxf(mine, FLT_MIN), FLT_MAX);      // (a masked score is -inf and has to stay it; scores this small are none)
                 if (a.l2scale < 0.f) {                    // (the row's maximum is taken before the factor)
 #pragma unroll
                     for (int k = 0; k < CPT / 2; ++k) r[k] ^= 0x80008000u;
