@@ -31,6 +31,7 @@
 // CTAs and re-reads the KV once per (worker, token) on CUDA cores (src/kernels/kernel_v21.cuh:62-66,957-964).
 #pragma once
 #include <cuda.h>
+#include <float.h>
 #include <limits.h>
 
 #include <type_traits>
@@ -105,7 +106,7 @@ struct DenseArgs {
     // Pages in 4 bits (hogatt_q4_dense.cuh): [0] keys, [1] values.
     const unsigned char* codes[2];
     const unsigned char* scales[2];
-    const float* factor;   // [total_q, Hq]: what a row's products are multiplied with, or nullptr: l2scale for all
+    const float* factor;   // [F, total_q, Hq]: what a row's products are multiplied with, or nullptr: l2scale for all
     int num_blocks;
     int most_keys;         // paged: no sequence is taken for longer
     uint32_t block_mul, block_shift;       // key / block_size = (umulhi(key, mul) + key) >> shift
@@ -986,14 +987,20 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
                 any = false;
                 if constexpr (Q4) {
                     odd_groups = 0;
-                    if (a.factor) {
-                        scale2 = id.valid ? a.factor[(size_t)id.s * a.Hq + d.h * a.G + id.g] : 1.f;
-                        grow_by = 8.f / scale2;
-                    }
                 }
             }
             int lim = 0;                                       // keys of the fragment that the row sees: [0, lim)
             if (id.valid) lim = min(dense_location<PAGED>(a, d.f, id), dense_length<PAGED>(a, d.f, id.w) - 1) + 1;
+            if constexpr (Q4) {
+                if (a.factor && lim > 0) {                     // (a fragment that the row does not see leaves everything as it is)
+                    const float mine = a.factor[((size_t)d.f * a.total_q + id.s) * a.Hq + d.h * a.G + id.g];
+                    // what the fragments before this one have left, as a product of this one's; as long as their powers of two are
+                    // 2^126 apart at most it is off by 2^-23 in the exponent, and beyond that one of the two counts for nothing
+                    if (m_run != -INFINITY && mine != scale2) m_run = fminf(fmaxf(m_run * scale2 / mine, -FLT_MAX), FLT_MAX);
+                    scale2 = mine;
+                    grow_by = 8.f / mine;
+                }
+            }
             const int stride = d.single() ? 2 : 1, t1 = d.single() ? d.t1 : min(d.t1, ((g ? d.vis1 : d.vis0) + kDenseTile - 1) / kDenseTile);
 #pragma unroll 1
             for (int t = d.t0 + (d.single() ? g : 0); t < t1; t += stride) {

@@ -113,8 +113,8 @@ int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
         pl->ctas = std::min(sms, kDenseMaxCtas);
         pl->w = carve_dense_plan(pl->blocks, p->Hkv, p->F, pl->ctas);
         pl->queries = pl->w.total;
-        const size_t rows = (size_t)p->total_q_tokens * p->Hq;
-        pl->factor = pl->queries + (p->dtype == HOGATT_BF16 ? align_up(rows * p->F * 128 * sizeof(__half), 256) : 0);
+        const size_t rows = (size_t)p->total_q_tokens * p->Hq * p->F;
+        pl->factor = pl->queries + (p->dtype == HOGATT_BF16 ? align_up(rows * 128 * sizeof(__half), 256) : 0);
         pl->total = pl->factor + align_up(rows * sizeof(float), 256);
         return HOGATT_OK;
     }
@@ -298,9 +298,9 @@ int launch_q4_dense(const hogatt_paged_q4_problem* x, const Q4Plan& pl, int dev,
     if (rc != HOGATT_OK) return rc;
     HOGATT_CUDA_OK(launch_kernel(dense_plan_kernel<true>, dim3(1), dim3(kDensePlanThreads), 0, stream, d));
     if constexpr (convert) {
-        const int rows = p->total_q_tokens * p->Hq;
+        const int rows = p->F * p->total_q_tokens * p->Hq;
         HOGATT_CUDA_OK(launch_kernel(q4_dense_queries_kernel, dim3((rows + 7) / 8), dim3(256), 0, stream, static_cast<const __nv_bfloat16*>(p->queries),
-                                     reinterpret_cast<__half*>(ws + pl.queries), reinterpret_cast<float*>(ws + pl.factor), p->F, rows, d.l2scale));
+                                     reinterpret_cast<__half*>(ws + pl.queries), reinterpret_cast<float*>(ws + pl.factor), rows, d.l2scale));
     }
     static std::atomic<size_t> granted[kMaxDevices];
     constexpr size_t smem = DenseCfgOf<true>::OFF_END;

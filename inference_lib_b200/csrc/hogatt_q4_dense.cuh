@@ -11,7 +11,7 @@
 // Slower: four unpacking warps of 24 (registers spill: 220 us); a third one for a quarter of both tiles, both products issued by one warp (219 us).
 // 96 registers for every thread: nothing is left to take from the other warps.
 //
-// fp16 for both products: six significant bits times a probability; bf16 queries become fp16 once per call, a power of two per (token, head)
+// fp16 for both products: six significant bits times a probability; bf16 queries become fp16 once per call, a power of two per row
 // taken out (q4_dense_queries_kernel), which the softmax multiplies back in.
 //
 // Values that are not numbers are stored as zeros, keys without a page as zeros too; what is special about a tile travels to the softmax
@@ -153,28 +153,23 @@ __device__ __forceinline__ uint32_t q4_odd_groups(const DenseArgs& a, int w, int
     return odd;
 }
 
-// bf16 queries as fp16, each (token, head)'s largest finite magnitude (over the fragments) brought to [2^14, 2^15); factor: what brings its
-// scores back, with the scale.  A fragment's row with an infinity or a NaN becomes NaN.  One warp per (token, head), four channels per lane.  It
-// starts beside the plan kernel, which is behind everything that may still write the queries, and ends after it.
-__global__ void __launch_bounds__(256) q4_dense_queries_kernel(const __nv_bfloat16* q, __half* out, float* factor, int F, int rows, float l2scale) {
+// bf16 queries as fp16, each row's (fragment, token, head) largest magnitude brought to [2^14, 2^15); factor: what brings its scores back, with the
+// scale.  (One power of two for all fragments would be the largest one's, also of a fragment that the row does not see, where anything may stand.)
+// A row with an infinity or a NaN becomes NaN.  One warp per row, four channels per lane.  It starts beside the plan kernel, which is behind
+// everything that may still write the queries, and ends after it.
+__global__ void __launch_bounds__(256) q4_dense_queries_kernel(const __nv_bfloat16* q, __half* out, float* factor, int rows, float l2scale) {
     const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row < rows) {
-        auto load = [&](int f) { return *reinterpret_cast<const uint2*>(q + ((size_t)f * rows + row) * 128 + lane * 4); };
-        auto largest = [](uint2 v) { return max(max(v.x & 0x7fff0000u, (v.x & 0x7fffu) << 16), max(v.y & 0x7fff0000u, (v.y & 0x7fffu) << 16)); };
-        uint32_t top = 0;
-        for (int f = 0; f < F; ++f) {
-            const uint32_t mine = __reduce_max_sync(0xffffffffu, largest(load(f)));
-            if (mine < 0x7f800000u) top = max(top, mine);
-        }
-        const int e = min(120, 14 - ((int)(top >> 23) - 127));
+        const uint2 x = *reinterpret_cast<const uint2*>(q + (size_t)row * 128 + lane * 4);
+        const uint32_t mine = max(max(x.x & 0x7fff0000u, (x.x & 0x7fffu) << 16), max(x.y & 0x7fff0000u, (x.y & 0x7fffu) << 16));
+        const uint32_t top = __reduce_max_sync(0xffffffffu, mine);
+        const bool finite = top < 0x7f800000u;
+        const int e = finite ? min(120, 14 - ((int)(top >> 23) - 127)) : 0;
         if (lane == 0) factor[row] = fmaxf(l2scale * __int_as_float((127 - e) << 23), 1e-36f);
-        for (int f = 0; f < F; ++f) {
-            const uint2 x = load(f);
-            const float up = __any_sync(0xffffffffu, largest(x) >= 0x7f800000u) ? NAN : __int_as_float((e + 127) << 23);
-            const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(&x);
-            *reinterpret_cast<uint2*>(out + ((size_t)f * rows + row) * 128 + lane * 4) =
-                make_uint2(pack2<__half>(__low2float(v[0]) * up, __high2float(v[0]) * up), pack2<__half>(__low2float(v[1]) * up, __high2float(v[1]) * up));
-        }
+        const float up = finite ? __int_as_float((e + 127) << 23) : NAN;
+        const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(&x);
+        *reinterpret_cast<uint2*>(out + (size_t)row * 128 + lane * 4) =
+            make_uint2(pack2<__half>(__low2float(v[0]) * up, __high2float(v[0]) * up), pack2<__half>(__low2float(v[1]) * up, __high2float(v[1]) * up));
     }
     pdl_wait();
     pdl_trigger();

@@ -42,3 +42,24 @@ def test_a_scale_that_is_no_number(A, dtype, E, G, scale, kernel):
     wide[:, :4] = table
     got, exact = paged(A, q, loc, torch.tensor([[50, 50]], dtype=torch.int32), cache, wide, scale, cu=torch.tensor([0, 150, 151], dtype=torch.int32), kernel=kernel)
     q4_util.check(got, exact)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_fragments_whose_queries_differ_in_size(A, dtype, kernel):
+    """What a row holds for a fragment that it does not see does not reach what it sees, however large; and where it sees both, each counts as it is."""
+    cache, gen = small_cache(43, 24, 2, 16, 128)
+    table = torch.arange(24, dtype=torch.int32).reshape(2, 12)
+    T, cu = 200, torch.tensor([0, 199, 200], dtype=torch.int32)
+    large = 1e30 if dtype == torch.bfloat16 else 6e4
+    q = torch.randn(3, T, 8, 128, generator=gen)
+    loc = torch.from_numpy(np.random.default_rng(43).integers(-1, 190, (3, T)).astype(np.int32))
+    lens = torch.tensor([[192, 192], [192, 0], [150, 192]], dtype=torch.int32)
+    blind = torch.arange(T) % 3 == 0
+    loc[0, blind], q[0, blind] = -1, large                       # in front of what it sees
+    loc[2, 50:60], q[2, 50:60] = -5, -large                      # behind it
+    q[1, 199] = large                                            # a length of zero
+    q[1, 100:110], q[2, 100:110] = q[1, 100:110] * 2.0 ** -9, q[2, 100:110] * 2.0 ** 2       # seen, of different sizes
+    got, exact = paged(A, q.to(dtype), loc, lens, cache, table, 128 ** -0.5, cu=cu, kernel=kernel)
+    # (`large` stands behind no visible key: the bound on the scores is that of the others)
+    q4_util.check(got, exact)
