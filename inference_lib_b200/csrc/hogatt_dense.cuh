@@ -106,7 +106,7 @@ struct DenseArgs {
     // Pages in 4 bits (hogatt_q4_dense.cuh): [0] keys, [1] values.
     const unsigned char* codes[2];
     const unsigned char* scales[2];
-    const float* factor;   // [F, total_q, Hq]: what a row's products are multiplied with, or nullptr: l2scale for all
+    const float* factor;   // [F, total_q, Hq]: what a row's products are multiplied with
     int num_blocks;
     int most_keys;         // paged: no sequence is taken for longer
     uint32_t block_mul, block_shift;       // key / block_size = (umulhi(key, mul) + key) >> shift
@@ -360,8 +360,9 @@ __global__ void __launch_bounds__(kDensePlanThreads) dense_plan_kernel(const __g
     // The rotation kernel writes nothing that is read here.  It starts at once and makes the loads below slower, but its own
     // time is what the attention kernel waits for (let go behind them it began 4 us later: 4,000 tokens 25 -> 15 us to the end
     // of both, together with end_after_predecessor).  A packed call has no rotation: the attention kernel is let in behind the
-    // loads (0.2 us of every such call: 512 tokens of 2,000 keys 39.3 us with its CTAs there before, 39.1 now).
-    if constexpr (!PAGED) pdl_trigger();
+    // loads (0.2 us of every such call: 512 tokens of 2,000 keys 39.3 us with its CTAs there before, 39.1 now).  Over 4-bit pages the pass
+    // over the queries comes next, at once like the rotation.
+    if (!PAGED || a.factor) pdl_trigger();
     // exclusive prefix of one value per thread over the CTA; *total gets the sum
     auto scan = [&](long long v, long long* total) {
         long long x = v;
@@ -987,15 +988,18 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
                 any = false;
                 if constexpr (Q4) {
                     odd_groups = 0;
+                    scale2 = a.l2scale;                        // (of a row that sees nothing: a number)
+                    grow_by = 8.f / scale2;
                 }
             }
             int lim = 0;                                       // keys of the fragment that the row sees: [0, lim)
             if (id.valid) lim = min(dense_location<PAGED>(a, d.f, id), dense_length<PAGED>(a, d.f, id.w) - 1) + 1;
             if constexpr (Q4) {
-                if (a.factor && lim > 0) {                     // (a fragment that the row does not see leaves everything as it is)
+                if (lim > 0) {                                 // (a fragment that the row does not see leaves everything as it is)
                     const float mine = a.factor[((size_t)d.f * a.total_q + id.s) * a.Hq + d.h * a.G + id.g];
                     // what the fragments before this one have left, as a product of this one's; as long as their powers of two are
-                    // 2^126 apart at most it is off by 2^-23 in the exponent, and beyond that one of the two counts for nothing
+                    // 2^126 apart at most it is off by 2^-23 in the exponent, and beyond that one of the two counts for nothing.  (NaN: a query
+                    // that is no number; every probability of the row becomes NaN.)
                     if (m_run != -INFINITY && mine != scale2) m_run = fminf(fmaxf(m_run * scale2 / mine, -FLT_MAX), FLT_MAX);
                     scale2 = mine;
                     grow_by = 8.f / mine;

@@ -285,11 +285,8 @@ int launch_q4_dense(const hogatt_paged_q4_problem* x, const Q4Plan& pl, int dev,
     d.block_shift = by_block.shift;
     d.out_scale = x->value_unit;
     constexpr bool convert = std::is_same<T, __nv_bfloat16>::value;
-    const void* q = p->queries;
-    if (convert) {
-        d.factor = reinterpret_cast<float*>(ws + pl.factor);
-        q = ws + pl.queries;
-    }
+    d.factor = reinterpret_cast<float*>(ws + pl.factor);
+    const void* const q = convert ? ws + pl.queries : p->queries;
     DenseMaps maps;
     memset(&maps, 0, sizeof(maps));
     const cuuint64_t qdims[5] = {128, (cuuint64_t)d.G, (cuuint64_t)d.Hkv, (cuuint64_t)d.total_q, (cuuint64_t)d.F};
@@ -297,11 +294,9 @@ int launch_q4_dense(const hogatt_paged_q4_problem* x, const Q4Plan& pl, int dev,
     rc = encode_map(&maps.q, q, HOGATT_F16, 5, qdims, qbox);
     if (rc != HOGATT_OK) return rc;
     HOGATT_CUDA_OK(launch_kernel(dense_plan_kernel<true>, dim3(1), dim3(kDensePlanThreads), 0, stream, d));
-    if constexpr (convert) {
-        const int rows = p->F * p->total_q_tokens * p->Hq;
-        HOGATT_CUDA_OK(launch_kernel(q4_dense_queries_kernel, dim3((rows + 7) / 8), dim3(256), 0, stream, static_cast<const __nv_bfloat16*>(p->queries),
-                                     reinterpret_cast<__half*>(ws + pl.queries), reinterpret_cast<float*>(ws + pl.factor), rows, d.l2scale));
-    }
+    const int rows = p->F * p->total_q_tokens * p->Hq;
+    HOGATT_CUDA_OK(launch_kernel(q4_dense_queries_kernel<T>, dim3((rows + 7) / 8), dim3(256), 0, stream, static_cast<const T*>(p->queries),
+                                 reinterpret_cast<__half*>(ws + pl.queries), reinterpret_cast<float*>(ws + pl.factor), rows, d.l2scale));
     static std::atomic<size_t> granted[kMaxDevices];
     constexpr size_t smem = DenseCfgOf<true>::OFF_END;
     if (smem > (size_t)smem_optin) return HOGATT_ERR_CUDA;

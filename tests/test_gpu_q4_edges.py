@@ -63,3 +63,28 @@ def test_fragments_whose_queries_differ_in_size(A, dtype, kernel):
     got, exact = paged(A, q.to(dtype), loc, lens, cache, table, 128 ** -0.5, cu=cu, kernel=kernel)
     # (`large` stands behind no visible key: the bound on the scores is that of the others)
     q4_util.check(got, exact)
+
+
+@pytest.mark.parametrize("dtype,E", [(torch.bfloat16, 128), (torch.float16, 128), (torch.float16, 64), (torch.float32, 64)])
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("F", [1, 2])
+def test_infinite_queries_are_nan_by_every_kernel(A, dtype, E, kernel, F):
+    """A row whose query holds an infinity is NaN where it sees a key, whichever sign its scores have; alone, in a chunk, over two fragments."""
+    skip_unless_eligible(kernel, dtype, E, E, True, 16)
+    cache, gen = small_cache(42, 24, 2, 16, E)
+    table = torch.arange(24, dtype=torch.int32).reshape(2, 12)
+    T, cu = 150, torch.tensor([0, 149, 150], dtype=torch.int32)
+    q = torch.randn(F, T, 8, E, generator=gen).to(dtype)
+    loc = torch.from_numpy(np.random.default_rng(42).integers(-1, 190, (F, T)).astype(np.int32))
+    for row, value, seen in ((3, float("inf"), 0), (4, -float("inf"), 0), (60, float("inf"), 150), (61, -float("inf"), 150), (100, float("nan"), 5),
+                             (149, -float("inf"), 0), (90, float("inf"), -1), (91, float("nan"), -1)):
+        q[F - 1, row, :, 3] = value
+        loc[F - 1, row] = seen
+        if F == 2:
+            loc[0, row] = 20 if row != 149 else -1               # (the other fragment's rows are ordinary ones)
+    lens = torch.tensor([[192, 192]] * F, dtype=torch.int32)
+    got, exact = paged(A, q, loc, lens, cache, table, E ** -0.5, cu=cu, kernel=kernel)
+    bad = [3, 4, 60, 61, 100, 149]
+    exact[0][bad] = np.nan
+    q4_util.check(got, exact)
+    assert bool(got[bad].isnan().all()) and not bool(got[[90, 91]].isnan().any())
