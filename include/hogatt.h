@@ -353,8 +353,8 @@ int hogatt_copy_to_blocks_rows_launch(const void* key_states, const void* value_
 /*
  * Attention over such a cache: hogatt_paged_sdpa_launch with key_cache / value_cache as the codes, and num_blocks given.
  * f32 / f16 / bf16 queries and outputs; E <= 256, Ev in {32, 64, 128, 256}.  `kernel`: AUTO; FMA (CUDA cores: all of those); MMA (mma.sync, f16 / bf16 with
- * E == Ev == 64 or 128: what AUTO takes there); DENSE (tcgen05, packed queries with E == Ev == 128, blocks of a multiple of 8 rows and a scale from 1e-30 to
- * 1e30: what AUTO takes for prompt chunks).  A row that sees a key is NaN where its query or the scale is no finite number; one that sees none is zero.
+ * E == Ev == 64 or 128: what AUTO takes there); DENSE (tcgen05, packed queries with E == Ev == 128, blocks of a multiple of 8 rows and scale * log2(e) * key
+ * unit from 1e-30 to 8192: what AUTO takes for prompt chunks).  A row that sees a key is NaN where its query or the scale is no finite number; one that sees none is zero.
  */
 typedef struct hogatt_paged_q4_problem {
     hogatt_paged_problem paged;

@@ -71,11 +71,17 @@ struct Q4Plan {
     size_t queries, factor;
 };
 
-// Packed queries on the tcgen05 kernel: head size 128, blocks of a multiple of eight rows.
-bool dense_eligible(const hogatt_paged_problem* p) {
+// What scores are multiplied with: the products of queries and of what the codes and scales alone stand for.
+float score_factor(const hogatt_paged_q4_problem* x) { return (float)((double)x->paged.scale * 1.4426950408889634 * x->key_unit); }
+
+// Packed queries on the tcgen05 kernel: head size 128, blocks of a multiple of eight rows.  The factor of the scores lies where neither it nor 8 / factor
+// leaves fp32, not even times the power of two, 2^-120 to 2^113, that a row of bf16 queries is scaled by (clamped at 1e-36).
+bool dense_eligible(const hogatt_paged_q4_problem* x) {
+    const hogatt_paged_problem* p = &x->paged;
+    const float factor = score_factor(x);
     return p->cu_seqlens_q != nullptr && (p->dtype == HOGATT_F16 || p->dtype == HOGATT_BF16) && p->E == 128 && p->Ev == 128 && p->block_size % 8 == 0 &&
            p->Hq / p->Hkv <= kDenseRows && (int64_t)p->num_blocks * p->Hkv * p->block_size < ((int64_t)1 << 31) &&
-           (int64_t)p->total_q_tokens * p->Hq * p->F < ((int64_t)1 << 31) && p->scale >= 1e-30f && p->scale <= 1e30f;
+           (int64_t)p->total_q_tokens * p->Hq * p->F < ((int64_t)1 << 31) && factor >= 1e-30f && factor <= 8192.f;
 }
 // AUTO takes it where the tokens beyond one per sequence, over as many keys as the block table has room for, would keep the other
 // kernel busy for long (as for 16-bit pages).
@@ -96,7 +102,7 @@ int plan_q4(const hogatt_paged_q4_problem* x, int sms, Q4Plan* pl) {
     if (p->Ev != 32 && p->Ev != 64 && p->Ev != 128 && p->Ev != 256) return HOGATT_ERR_UNSUPPORTED_HEAD_DIM;
     if (p->F > 4096) return HOGATT_ERR_TOO_MANY_FRAGMENTS;
     const bool mma = p->dtype != HOGATT_F32 && p->E == p->Ev && (p->E == 64 || p->E == 128);
-    const bool dense = dense_eligible(p);
+    const bool dense = dense_eligible(x);
     if (p->kernel != HOGATT_KERNEL_AUTO && p->kernel != HOGATT_KERNEL_FMA && !(p->kernel == HOGATT_KERNEL_MMA && mma) &&
         !(p->kernel == HOGATT_KERNEL_DENSE && dense))
         return HOGATT_ERR_BAD_KERNEL_CHOICE;
@@ -255,7 +261,7 @@ int launch_q4_dense(const hogatt_paged_q4_problem* x, const Q4Plan& pl, int dev,
     d.total_q = p->total_q_tokens;
     d.block_size = p->block_size;
     d.max_blocks = p->max_blocks_per_seq;
-    d.l2scale = (float)((double)p->scale * 1.4426950408889634 * x->key_unit);
+    d.l2scale = score_factor(x);
     d.loc = p->locations;
     d.flen = p->fragment_lengths;
     d.cu = p->cu_seqlens_q;
@@ -394,7 +400,7 @@ int hogatt_paged_q4_sdpa_launch(const hogatt_paged_q4_problem* x, hogatt_stream_
     if (rc != HOGATT_OK) return rc;
     const hogatt_paged_problem* p = &x->paged;
     if (!unit_ok(x->key_unit) || !unit_ok(x->value_unit)) return HOGATT_ERR_BAD_UNIT;
-    if (std::isfinite(p->scale) && !std::isfinite((float)((double)p->scale * 1.4426950408889634 * x->key_unit))) return HOGATT_ERR_BAD_UNIT;
+    if (std::isfinite(p->scale) && !std::isfinite(score_factor(x))) return HOGATT_ERR_BAD_UNIT;
     if (!p->out || !p->queries || !p->locations || !p->fragment_lengths || !p->key_cache || !p->value_cache || !x->key_scales ||
         !x->value_scales || !p->block_table || !p->workspace)
         return HOGATT_ERR_NULL_POINTER;
@@ -420,7 +426,7 @@ int hogatt_paged_q4_sdpa_launch(const hogatt_paged_q4_problem* x, hogatt_stream_
     a.tokens_per_group = pl.tokens_per_group; a.head_blocks = pl.head_blocks; a.groups_bound = pl.groups_bound;
     a.splits = pl.splits;
     // (a scale that is no number: every score is inf - inf or 0 * inf, NaN)
-    a.l2scale = std::isfinite(p->scale) ? (float)((double)p->scale * 1.4426950408889634 * x->key_unit) : NAN;
+    a.l2scale = std::isfinite(p->scale) ? score_factor(x) : NAN;
     if (packed) {     // q [F,total_q,Hq,E], out [total_q,Hq,Ev], loc [F,total_q], len [F,W]; s is the packed token index
         a.q_f = (long long)a.total_q * p->Hq * p->E; a.q_w = 0; a.q_s = (long long)p->Hq * p->E; a.q_h = p->E;
         a.o_w = 0; a.o_s = (long long)p->Hq * p->Ev; a.o_h = p->Ev;

@@ -38,3 +38,14 @@ def test_tables_wider_than_a_row_counts_are_refused(lib, width, rc):
     import ctypes as C
     from tests.test_q4_host import _blocks
     assert lib.hogatt_step_blocks_launch(C.byref(_blocks(_cabi.StepBlocks, max_blocks=width, workspace_bytes=8)), None) == rc
+
+
+@pytest.mark.parametrize("scale,unit,rc", [(0.1, 1.0, NULL), (1e-30, 1.0, NULL), (1e-20, 2.0 ** -64, -9), (1e-30, 2.0 ** -28, -9), (1e-30, 2.0 ** 64, NULL), (5e3, 1.0, NULL),
+                                           (6e3, 1.0, -9), (0.1, 2.0 ** 20, -9), (1e25, 2.0 ** -63, -9), (float("nan"), 1.0, -9), (float("inf"), 1.0, -9),
+                                           (0.0, 1.0, -9), (-0.1, 1.0, -9)])
+def test_the_chunks_kernel_goes_by_scale_times_unit(lib, scale, unit, rc):
+    """Asked for by name where it is refused; where it is not, the missing output is what is refused."""
+    import ctypes as C
+    from tests.test_q4_host import _paged
+    x = _paged(kernel=4, cu_seqlens_q=4096, total_q_tokens=4, scale=scale, key_unit=unit, out=None)
+    assert lib.hogatt_paged_q4_sdpa_launch(C.byref(x), None) == rc

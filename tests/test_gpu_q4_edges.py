@@ -88,3 +88,21 @@ def test_infinite_queries_are_nan_by_every_kernel(A, dtype, E, kernel, F):
     exact[0][bad] = np.nan
     q4_util.check(got, exact)
     assert bool(got[bad].isnan().all()) and not bool(got[[90, 91]].isnan().any())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("scale,unit,size", [(1e-30, 2.0 ** -64, 1.0), (1e-30, 2.0 ** -28, 1.0), (1e-12, 2.0 ** -40, 1.0), (2e3, 2.0 ** -12, 0.5), (0.088, 2.0 ** -20, 10000.0),
+                                             (1e20, 2.0 ** -63, 0.3), (1e-30, 2.0 ** 64, 0.1), (3e-4, 2.0 ** 20, 2.0 ** -10)])
+def test_scales_and_units_of_a_chunk(A, dtype, scale, unit, size):
+    """A chunk large enough for the kernel that chunks take by themselves, scale times unit from one end of its range to the other."""
+    cache, gen = small_cache(44, 40, 2, 8, 128)                  # (codes and scales; what they stand for goes by the unit)
+    W, width = 2, 480
+    table = torch.full((W, width), -1, dtype=torch.int32)
+    table[:, :20] = torch.randperm(40, generator=gen).to(torch.int32).reshape(W, 20)
+    T, cu = 161, torch.tensor([0, 160, 161], dtype=torch.int32)
+    assert (T - W) * 8 * width * 8 >= 4.5e6
+    q = (torch.randn(1, T, 8, 128, generator=gen) * size).to(dtype)
+    loc = torch.cat([torch.arange(160), torch.tensor([159])]).to(torch.int32)[None]
+    loc[0, 5] = -1
+    got, exact = paged(A, q, loc, torch.tensor([[160, 155]], dtype=torch.int32), cache, table, scale, (unit, 1.0), cu=cu)
+    q4_util.check(got, exact)
