@@ -1075,7 +1075,8 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
                         }
                     }
                 }
-                const float bias = (m_run == -INFINITY) ? 0.f : -m_run * scale2;
+                // (Q4: fp16 probabilities of up to 2^15 instead of 2^8, so that small ones beside them do not leave its range)
+                const float bias = (m_run == -INFINITY) ? 0.f : (Q4 ? 7.f : 0.f) - m_run * scale2;
                 const uint64_t scale_pair = pair_f32(scale2, scale2), bias_pair = pair_f32(bias, bias);
                 uint64_t sum[2] = {0ull, 0ull};                             // (two fp32 zeros each)
 #pragma unroll

@@ -18,8 +18,11 @@
 // P goes from the accumulators of the first product to the B operand of the second by movmatrix.
 //
 // Every warp works alone: 16 keys of each 128-key tile, fetched by its own cp.async copies into its own ring, its own running maximum and
-// sum; the eight (or four) warps meet only where a unit ends.  Rows are looked up in the block table one tile ahead of their copies.  O is
-// rescaled only when some score exceeds the row's reference by 2^7 (P then stays below 128 in fp16).
+// sum; the eight (or four) warps meet only where a unit ends.  Rows are looked up in the block table one tile ahead of their copies.
+//
+// P in fp16: a row's reference lies 2^8 below its maximum and O is rescaled only when some score exceeds it by 2^15, so the largest probability stands
+// between 2^8 and 2^15, and fp16's 11 bits reach down to 2^-22 of it, its last one to 2^-32.  (With the maximum itself as the reference all keys
+// below 2^-25 of the largest were lost: beside a key that takes nearly all of the weight, thousands of others count together.)
 //
 // Split: units (<= 16 query rows that share keys, kv head) are cut into 128-key tiles, all units' tiles are one list, every CTA takes an
 // equal contiguous share (two CTAs per SM), in which a unit's start and end count as some tiles.  A share's part of a unit is a partial; q4_mma_merge_kernel adds them up.  With as many units as
@@ -34,6 +37,7 @@
 namespace hogatt {
 
 constexpr int kQ4Ctas = 2;       // resident CTAs of eight warps per SM (four of four warps)
+constexpr float kQ4RefBelow = 8.f, kQ4RefAbove = 15.f;      // powers of two: a row's reference below its maximum, a score above it that moves it
 
 struct Q4MmaArgs {
     PagedArgs p;                  // kcache / vcache: the codes; splits: unused; groups_bound: entries of the prefix
@@ -582,13 +586,13 @@ __global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) grow = grow || fmaxf(c[n][i], c[n][i + 2]) * factor[n][i] > m[n][i] + 7.f;
-                if (__any_sync(0xffffffffu, grow)) {      // (rare behind the first tiles) every row's reference becomes its maximum so far
+                    for (int i = 0; i < 2; ++i) grow = grow || fmaxf(c[n][i], c[n][i + 2]) * factor[n][i] > m[n][i] + kQ4RefAbove;
+                if (__any_sync(0xffffffffu, grow)) {      // (rare behind the first tiles) every row's reference follows its maximum so far
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            float top = fmaxf(m[n][i], fmaxf(c[n][i], c[n][i + 2]) * factor[n][i]);
+                            float top = fmaxf(m[n][i], fmaf(fmaxf(c[n][i], c[n][i + 2]), factor[n][i], -kQ4RefBelow));
 #pragma unroll
                             for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
                             const float down = exp2_fast(m[n][i] - top);

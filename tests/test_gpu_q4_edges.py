@@ -106,3 +106,40 @@ def test_scales_and_units_of_a_chunk(A, dtype, scale, unit, size):
     loc[0, 5] = -1
     got, exact = paged(A, q, loc, torch.tensor([[160, 155]], dtype=torch.int32), cache, table, scale, (unit, 1.0), cu=cu)
     q4_util.check(got, exact)
+
+
+def fine_tolerance(dtype, ref, weight, top, keys, vmax):
+    """q4_util.tolerance with what the tensor-core kernels hold of small probabilities: the row's largest one stands at 2^7 or more of fp16's
+    range, so a probability below 2^-14 is off by at most 2^-25 / 2^7 of the largest one (instead of 2^-25).  `keys`: per key that is as large."""
+    p = 2 * (259 * 2.0 ** -23 * top + 4 * 2.0 ** -23) + 2 * keys * 2.0 ** -23 + (0 if dtype == torch.float32 else 2.0 ** -11)
+    return q4_util.HALF_STEP[dtype] * np.abs(ref) + p * weight + keys * 2.0 ** -32 * vmax + (2.0 ** -25 if dtype == torch.float16 else 1e-30)
+
+
+@pytest.mark.parametrize("dtype,E", [(torch.bfloat16, 128), (torch.float16, 128), (torch.bfloat16, 64), (torch.float32, 64)])
+@pytest.mark.parametrize("G", [2, 12])
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_small_probabilities_beside_large_ones(A, dtype, E, G, many, kernel):
+    """One key, or one of every sixteen, has nearly all of a row's weight and values of zero: the output is what the others add up to, 2^-25 of it each."""
+    skip_unless_eligible(kernel, dtype, E, E, True, 16)
+    gen = torch.Generator().manual_seed(45)
+    bs, blocks, keys, T, unit = 16, 20, 3000, 40, 1024.0
+    k, v = torch.zeros(blocks, 1, bs, E), unit * (1 + torch.randint(0, 4, (blocks, 1, bs, E), generator=gen) * 0.5)
+    heavy = slice(0, blocks if many else 1)
+    k[heavy, 0, 3, 0], v[heavy, 0, 3] = 6.0, 0.0
+    k[..., 16:] = torch.where(torch.rand(blocks, 1, bs, E - 16, generator=gen) < 0.5, 0.25, -0.25)
+    (kc, ks), (vc, vs) = q4_util.quantise(k, 1.0), q4_util.quantise(v, unit)
+    table = torch.from_numpy(np.random.default_rng(45).integers(1, blocks, (1, 188)).astype(np.int32))
+    table[0, 5] = 0                                          # (key 83 is the heavy one, where there is one)
+    q = torch.zeros(1, T, G, E)
+    q[..., 0] = 25.5 * np.log(2) / 6.0 * 8
+    q[..., 16:] = torch.randn(1, T, G, E - 16, generator=gen) * 0.5
+    loc = torch.from_numpy(np.random.default_rng(46).integers(100, keys, (1, T)).astype(np.int32))
+    loc[0, 0] = keys - 1
+    got, exact = paged(A, q.to(dtype), loc, torch.tensor([[keys]], dtype=torch.int32), [kc, vc, ks, vs], table, 0.125, (1.0, unit),
+                       cu=torch.tensor([0, T], dtype=torch.int32), kernel=kernel)
+    ref, weight, top, _, vmax = exact
+    assert 1e-4 < np.abs(ref).max() < 1.0
+    # (at least six large ones among the first 101 keys: no more than 32 keys for each)
+    far = np.abs(got.cpu().double().numpy() - ref) / fine_tolerance(dtype, ref, weight, top, 32 if many else keys, vmax)
+    assert far.max() <= 1.0, f"{far.max():.2f} times the tolerance"
