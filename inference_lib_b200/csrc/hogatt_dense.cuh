@@ -1075,9 +1075,11 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
                         }
                     }
                 }
-                // (Q4: fp16 probabilities of up to 2^15 instead of 2^8, so that small ones beside them do not leave its range)
-                const float bias = (m_run == -INFINITY) ? 0.f : (Q4 ? 7.f : 0.f) - m_run * scale2;
+                // Q4: fp16 probabilities of up to 2^15 instead of 2^8, so that small ones beside them do not leave its range; and the difference first,
+                // then the scale, so that scores beyond 2^27 are not left with the rounding of their maximum times the scale
+                const float shift = (m_run == -INFINITY) ? 0.f : -m_run, bias = Q4 ? 7.f : shift * scale2;
                 const uint64_t scale_pair = pair_f32(scale2, scale2), bias_pair = pair_f32(bias, bias);
+                [[maybe_unused]] const uint64_t shift_pair = pair_f32(shift, shift);
                 uint64_t sum[2] = {0ull, 0ull};                             // (two fp32 zeros each)
 #pragma unroll
                 for (int c = 0; c < COLS / 32; ++c) {
@@ -1085,7 +1087,9 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         float x0, x1;
-                        unpair_f32(fma2(pair_f32(s[c * 32 + 2 * k], s[c * 32 + 2 * k + 1]), scale_pair, bias_pair), x0, x1);
+                        uint64_t z = pair_f32(s[c * 32 + 2 * k], s[c * 32 + 2 * k + 1]);
+                        if constexpr (Q4) z = add2(z, shift_pair);
+                        unpair_f32(fma2(z, scale_pair, bias_pair), x0, x1);
                         x0 = fast_exp2(x0);
                         x1 = fast_exp2(x1);
                         sum[k & 1] = add2(sum[k & 1], pair_f32(x0, x1));

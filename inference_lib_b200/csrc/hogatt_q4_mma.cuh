@@ -582,17 +582,21 @@ __global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel
                             if (k0 + key >= lim[n][i & 1] || (bad >> key & 1)) c[n][i] = -INFINITY;
                         }
                 }
+                // (scores rounded in front of the difference: fused, the rounding of m would be what is left of scores beyond 2^27)
                 bool grow = false;
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) grow = grow || fmaxf(c[n][i], c[n][i + 2]) * factor[n][i] > m[n][i] + kQ4RefAbove;
+                    for (int i = 0; i < 4; ++i) c[n][i] = __fmul_rn(c[n][i], factor[n][i & 1]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) grow = grow || fmaxf(c[n][i], c[n][i + 2]) > m[n][i] + kQ4RefAbove;
+                }
                 if (__any_sync(0xffffffffu, grow)) {      // (rare behind the first tiles) every row's reference follows its maximum so far
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            float top = fmaxf(m[n][i], fmaf(fmaxf(c[n][i], c[n][i + 2]), factor[n][i], -kQ4RefBelow));
+                            float top = fmaxf(m[n][i], fmaxf(c[n][i], c[n][i + 2]) - kQ4RefBelow);
 #pragma unroll
                             for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
                             const float down = exp2_fast(m[n][i] - top);
@@ -609,7 +613,7 @@ __global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) c[n][i] = exp2_fast(fmaf(c[n][i], factor[n][i & 1], -m[n][i & 1]));
+                    for (int i = 0; i < 4; ++i) c[n][i] = exp2_fast(c[n][i] - m[n][i & 1]);
                     l[n][0] += c[n][0] + c[n][2];
                     l[n][1] += c[n][1] + c[n][3];
                     pb[n][0] = movmatrix(pack2<__half>(c[n][0], c[n][1]));

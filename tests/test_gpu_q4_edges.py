@@ -143,3 +143,61 @@ def test_small_probabilities_beside_large_ones(A, dtype, E, G, many, kernel):
     # (at least six large ones among the first 101 keys: no more than 32 keys for each)
     far = np.abs(got.cpu().double().numpy() - ref) / fine_tolerance(dtype, ref, weight, top, 32 if many else keys, vmax)
     assert far.max() <= 1.0, f"{far.max():.2f} times the tolerance"
+
+
+@pytest.mark.parametrize("dtype,size", [(torch.bfloat16, 2.0 ** 16), (torch.bfloat16, 2.0 ** 27), (torch.bfloat16, 2.0 ** 70), (torch.float16, 2.0 ** 15)])
+@pytest.mark.parametrize("E", [128, 64])
+@pytest.mark.parametrize("G", [2, 12])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_scores_beyond_what_an_exponent_resolves(A, dtype, size, E, G, kernel):
+    """Scores of 2^27 and far beyond, some below zero: the key with the largest one has all of the weight."""
+    skip_unless_eligible(kernel, dtype, E, E, True, 16)
+    gen, rng = torch.Generator().manual_seed(47), np.random.default_rng(47)
+    bs, blocks, T = 16, 12, 140
+    k = torch.zeros(blocks, 1, bs, E)
+    k[..., 0] = torch.tensor([6.0, 4, 3, 2, 1.5, 1, 0.5, 0, -6])[torch.randint(0, 9, (blocks, 1, bs), generator=gen)]
+    scales = 2.0 ** torch.randint(-3, 9, (blocks, 1, bs, 1), generator=gen)          # (powers of two times 1.5 at most: rows differ by a quarter or are equal)
+    (kc, ks), (vc, vs) = q4_util.quantise(k * scales, 1.0), q4_util.random_cache(gen, blocks, 1, bs, E)
+    table = torch.randperm(blocks, generator=gen).to(torch.int32)[None]
+    q = torch.zeros(1, T, G, E)
+    q[..., 0] = size
+    q[0, ::3, :, 0] = -size
+    loc = torch.from_numpy(rng.integers(0, 192, (1, T)).astype(np.int32))
+    got, _ = paged(A, q.to(dtype), loc, torch.tensor([[192]], dtype=torch.int32), [kc, vc, ks, vs], table, 1.0, cu=torch.tensor([0, T], dtype=torch.int32), kernel=kernel)
+    key = q4_util.sequence(kc, ks, 1.0, table[0], 192)[0][0, :, 0]
+    val = q4_util.sequence(vc, vs, 1.0, table[0], 192)[0][0]
+    for i in range(T):
+        z = key[:int(loc[0, i]) + 1] * (-1 if i % 3 == 0 else 1)
+        want = val[:len(z)][z == z.max()].mean(0)                # (equal keys share; the next one is 2^15 / 16 or more behind)
+        assert np.abs(got[i].cpu().double().numpy() - want).max() <= (q4_util.HALF_STEP[dtype] + 2.0 ** -11 + 200 * 2.0 ** -23) * np.abs(val).max(), i
+
+
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 60, 2.0 ** 100])
+@pytest.mark.parametrize("first", [0, 1])
+@pytest.mark.parametrize("G", [2, 12])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_fragments_whose_scores_lie_far_apart(A, size, first, G, kernel):
+    """One fragment's scores are ordinary, the other's so large that they take all of the weight or none of it; equal ones share."""
+    gen, rng = torch.Generator().manual_seed(48), np.random.default_rng(48)
+    bs, blocks, T, E = 16, 24, 140, 128
+    k = torch.zeros(blocks, 1, bs, E)
+    k[..., 0] = torch.tensor([6.0, 3, 1, 0.5, 0, -1, -6])[torch.randint(0, 7, (blocks, 1, bs), generator=gen)]
+    k[:14, ..., 0] = -k[:14, ..., 0].abs()                       # (rows that see few keys: none above zero)
+    (kc, ks), (vc, vs) = q4_util.quantise(k, 1.0), q4_util.random_cache(gen, blocks, 1, bs, E)
+    table = torch.arange(blocks, dtype=torch.int32)[None]
+    q = torch.zeros(2, T, G, E)
+    q[first, ..., 0], q[1 - first, ..., 0] = size, 0.25
+    loc = torch.from_numpy(rng.integers(-1, blocks * bs, (2, T)).astype(np.int32))
+    lens = torch.full((2, 1), blocks * bs, dtype=torch.int32)
+    got, _ = paged(A, q.bfloat16(), loc, lens, [kc, vc, ks, vs], table, 1.0, cu=torch.tensor([0, T], dtype=torch.int32), kernel=kernel)
+    key, val = (q4_util.sequence(*x, 1.0, table[0], blocks * bs)[0][0] for x in ((kc, ks), (vc, vs)))
+    for i in range(T):
+        n = [int(x) + 1 for x in loc[:, i]]
+        z = np.concatenate([key[:n[f], 0] * (size if f == first else 0.25) for f in range(2)])
+        if not len(z):
+            assert bool((got[i] == 0).all())
+            continue
+        p = np.exp(z - z.max())
+        want = (p[:, None] * np.concatenate([val[:x] for x in n])).sum(0) / p.sum()
+        # the output's rounding, the probabilities' in fp16 and what 768 keys' sums and scores below 2^4 add in fp32
+        assert np.abs(got[i].cpu().double().numpy() - want).max() <= (2.0 ** -8 + 2.0 ** -11 + 2 * 800 * 2.0 ** -23) * np.abs(val).max(), i
