@@ -201,3 +201,91 @@ def test_fragments_whose_scores_lie_far_apart(A, size, first, G, kernel):
         want = (p[:, None] * np.concatenate([val[:x] for x in n])).sum(0) / p.sum()
         # the output's rounding, the probabilities' in fp16 and what 768 keys' sums and scores below 2^4 add in fp32
         assert np.abs(got[i].cpu().double().numpy() - want).max() <= (2.0 ** -8 + 2.0 ** -11 + 2 * 800 * 2.0 ** -23) * np.abs(val).max(), i
+
+
+LONG = [
+    # sequences of keys (one token each), Hkv, G, E, bs, kernel: what runs
+    ([9000], 1, 4, 128, 16, 2),                    # shares of one unit: many partials, the merge step's second round
+    ([40000], 1, 8, 64, 32, 2),
+    ([70000, 33], 1, 12, 128, 16, 2),              # sixteen rows; more than 32 tiles of a share: the second window of page numbers
+    ([150001], 2, 2, 64, 64, 2),
+    ([30000, 9000, 129], 2, 4, 128, 8, 2),         # rows looked up one by one
+    ([4300] * 75, 4, 4, 128, 16, 2),               # units with a CTA each
+    ([2300] * 3 + [100] * 220, 4, 2, 64, 16, 2),   # four warps a CTA
+    ([5000, 4096, 4097], 1, 2, 128, 16, 1),        # CUDA cores
+]
+
+
+def long_exact(q, lens, cache, table, scale, bs):
+    """Output and what bounds its error, like q4_util.attention, for single tokens that see all keys, with whole arrays."""
+    kc, vc, ks, vs = cache
+    K, V = q4_util.values(kc, ks, 1.0), q4_util.values(vc, vs, 1.0)
+    W, Hq, E = q.shape
+    Hkv = kc.shape[1]
+    out, weight, top = np.zeros((W, Hq, V.shape[-1])), np.zeros((W, Hq, V.shape[-1])), 0.0
+    qd = q.double().numpy().reshape(W, Hkv, Hq // Hkv, E)
+    for w, n in enumerate(lens):
+        pages = table[w, :-(-n // bs)].numpy()
+        k, v = (x[pages].transpose(1, 0, 2, 3).reshape(Hkv, -1, E)[:, :n] for x in (K, V))
+        z = np.einsum("hge,hle->hgl", qd[w], k) * scale
+        top = max(top, float(np.einsum("hge,hle->hgl", np.abs(qd[w]), np.abs(k)).max() * scale))
+        p = np.exp(z - z.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        out[w], weight[w] = (np.einsum("hgl,hle->hge", p, x).reshape(Hq, E) for x in (v, np.abs(v)))
+    return out, weight, top, max(lens), float(np.abs(V).max())
+
+
+@pytest.mark.parametrize("case", LONG, ids=[str(i) for i in range(len(LONG))])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_long_sequences(A, case, dtype):
+    """Few pages under many table entries; a loud key now and then, so that the rows' references move."""
+    lens, Hkv, G, E, bs, kernel = case
+    gen, rng = torch.Generator().manual_seed(sum(lens)), np.random.default_rng(sum(lens))
+    W, blocks, width = len(lens), 53, -(-max(lens) // bs)
+    cache = [x for pair in zip(*(q4_util.random_cache(gen, blocks, Hkv, bs, E) for _ in range(2))) for x in pair]
+    table = torch.from_numpy(rng.integers(0, blocks - 1, (W, width)).astype(np.int32))
+    cache[2][blocks - 1] += 12                               # (a page of keys that are larger by half an exponent: far back, once)
+    table[:, width * 3 // 4] = blocks - 1
+    q = torch.randn(1, W, Hkv * G, 1, E, generator=gen).to(dtype)
+    exact = long_exact(q[0, :, :, 0], lens, cache, table, E ** -0.5, bs)
+    dc = dev(*cache)
+    from inference_lib_b200 import _cabi
+    out = torch.full((W, Hkv * G, E), float("nan"), dtype=dtype, device=DEV)
+    ints = dev(torch.tensor([[n - 1 for n in lens]], dtype=torch.int32), table, torch.tensor([lens], dtype=torch.int32), torch.arange(W + 1, dtype=torch.int32))
+    x, keep = _cabi.bind_paged_q4(out=out, queries=q[:, :, :, 0].contiguous().to(DEV), locations=ints[0], key_cache=dc[0], value_cache=dc[1], key_scales=dc[2].view(E4M3),
+                                  value_scales=dc[3].view(E4M3), block_table=ints[1], scale=E ** -0.5, fragment_lengths=ints[2], cu_seqlens_q=ints[3], kernel=kernel)
+    keep[0].fill_(0xFF)
+    assert _cabi.launch_paged_q4(x, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    q4_util.check(out, exact)
+    # the fixed layout, where every sequence has as many
+    if len(set(lens)) == 1:
+        got = A.hogwild_paged_sdpa_q4(q.to(DEV), ints[0][..., None], dc[0], dc[1], dc[2].view(E4M3), dc[3].view(E4M3), ints[1], E ** -0.5, ints[2][0, :1])
+        q4_util.check(got[:, :, 0], exact)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("counts,keys", [([130], 9000), ([33, 257, 1], 5000)])
+def test_chunks_behind_long_sequences(A, dtype, counts, keys):
+    """A chunk's rows at the end of thousands of keys, on the kernel that chunks take."""
+    gen, rng = torch.Generator().manual_seed(keys), np.random.default_rng(keys)
+    Hkv, G, E, bs, blocks, W = 1, 4, 128, 16, 53, len(counts)
+    cache = [x for pair in zip(*(q4_util.random_cache(gen, blocks, Hkv, bs, E) for _ in range(2))) for x in pair]
+    table = torch.from_numpy(rng.integers(0, blocks, (W, -(-keys // bs))).astype(np.int32))
+    rows = [(w, keys - n + i) for w, n in enumerate(counts) for i in range(n)]
+    q = torch.randn(1, len(rows), Hkv * G, E, generator=gen).to(dtype)
+    cu = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32)
+    loc = torch.tensor([[p for _, p in rows]], dtype=torch.int32)
+    st = status()
+    got = torch.empty(len(rows), Hkv * G, E, dtype=dtype, device=DEV)
+    from inference_lib_b200 import _cabi
+    dc = dev(*cache)
+    x, keep = _cabi.bind_paged_q4(out=got, queries=q.to(DEV), locations=loc.to(DEV), key_cache=dc[0], value_cache=dc[1], key_scales=dc[2].view(E4M3),
+                                  value_scales=dc[3].view(E4M3), block_table=table.to(DEV), scale=E ** -0.5, fragment_lengths=torch.tensor([[keys] * W], dtype=torch.int32, device=DEV),
+                                  cu_seqlens_q=cu.to(DEV), kernel=4, status=st)
+    assert _cabi.launch_paged_q4(x, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    some = sorted({0, 1, len(rows) - 1, *(int(i) for i in rng.integers(0, len(rows), 12))})
+    exact = long_exact(q[0, some], [rows[i][1] + 1 for i in some], cache, table[[rows[i][0] for i in some]], E ** -0.5, bs)
+    q4_util.check(got[some], exact)
+    assert int(st) == 0 and bool(got.isfinite().all())
