@@ -207,11 +207,12 @@ LONG = [
     # sequences of keys (one token each), Hkv, G, E, bs, kernel: what runs
     ([9000], 1, 4, 128, 16, 2),                    # shares of one unit: many partials, the merge step's second round
     ([40000], 1, 8, 64, 32, 2),
-    ([70000, 33], 1, 12, 128, 16, 2),              # sixteen rows; more than 32 tiles of a share: the second window of page numbers
+    ([70000, 33], 1, 12, 128, 16, 2),              # sixteen rows
     ([150001], 2, 2, 64, 64, 2),
     ([30000, 9000, 129], 2, 4, 128, 8, 2),         # rows looked up one by one
-    ([4300] * 75, 4, 4, 128, 16, 2),               # units with a CTA each
-    ([2300] * 3 + [100] * 220, 4, 2, 64, 16, 2),   # four warps a CTA
+    ([1300003], 1, 2, 64, 64, 2),                  # more than 32 tiles of a share: the second window of page numbers
+    ([4300] * 75, 4, 4, 128, 16, 2),               # units with a CTA each, 34 tiles
+    ([2300] * 3 + [100] * 220, 4, 2, 64, 16, 2),   # four warps a CTA, 36 tiles
     ([5000, 4096, 4097], 1, 2, 128, 16, 1),        # CUDA cores
 ]
 
