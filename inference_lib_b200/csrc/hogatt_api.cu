@@ -1209,7 +1209,7 @@ const char* hogatt_status_string(int status) {
         case HOGATT_ERR_BAD_KERNEL_CHOICE: return "the requested kernel cannot run this dtype / head size";
         case HOGATT_ERR_TOO_LARGE: return "problem too large for 32-bit row indexing";
         case HOGATT_ERR_EXCEEDS_STATIC_SCRATCH: return "problem needs more scratch than the fixed HOGATT_STATIC_SCRATCH_BYTES array of hogatt_fused_launch_static; use hogatt_fused_launch with a caller workspace";
-        case HOGATT_ERR_BAD_UNIT: return "a 4-bit cache's unit is not a power of two between 2^-64 and 2^64";
+        case HOGATT_ERR_BAD_UNIT: return "a 4-bit cache's unit is not a power of two between 2^-64 and 2^64, or takes scale * log2(e) * unit out of fp32";
     }
     return "unknown status";
 }

@@ -49,3 +49,8 @@ def test_the_chunks_kernel_goes_by_scale_times_unit(lib, scale, unit, rc):
     from tests.test_q4_host import _paged
     x = _paged(kernel=4, cu_seqlens_q=4096, total_q_tokens=4, scale=scale, key_unit=unit, out=None)
     assert lib.hogatt_paged_q4_sdpa_launch(C.byref(x), None) == rc
+
+
+def test_the_unit_error_names_both_of_its_causes(lib):
+    text = lib.hogatt_status_string(-12).decode()
+    assert "power of two" in text and "scale" in text
