@@ -44,6 +44,10 @@ struct PagedArgs {
     int* status;              // optional
 };
 
+// The page of entry `i` of a sequence's table.  A length beyond the table and an entry of -1 (page bookkeeping leaves it where a sequence has no page)
+// are the caller's error in what a row may see; the reads stay inside the table and the cache regardless.
+__device__ __forceinline__ int page_at(const int* table, int i, int max_blocks) { return max(0, table[min(i, max_blocks - 1)]); }
+
 // Which worker and which of its token groups a global group index is.  Linear scan over workers
 // (the reference does the same per CTA, src/kernels/kernel_v21.cuh:15-23).  Returns false past the end.
 struct PagedUnit {
@@ -164,7 +168,7 @@ __global__ void __launch_bounds__(kFmaThreads) paged_attention_kernel(const __gr
                 const int tok = i / kvr, c = i - tok * kvr;
                 if (tok < ntok) {
                     const int l = tok0 + tok;
-                    const size_t row = ((size_t)table[min(l / a.block_size, a.max_blocks - 1)] * a.Hkv + u.hkv) * a.block_size + l % a.block_size;
+                    const size_t row = ((size_t)page_at(table, l / a.block_size, a.max_blocks) * a.Hkv + u.hkv) * a.block_size + l % a.block_size;
                     const int4 raw = load_16(static_cast<const T*>(a.kcache) + row * E + c * VEC);
                     const T* x = reinterpret_cast<const T*>(&raw);
 #pragma unroll
@@ -176,7 +180,7 @@ __global__ void __launch_bounds__(kFmaThreads) paged_attention_kernel(const __gr
                 int4 raw = make_int4(0, 0, 0, 0);                     // rows past the tile end must be finite
                 if (tok < ntok) {
                     const int l = tok0 + tok;
-                    const size_t row = ((size_t)table[min(l / a.block_size, a.max_blocks - 1)] * a.Hkv + u.hkv) * a.block_size + l % a.block_size;
+                    const size_t row = ((size_t)page_at(table, l / a.block_size, a.max_blocks) * a.Hkv + u.hkv) * a.block_size + l % a.block_size;
                     raw = load_16(static_cast<const T*>(a.vcache) + row * EV + c * VEC);
                 }
                 const T* x = reinterpret_cast<const T*>(&raw);
@@ -303,9 +307,8 @@ __global__ void __launch_bounds__(PagedMmaCfg<HD, BULK, NS>::THREADS, BULK && NS
             while (t >= pre[f + 1]) ++f;
             const int tok0 = (t - pre[f]) * C::TILE;
             ntok_next = min(C::TILE, vis[f] - tok0);
-            // (a length beyond the block table is the caller's error; the lookup stays inside the table regardless)
             const int l = tok0 + min((lane & 7) * 8, ntok_next - 1), blk = l / a.block_size;
-            row_next = ((long long)table[min(blk, a.max_blocks - 1)] * a.Hkv + u.hkv) * a.block_size + (l - blk * a.block_size);
+            row_next = ((long long)page_at(table, blk, a.max_blocks) * a.Hkv + u.hkv) * a.block_size + (l - blk * a.block_size);
         };
         if (t0 < t1) look_up(t0);
         int issued = 0;
@@ -347,8 +350,7 @@ __global__ void __launch_bounds__(PagedMmaCfg<HD, BULK, NS>::THREADS, BULK && NS
             const int tok = warp * RW + (j % RW) + (j / RW) * RP;
             const int l = tok0 + (tok < ntok ? tok : 0);
             const int blk = l / a.block_size;
-            // (a length beyond the block table is the caller's error; the lookup stays inside the table regardless)
-            mine = ((long long)table[min(blk, a.max_blocks - 1)] * a.Hkv + u.hkv) * a.block_size + (l - blk * a.block_size);
+            mine = ((long long)page_at(table, blk, a.max_blocks) * a.Hkv + u.hkv) * a.block_size + (l - blk * a.block_size);
         }
         const int c = lane % CPR, sub = lane / CPR;
 #pragma unroll

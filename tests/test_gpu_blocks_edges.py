@@ -104,3 +104,33 @@ def test_a_length_below_zero_in_place(A):
     rng = np.random.default_rng(12)
     refs, table = pool(rng, 20, 4, 5, [7, 0, 9])
     run_step(A, refs, table, [7, -3, 9], None, [1, 2, 0], 4, some_caches(rng, 20), out=lambda a: (a[0], a[1], a[2], ints([7] * 3)))
+
+
+@pytest.mark.parametrize("dtype,G,E,bs,packed", [(torch.bfloat16, 4, 128, 16, False), (torch.float16, 2, 64, 12, False), (torch.float32, 2, 64, 8, False),
+                                                 (torch.bfloat16, 4, 128, 16, True), (torch.float16, 16, 128, 8, False)])
+def test_sixteen_bit_reads_stay_inside_the_cache(A, dtype, G, E, bs, packed):
+    """Rows that see keys of pages that are not there are the caller's error: what they hold is not defined, but it comes from the cache, and other rows are
+    as they would be beside any table."""
+    gen = torch.Generator().manual_seed(53)
+    Hkv, blocks, width, W = 2, 40, 20, 3
+    around = [torch.full((blocks + 200, Hkv, bs, E), float("nan"), dtype=dtype, device=DEV) for _ in range(2)]
+    caches = [a[200:] for a in around]
+    for c in caches:
+        c.copy_(torch.randn(c.shape, generator=gen).to(dtype))
+    table = torch.randperm(blocks, generator=gen).to(torch.int32)[:width].repeat(W, 1)
+    bad = table.clone()
+    bad[1, 2], bad[1, 7:] = -1, -1
+    keys = width * bs
+    if packed:
+        counts = [1, 300, 1]
+        cu = ints([0, 1, 301, 302])
+        q = torch.randn(1, 302, Hkv * G, E, generator=gen).to(dtype).to(DEV)
+        loc, lens = torch.full((1, 302), keys - 1, dtype=torch.int32, device=DEV), ints([[keys] * W])
+        outs = [A.hogwild_varlen_paged_sdpa(q, loc, *caches, t.to(DEV), 0.1, lens, cu) for t in (table, bad)]
+        good = [0, 301]
+    else:
+        q = torch.randn(1, W, Hkv * G, 1, E, generator=gen).to(dtype).to(DEV)
+        loc = torch.full((1, W, 1), keys - 1, dtype=torch.int32, device=DEV)
+        outs = [A.hogwild_paged_sdpa(q, loc, *caches, t.to(DEV), 0.1, ints([keys])) for t in (table, bad)]
+        good = [0, 2]
+    assert torch.equal(outs[0][good], outs[1][good]) and bool(torch.cat(outs).isfinite().all())
