@@ -340,8 +340,8 @@ int hogatt_copy_to_blocks_rows_launch(const void* key_states, const void* value_
  *   scales e4m3  [num_blocks, Hkv, block_size, E/16]   one per 16 consecutive channels
  *   value[e] = e2m1(code[e]) * scale[e / 16] * unit
  * `unit` is a power of two between 2^-64 and 2^64 that the caller keeps for the cache's keys and for its values (HOGATT_ERR_BAD_UNIT
- * otherwise, and where attention's scale * log2(e) * key unit leaves fp32): it moves the range of the scales, 2^-9 to 448, to where the numbers are.  1 suits numbers between 0.1 and 2,688; groups
- * whose largest magnitude is below 6 * 2^-6 * unit lose precision, below 3 * 2^-9 * unit they are stored as zeros.
+ * otherwise, and where attention's scale * log2(e) * key unit leaves fp32): it moves the range of the scales, 2^-9 to 448, to where
+ * the numbers are.  1 suits numbers between 0.1 and 2,688; groups whose largest magnitude is below 6 * 2^-6 * unit lose precision, below 3 * 2^-9 * unit they are stored as zeros.
  * Writing: with a = the group's largest magnitude, scale = e4m3(a / (6 unit)), at most 448; code = e2m1(x / (scale unit)), at most 6;
  * all roundings to the nearest, ties to even, divisions in fp32.  A group that holds an infinity or a NaN gets the scale NaN, and every
  * row that sees it is NaN: in the channels of that group (values) or in all (keys).
@@ -448,7 +448,7 @@ typedef struct hogatt_block_tensors {
  *      pages (512): it and all rows behind it get none, and their tables stay as step 1 leaves them.
  * Writes refs_out, table_out [rows_out, max_blocks], lengths_out [rows_out] = the rows' lengths without the new tokens, room [rows_out].  Outputs
  * may be the inputs' buffers (refs always; table and lengths without a source).  Enqueues one kernel, one more per 128 caches when
- * there are new tokens.
+ * there are new tokens.  At most HOGATT_MAX_BLOCK_ROWS rows, fewer than 2^30 columns and 2^31 - 1 pages (HOGATT_ERR_TOO_LARGE).
  */
 typedef struct hogatt_step_blocks {
     int32_t num_blocks, block_size, max_blocks, rows_in, rows_out;

@@ -6,13 +6,15 @@
 // their scales -- exact in fp16 -- and stored where the 128-byte swizzle wants them.  Unpacking into 16-bit pages in the workspace first would
 // take four times the cache's memory.
 //
-// Bound by those two warps, which share their schedulers with the softmax warps: 2,048 tokens of 4,000 keys, 32 / 8 heads, fp16: 159 us (145
-// without the copies, 120 without the conversions, 106 without either); two chunks of 512 tokens of 6,000 keys beside six single tokens, bf16: 181 us.
+// Bound by those two warps, which share their schedulers with the softmax warps: 2,048 tokens of 4,000 keys, 32 / 8 heads, fp16: 164 us (of 159,
+// when that was measured, 145 were left without the copies, 120 without the conversions, 106 without either); two chunks of 512 tokens of 6,000
+// keys beside six single tokens, bf16: 181 us.
 // Slower: four unpacking warps of 24 (registers spill: 220 us); a third one for a quarter of both tiles, both products issued by one warp (219 us).
 // 96 registers for every thread: nothing is left to take from the other warps.
 //
 // fp16 for both products: six significant bits times a probability; bf16 queries become fp16 once per call, a power of two per row
-// taken out (q4_dense_queries_kernel), which the softmax multiplies back in.
+// taken out (q4_dense_queries_kernel), which the softmax multiplies back in.  A row's largest probability stands between 2^7 and 2^15 of fp16's range
+// (the running maximum may lag by 2^8), so that those below it keep their bits down to 2^-21 of it.
 //
 // Values that are not numbers are stored as zeros, keys without a page as zeros too; what is special about a tile travels to the softmax
 // warps in a ring of eight entries (K tiles are at most three ahead of the scores that are read), and only for such tiles they look

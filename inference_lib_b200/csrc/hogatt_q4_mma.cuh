@@ -2,8 +2,8 @@
 //
 // By its bytes bound by HBM: 9/8 byte per (key, channel) of K and V together, 144 bytes per key and kv head at head size 128, against 512 in
 // 16 bits -- so what a key costs on the SM counts: at the full copy rate an SM has to finish one every six cycles.  Bound by instruction issue:
-// 340 instructions of a warp per 16 keys, the schedulers at 62-64 %.  2 sequences of 131,072 keys, 8 kv heads of 4 heads: 76.5 us = 3.95 TB/s;
-// 24 of 6,000 keys down to 1,331, 5 heads: 40 us; 8 of 16,384 keys, 2 kv heads of 16 heads: 31.6 us, of which the walk is ten.
+// 350 instructions of a warp per 16 keys, the schedulers at 62 %.  2 sequences of 131,072 keys, 8 kv heads of 4 heads: 77.0 us = 3.92 TB/s;
+// 24 of 6,000 keys down to 1,331, 5 heads: 40 us; 8 of 16,384 keys, 2 kv heads of 16 heads: 31.7 us, of which the walk is ten.
 //
 // Both products are taken transposed, keys or value channels as the M of mma.sync m16n8k16 and up to eight query rows as its N:
 //     S^T [16 keys x 8 rows] = K [16 x E] Q^T,      O^T [E x 8 rows] += V^T [E x 16 keys] P^T
