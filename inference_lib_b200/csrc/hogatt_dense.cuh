@@ -1051,14 +1051,16 @@ dense_attention_kernel(const __grid_constant__ DenseArgs a, const __grid_constan
                 // O is stored at scale 2^(-m_run * scale2).  It is only brought to a new scale when a row's max has grown by
                 // more than a factor 2^8 (so every exponent below stays <= 8) or nothing has been accumulated yet.  Only
                 // then do the two halves of the rows need each other's maxima.
-                if (pair_any(pair_bar, mt > m_run + grow_by || !ok)) {
+                // (Q4: the difference is compared, since m_run + grow_by is rounded)
+                auto grows = [&](float x) { return Q4 ? x - m_run > grow_by : x > m_run + grow_by; };
+                if (pair_any(pair_bar, grows(mt) || !ok)) {
                     ok = !pair_any(pair_bar, !ok);
                     if (!ok) break;
                     *stat = mt;
                     named_barrier_sync(pair_bar, 64);
                     mt = fmaxf(mt, *other);
                     named_barrier_sync(pair_bar, 64);          // (read before it is written again)
-                    const bool grow = mt > m_run + grow_by;                     // (m_run = -inf: any finite max grows it)
+                    const bool grow = grows(mt);                                // (m_run = -inf: any finite max grows it)
                     const float m_new = grow ? mt : m_run;
                     const float alpha = grow ? fast_exp2((m_run - m_new) * scale2) : 1.f;      // (m_run = -inf -> 0)
                     m_run = m_new;

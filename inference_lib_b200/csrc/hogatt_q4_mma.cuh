@@ -20,8 +20,8 @@
 // Every warp works alone: 16 keys of each 128-key tile, fetched by its own cp.async copies into its own ring, its own running maximum and
 // sum; the eight (or four) warps meet only where a unit ends.  Rows are looked up in the block table one tile ahead of their copies.
 //
-// P in fp16: a row's reference lies 2^8 below its maximum and O is rescaled only when some score exceeds it by 2^15, so the largest probability stands
-// between 2^8 and 2^15, and fp16's 11 bits reach down to 2^-22 of it, its last one to 2^-32.  (With the maximum itself as the reference all keys
+// P in fp16: a row's reference lies 2^7 below its maximum and O is rescaled only when some score exceeds it by 2^15, so the largest probability stands
+// between 2^7 and 2^15, and fp16's 11 bits reach down to 2^-21 of it, its last one to 2^-31.  (With the maximum itself as the reference all keys
 // below 2^-25 of the largest were lost: beside a key that takes nearly all of the weight, thousands of others count together.)
 //
 // Split: units (<= 16 query rows that share keys, kv head) are cut into 128-key tiles, all units' tiles are one list, every CTA takes an
@@ -37,7 +37,9 @@
 namespace hogatt {
 
 constexpr int kQ4Ctas = 2;       // resident CTAs of eight warps per SM (four of four warps)
-constexpr float kQ4RefBelow = 8.f, kQ4RefAbove = 15.f;      // powers of two: a row's reference below its maximum, a score above it that moves it
+// Powers of two: a row's reference below its maximum, a score above it that moves it.  (Maxima of 2^24 and more round what is taken off: 7 becomes 8 at most, 8
+// became 16, which is beyond fp16.)
+constexpr float kQ4RefBelow = 7.f, kQ4RefAbove = 15.f;
 
 struct Q4MmaArgs {
     PagedArgs p;                  // kcache / vcache: the codes; splits: unused; groups_bound: entries of the prefix
@@ -582,14 +584,15 @@ __global__ void __launch_bounds__(WARPS * 32, kQ4Ctas * 8 / WARPS) q4_mma_kernel
                             if (k0 + key >= lim[n][i & 1] || (bad >> key & 1)) c[n][i] = -INFINITY;
                         }
                 }
-                // (scores rounded in front of the difference: fused, the rounding of m would be what is left of scores beyond 2^27)
+                // (scores rounded in front of the difference: fused, the rounding of m would be what is left of scores beyond 2^27; and the
+                // difference is compared, not m + 15, which from 2^24 on is rounded upwards)
                 bool grow = false;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) c[n][i] = __fmul_rn(c[n][i], factor[n][i & 1]);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) grow = grow || fmaxf(c[n][i], c[n][i + 2]) > m[n][i] + kQ4RefAbove;
+                    for (int i = 0; i < 2; ++i) grow = grow || fmaxf(c[n][i], c[n][i + 2]) - m[n][i] > kQ4RefAbove;
                 }
                 if (__any_sync(0xffffffffu, grow)) {      // (rare behind the first tiles) every row's reference follows its maximum so far
 #pragma unroll

@@ -290,3 +290,36 @@ def test_chunks_behind_long_sequences(A, dtype, counts, keys):
     exact = long_exact(q[0, some], [rows[i][1] + 1 for i in some], cache, table[[rows[i][0] for i in some]], E ** -0.5, bs)
     q4_util.check(got[some], exact)
     assert int(st) == 0 and bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("G", [4, 16])
+@pytest.mark.parametrize("kernel", [1, 2, 4])
+@pytest.mark.parametrize("power", [20, 24, 25, 26, 27, 28, 30])
+def test_scores_a_few_steps_apart(A, dtype, G, kernel, power):
+    """Scores of 2^power, where fp32 has steps of 2 to 128: 128 keys of them, then 128 that are j steps larger, j by row."""
+    gen = torch.Generator().manual_seed(49)
+    Hkv, E, bs, T, unit = 8, 128, 16, 300, 2.0 ** (power - 25)
+    k = torch.zeros(16, Hkv, bs, E)
+    k[..., 0], k[..., 1], k[8:, ..., 16], k[8:, ..., 17] = 1024 * unit, 1536 * unit, unit, 1.5 * unit       # (6 times the scale beside 4 times it: exact)
+    (kc, ks), (vc, vs) = q4_util.quantise(k, unit), q4_util.random_cache(gen, 16, Hkv, bs, E)
+    assert np.array_equal(q4_util.values(kc, ks, unit), k.double().numpy())
+    step = 2.0 ** (power - 23)
+    j = torch.arange(T) % 50
+    q = torch.zeros(1, T, Hkv * G, E)
+    q[..., 0], q[..., 16] = 2.0 ** 15, (j * step / unit)[None, :, None]
+    table, loc = torch.arange(16, dtype=torch.int32)[None], torch.full((1, T), 255, dtype=torch.int32)
+    dc = dev(kc, vc, ks, vs)
+    out = torch.full((T, Hkv * G, E), 7.0, dtype=dtype, device=DEV)
+    from inference_lib_b200 import _cabi
+    x, keep = _cabi.bind_paged_q4(out=out, queries=q.to(dtype).to(DEV), locations=loc.to(DEV), key_cache=dc[0], value_cache=dc[1], key_scales=dc[2].view(E4M3),
+                                  value_scales=dc[3].view(E4M3), block_table=table.to(DEV), scale=float(np.log(2)), key_unit=unit,
+                                  fragment_lengths=torch.tensor([[256]], dtype=torch.int32, device=DEV), cu_seqlens_q=torch.tensor([0, T], dtype=torch.int32, device=DEV),
+                                  kernel=kernel)
+    assert _cabi.launch_paged_q4(x, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    # (log2 e * ln 2 is 1 in fp32, and every score is a number of it)
+    v = q4_util.sequence(vc, vs, 1.0, table[0], 256)[0].repeat(G, 0)                # [Hq,256,E]
+    less = 2.0 ** -(j.double().numpy() * step)[:, None, None]
+    want = (v[None, :, :128].sum(2) * less + v[None, :, 128:].sum(2)) / (128 * (1 + less))
+    assert np.abs(out.cpu().double().numpy() - want).max() <= (q4_util.HALF_STEP[dtype] + 2.0 ** -11 + 260 * 2.0 ** -23) * np.abs(v).max()
