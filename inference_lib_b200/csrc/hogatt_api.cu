@@ -1329,7 +1329,7 @@ int hogatt_copy_to_blocks_rows_launch(const void* key_states, const void* value_
                                       int32_t max_blocks, int32_t num_blocks, int32_t dtype, hogatt_stream_t stream_) {
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
     if (!key_states || !value_states || !key_cache || !value_cache || !block_table || !seq_lengths) return HOGATT_ERR_NULL_POINTER;
-    if (B <= 0 || Hkv <= 0 || S_new < 0 || E <= 0 || Ev <= 0 || block_size <= 0 || max_blocks <= 0 || num_blocks <= 0) return HOGATT_ERR_BAD_SHAPE;
+    if (B <= 0 || Hkv <= 0 || S_new < 0 || E <= 0 || Ev <= 0 || block_size <= 0 || max_blocks <= 0 || num_blocks < 0) return HOGATT_ERR_BAD_SHAPE;
     if (dtype != HOGATT_F32 && dtype != HOGATT_F16 && dtype != HOGATT_BF16) return HOGATT_ERR_UNSUPPORTED_DTYPE;
     const int vec = 16 / (int)dtype_size(dtype);
     if (E % vec != 0 || Ev % vec != 0) return HOGATT_ERR_UNSUPPORTED_HEAD_DIM;

@@ -13,7 +13,7 @@ def lib():
 
 
 @pytest.mark.parametrize("change,rc", [
-    ({}, OK), ({0: None}, NULL), ({4: None}, NULL), ({5: None}, NULL), ({6: None}, OK), ({7: 0}, SHAPE), ({9: -1}, SHAPE), ({14: 0}, SHAPE), ({14: -3}, SHAPE),
+    ({}, OK), ({0: None}, NULL), ({4: None}, NULL), ({5: None}, NULL), ({6: None}, OK), ({7: 0}, SHAPE), ({9: -1}, SHAPE), ({14: 0}, OK), ({14: -3}, SHAPE),
     ({15: 7}, DTYPE), ({10: 60}, HEAD), ({1: 4104}, ALIGN),
 ])
 def test_append_of_rows_refuses(lib, change, rc):
