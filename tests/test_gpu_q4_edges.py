@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests import q4_util
-from tests.test_gpu_q4 import DEV, E4M3, KERNELS, A, dev, odd_scales, paged, skip_unless_eligible, status, table_of  # noqa: F401
+from tests.test_gpu_q4 import DEV, E4M3, KERNELS, A, dev, paged, skip_unless_eligible, status  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -13,11 +13,6 @@ def small_cache(seed, blocks, Hkv, bs, E, units=(1.0, 1.0)):
     gen = torch.Generator().manual_seed(seed)
     (kc, ks), (vc, vs) = q4_util.random_cache(gen, blocks, Hkv, bs, E, units[0]), q4_util.random_cache(gen, blocks, Hkv, bs, E, units[1])
     return [kc, vc, ks, vs], gen
-
-
-def sign_rows(gen, blocks, Hkv, bs, E):
-    """Codes and scales of rows of +-1."""
-    return q4_util.quantise(torch.where(torch.rand(blocks, Hkv, bs, E, generator=gen) < 0.5, 6.0, -6.0), 6.0)
 
 
 @pytest.mark.parametrize("dtype,E,G", [(torch.bfloat16, 128, 4), (torch.float16, 64, 12), (torch.float32, 128, 2)])
